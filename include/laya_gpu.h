@@ -19,6 +19,11 @@
  *   laya_gpu_forward_dumpstats  (the same, as the reference's [dump] text)
  *   laya_gpu_linear          linear16             src/main.zig:1088-1099
  *                            (checked by --selftest, main.zig:420-536)
+ *   laya_gpu_rope, laya_gpu_attention
+ *                            ropeJob, attWorker    src/main.zig:2496-2521, 2431-2489
+ *                            (by themselves and with gradients; these, the
+ *                            backward pass and the policy loss have no
+ *                            counterpart as calls in the reference)
  *
  * All pointers are plain host or device pointers; no C++ or framework types
  * cross this boundary. Every call returns a laya_status; after a failure,
@@ -257,6 +262,165 @@ LAYA_API int laya_gpu_decision_tail_noalloc(laya_ctx* ctx, const float* hidden, 
  * kernel just before. */
 LAYA_API int laya_gpu_linear(const void* x, const void* w, const float* bias, float* out, int M, int N, int K,
                     int elem_dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Operators of a training step.
+ *
+ * The forward above rotates, attends and scores inside its own kernels and
+ * keeps nothing that a gradient needs. The calls below are the same
+ * operators by themselves, with their gradients, over rows that the caller
+ * holds: rotary positions, packed attention with its statistics and its
+ * backward pass, and the policy loss over a decision's options. They need no
+ * context. Each runs on `stream` (NULL = the legacy default stream) of the
+ * current device, allocates nothing, never synchronises, keeps no state
+ * between calls, and may be captured into a CUDA graph; calls on different
+ * streams share nothing unless the caller hands them the same buffers. Every
+ * pointer is device memory of the current device (other memory is refused
+ * with LAYA_ERR_ARG before anything is launched). laya_gpu_last_error(NULL)
+ * describes a failure.
+ *
+ * Offset tables, like laya_batch's, are device memory that the host does not
+ * read. The kernels check them: entries must not be negative, decrease or
+ * pass the row count, and no run may be longer than the stated longest. What
+ * fails is skipped without an access outside the buffers and recorded in the
+ * caller's status word; laya_gpu_op_status turns it into a return code. Rows
+ * before the first and behind the last entry are left as they were.
+ * ------------------------------------------------------------------------ */
+
+/* Wait for `stream`, read the status word (one int32 of device memory, zero
+ * before the first call that gets it; the operators only set bits in it) and
+ * clear it: LAYA_OK, LAYA_ERR_ARG (an offset table or an index failed a
+ * kernel's check) or LAYA_ERR_TIMEOUT (a bounded device-side wait ran out).
+ * Not during a capture. */
+LAYA_API int laya_gpu_op_status(int32_t* status, void* stream);
+
+/* Rotary positions (ropeJob, src/main.zig:2496-2521, has the half layout
+ * over the whole head, theta 160000). Pair i of a head of `rot_dim` rotated
+ * elements turns by pos * f_i:
+ *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos),
+ *   f_i = theta^(-2i / rot_dim)                               radians,
+ * divided by `factor` (>= 1) to reach longer contexts; with original_len >
+ * 0 only as far as the pair turns seldom within it: with r = original_len *
+ * f_i / (2 pi) turns and g = clamp((r - beta_slow) / (beta_fast -
+ * beta_slow), 0, 1), f_i becomes f_i (g + (1 - g) / factor). */
+typedef enum {
+    LAYA_ROPE_HALF = 0,        /* pair i = elements i and i + rot_dim / 2 */
+    LAYA_ROPE_INTERLEAVED = 1, /* pair i = elements 2i and 2i + 1 */
+} laya_rope_layout;
+
+#define LAYA_ROPE_MAX_HEAD_DIM 256
+
+/* Filled by laya_gpu_rope_plan; plain host memory, copied by each call. */
+typedef struct {
+    uint64_t turn[LAYA_ROPE_MAX_HEAD_DIM / 2]; /* turns a position, 2^-64 units, modulo 1 */
+    uint32_t head_dim, rot_dim;
+    int32_t layout;
+    float magnitude;
+} laya_rope_plan;
+
+/* head_dim even, <= LAYA_ROPE_MAX_HEAD_DIM; rot_dim even, 2 .. head_dim;
+ * theta > 1; factor >= 1; beta_fast > beta_slow >= 0; magnitude finite. Host
+ * only. */
+LAYA_API int laya_gpu_rope_plan(uint32_t head_dim, uint32_t rot_dim, double theta, int layout, double factor,
+                                uint32_t original_len, double beta_fast, double beta_slow, float magnitude,
+                                laya_rope_plan* plan);
+
+/* y = rotated x, for `heads` adjacent heads of each of n_tokens rows; row t
+ * of x starts at x + t * x_stride elements (y alike). Row t's position is
+ * positions[t] (any int32) or, with positions NULL, its place in its
+ * sequence of cu_seqlens[n_seqs + 1]; exactly one of the two is given.
+ * inverse != 0 turns the other way, still times magnitude: the transpose,
+ * which is the gradient. Elements behind rot_dim are copied. y may be x
+ * (same stride); otherwise the two must not overlap. elem_dtype: laya_dtype
+ * of both. Any alignment of the elements' own size; 16-byte aligned rows and
+ * chunks run faster. */
+LAYA_API int laya_gpu_rope(const laya_rope_plan* plan, const void* x, int64_t x_stride, void* y, int64_t y_stride,
+                           uint32_t n_tokens, uint32_t heads, const int32_t* cu_seqlens, uint32_t n_seqs,
+                           const int32_t* positions, int inverse, int elem_dtype, int32_t* status, void* stream);
+
+/* Attention over packed sequences (attWorker, src/main.zig:2431-2489), as an
+ * operator: per query row i and head,
+ *   s_ij = scale * q_i . k_j,  lse_i = log sum_j exp s_ij,
+ *   out_i = sum_j exp(s_ij - lse_i) v_j,
+ * over the keys j of the same sequence, |i - j| <= window unless window < 0.
+ * n_heads query heads share n_kv_heads key/value heads (n_heads /
+ * n_kv_heads neighbouring ones each). A token whose token_mask byte is 0 is
+ * absent (a padded batch's filler): no query sees it, its own out row is 0,
+ * its lse -inf, its gradients 0, and whatever its rows hold, NaN included,
+ * is not used. So are rows outside their sequence. The values of present
+ * tokens should be finite: a NaN reaches every row whose tile holds it. */
+#define LAYA_HEAD_DIM 64
+
+typedef struct {
+    const int32_t* cu_seqlens; /* [n_seqs + 1] token offsets */
+    const uint8_t* token_mask; /* [n_tokens], 0 = absent; NULL: all present */
+    int32_t* status;           /* the status word */
+    uint32_t n_seqs, n_tokens;
+    uint32_t max_len; /* no sequence is longer */
+    uint32_t n_heads, n_kv_heads;
+    int32_t window; /* keys to either side, < 0: all */
+    float scale;    /* > 0, 1/8 in the model */
+    int32_t elem_dtype; /* LAYA_DT_BF16 or LAYA_DT_F16: every row array */
+} laya_attention;
+
+/* q and out rows hold n_heads x 64 elements, k and v rows n_kv_heads x 64;
+ * row t starts at base + t * stride elements, strides multiples of 8, bases
+ * 16-byte aligned (columns of one packed projection output will do). lse
+ * (nullable) [n_heads][n_tokens] f32. out overlaps no input. */
+LAYA_API int laya_gpu_attention(const laya_attention* a, const void* q, int64_t q_stride, const void* k,
+                                int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride,
+                                float* lse, void* stream);
+
+/* Bytes that laya_gpu_attention_backward needs as workspace (0: bad shape). */
+LAYA_API uint64_t laya_gpu_attention_backward_workspace(const laya_attention* a);
+
+/* The gradients of sum(out * dout) with respect to q, k and v, from out and
+ * lse as laya_gpu_attention left them for the same inputs. Probabilities are
+ * recomputed from lse; key heads that several query heads share get the sum
+ * of their gradients. No atomics: the same inputs give the same bits. The
+ * gradients (strided like their inputs) overlap no input and not one
+ * another. workspace: device memory, 16-byte aligned, contents immaterial;
+ * calls that may overlap on the GPU need one each. */
+LAYA_API int laya_gpu_attention_backward(const laya_attention* a, const void* q, int64_t q_stride, const void* k,
+                                         int64_t k_stride, const void* v, int64_t v_stride, const void* out,
+                                         int64_t out_stride, const float* lse, const void* dout, int64_t dout_stride,
+                                         void* dq, int64_t dq_stride, void* dk, int64_t dk_stride, void* dv,
+                                         int64_t dv_stride, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* The clipped policy loss over each decision's options, with its gradient.
+ * With z = logits / temperature[qtype], log p = z - logsumexp(z) over the
+ * decision's own options, r = exp(log p_action - old_logp):
+ *   loss = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *          + kl_coef * sum_j p_j (log p_j - log ref_j) - entropy_coef * H(p),
+ * dlogits = grad * dloss/dlogits. An option whose logit is -inf is ruled out:
+ * p = 0, it adds nothing and its gradient is 0 (in ref_logits it should be
+ * -inf too: it then carries no reference probability either). A decision
+ * without options, or with every option ruled out, has loss 0 and gradient
+ * 0. The temperature is held to 1e-3 at least, as in the tempered softmax of
+ * src/main.zig:3799-3813. */
+typedef struct {
+    const int32_t* cu_options; /* [n_decisions + 1] option offsets */
+    const uint32_t* qtypes;    /* [n_decisions] 0..2; NULL: all 0 */
+    int32_t* status;           /* the status word */
+    uint32_t n_decisions, n_options;
+    uint32_t max_options; /* no decision has more */
+    float temperature[3];
+    float clip_low, clip_high; /* 0 <= clip_low <= 1, clip_high >= 0 */
+    float kl_coef, entropy_coef;
+    int32_t elem_dtype; /* of logits, ref_logits, dlogits */
+} laya_policy;
+
+/* logits, ref_logits (nullable: no reference, kl 0) [n_options]; actions
+ * [n_decisions], the option taken, counted within its decision; advantages,
+ * old_logp [n_decisions] f32; grad (nullable: 1) [n_decisions] f32, the
+ * gradient that reaches each decision's loss. Outputs, each nullable: loss,
+ * logp (of the action), kl, entropy [n_decisions] f32; dlogits [n_options].
+ * An action outside its decision, a qtype > 2 or a bad offset sets the status
+ * word; that decision's outputs are 0. dlogits overlaps no input. */
+LAYA_API int laya_gpu_policy_loss(const laya_policy* p, const void* logits, const void* ref_logits,
+                                  const int32_t* actions, const float* advantages, const float* old_logp,
+                                  const float* grad, float* loss, float* logp, float* kl, float* entropy,
+                                  void* dlogits, void* stream);
 
 #ifdef __cplusplus
 }

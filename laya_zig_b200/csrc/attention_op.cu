@@ -1,0 +1,565 @@
+// attention_op.cu -- packed attention as an operator: the forward with its
+// statistics and the backward pass, on mma.sync tiles of 64 x 64.
+//
+// Forward, per query row: the online softmax (running maximum and sum, one
+// pass over the keys), out = O / l and lse = m + log l.
+//
+// Backward, with the probabilities recomputed as P = exp(S - lse):
+//   delta_i = sum_d dO_id O_id            (= sum_j P_ij dP_ij)
+//   dP = dO V^T,  dS = P (dP - delta)
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
+// Two kernels, without atomics: one block per query tile walks the keys for
+// dQ (and leaves delta for the other), one per key tile walks the queries of
+// every head of its group for dK and dV. S and dP are computed in both, seven
+// products instead of five, which is what fixed summation order costs here.
+// P and dS are rounded to 16 bits as operands of the products that follow;
+// statistics, sums and accumulators are f32.
+//
+// Rows outside their sequence and absent tokens are filled with zeros on
+// their way into shared memory (cp.async with a source size of 0), so nothing
+// they hold enters a product: zero rows of Q and dO add nothing to dK and dV,
+// zero rows of K nothing to dQ, and the scores of such keys are masked where
+// the softmax sums them.
+#include <climits>
+
+#include "operators.cuh"
+
+namespace laya {
+namespace {
+
+constexpr int TB = 64;  // rows per tile
+constexpr int THREADS = 128;
+constexpr int TILE = TB * 64;  // elements
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Args {
+    const int* cu;
+    const uint8_t* mask;
+    int* status;
+    int n_seqs, n_tokens, max_len;
+    int group;  // query heads per key head
+    int window;
+    float scale;
+    int skip_len;  // sequences of at least this many tokens are another kernel's
+    AttnIO io;
+};
+
+// element offset of (row, col) in a 64 x 64 16-bit tile whose 16-byte chunks
+// are XORed by row: ldmatrix row fetches never share a bank
+__device__ __forceinline__ int swz(int r, int c) { return r * 64 + (((c >> 3) ^ (r & 7)) << 3) + (c & 7); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(p)));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// 16 (or 4) bytes from global to shared memory, zeros where !ok
+__device__ __forceinline__ void copy16(void* s, const void* g, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(s)), "l"(g), "r"(ok ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(void* s, const void* g, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(s)), "l"(g), "r"(ok ? 4 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Is token `i` of the sequence (any integer) there?
+__device__ __forceinline__ bool present(const Args& a, const SeqTile& t, int i) {
+    return i >= 0 && i < t.len && (!a.mask || a.mask[t.start + i] != 0);
+}
+
+// Rows row0 .. row0 + 63 of the sequence, 64 elements each, into a tile.
+template <typename T>
+__device__ __forceinline__ void load_tile(T* s, const AttnRows& rows, int head, const Args& a, const SeqTile& t,
+                                          int row0) {
+    const T* g = static_cast<const T*>(rows.p) + head * 64;
+#pragma unroll
+    for (int i = 0; i < TILE / 8 / THREADS; i++) {
+        const int idx = threadIdx.x + i * THREADS, r = idx >> 3, c = (idx & 7) * 8;
+        const bool ok = present(a, t, row0 + r);
+        const long long row = t.start + (ok ? row0 + r : 0);
+        copy16(s + swz(r, c), g + row * rows.ld + c, ok);
+    }
+}
+
+// Bits of the tile's 64 keys that are there.
+__device__ __forceinline__ void key_bits(uint32_t* bits, const Args& a, const SeqTile& t, int row0) {
+    const int w = threadIdx.x >> 5;
+    if (w < 2) {
+        const uint32_t b = __ballot_sync(0xffffffffu, present(a, t, row0 + (int)threadIdx.x));
+        if ((threadIdx.x & 31) == 0) bits[w] = b;
+    }
+}
+
+// A fragments (16 rows x 64) of a warp's rows of a tile.
+template <typename T>
+__device__ __forceinline__ void load_a(uint32_t (&f)[4][4], const T* s, int warp, int lane) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++) ldsm4(f[ks], s + swz(warp * 16 + (lane & 15), ks * 16 + (lane >> 4) * 8));
+}
+
+template <int N>
+__device__ __forceinline__ void clear(float (&c)[N][4]) {
+#pragma unroll
+    for (int j = 0; j < N; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+}
+
+// c[16 x 64 tile rows] = a (16 x 64) . tile^T
+template <typename T>
+__device__ __forceinline__ void mma_nt(float (&c)[8][4], const uint32_t (&a)[4][4], const T* tile, int lane) {
+    clear(c);
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+        for (int np = 0; np < 4; np++) {
+            uint32_t b[4];
+            ldsm4(b, tile + swz(np * 16 + (lane & 7) + (lane >> 4) * 8, ks * 16 + ((lane >> 3) & 1) * 8));
+            mma<T>(c[2 * np], a[ks], b[0], b[1]);
+            mma<T>(c[2 * np + 1], a[ks], b[2], b[3]);
+        }
+}
+
+// c[16 x 64] += p (16 x 64 tile rows, as accumulators) . tile
+template <typename T>
+__device__ __forceinline__ void mma_nn(float (&c)[8][4], const float (&p)[8][4], const T* tile, int lane) {
+#pragma unroll
+    for (int kk = 0; kk < 4; kk++) {
+        uint32_t a[4];
+        a[0] = pack2<T>(p[2 * kk][0], p[2 * kk][1]);
+        a[1] = pack2<T>(p[2 * kk][2], p[2 * kk][3]);
+        a[2] = pack2<T>(p[2 * kk + 1][0], p[2 * kk + 1][1]);
+        a[3] = pack2<T>(p[2 * kk + 1][2], p[2 * kk + 1][3]);
+#pragma unroll
+        for (int dp = 0; dp < 4; dp++) {
+            uint32_t b[4];
+            ldsm4_t(b, tile + swz(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, dp * 16 + (lane >> 4) * 8));
+            mma<T>(c[2 * dp], a, b[0], b[1]);
+            mma<T>(c[2 * dp + 1], a, b[2], b[3]);
+        }
+    }
+}
+
+// A warp's 16 x 64 accumulators, times two row factors, to rows of the
+// sequence; rows past its end are not written.
+template <typename T>
+__device__ __forceinline__ void store_rows(const AttnRows& rows, int head, const SeqTile& t, int r0, int lane,
+                                           const float (&c)[8][4], float f0, float f1) {
+    const int i0 = r0 + (lane >> 2), i1 = i0 + 8;
+    T* g = static_cast<T*>(rows.p) + head * 64 + 2 * (lane & 3);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        if (i0 < t.len)
+            *reinterpret_cast<uint32_t*>(g + (t.start + i0) * rows.ld + j * 8) =
+                f0 == 0.f ? 0u : pack2<T>(c[j][0] * f0, c[j][1] * f0);
+        if (i1 < t.len)
+            *reinterpret_cast<uint32_t*>(g + (t.start + i1) * rows.ld + j * 8) =
+                f1 == 0.f ? 0u : pack2<T>(c[j][2] * f1, c[j][3] * f1);
+    }
+}
+
+// Tiles [t0, t1) of the sequence that rows row0 .. row0 + 63 see.
+__device__ __forceinline__ void visible_tiles(const Args& a, const SeqTile& t, int* t0, int* t1) {
+    int lo = 0, hi = t.len;
+    if (a.window >= 0) {
+        lo = max(0, t.row0 - a.window);
+        hi = (int)min((long long)t.len, (long long)t.row0 + TB + a.window);
+    }
+    *t0 = lo / TB;
+    *t1 = (hi + TB - 1) / TB;
+}
+
+// Does some pair of the two tiles lie outside the window?
+__device__ __forceinline__ bool edge(int window, int row0, int col0) {
+    return window >= 0 && (row0 + TB - 1 - col0 > window || col0 + TB - 1 - row0 > window);
+}
+
+__device__ __forceinline__ bool block_tile(const Args& a, SeqTile* t) {
+    if (threadIdx.x == 0 && blockIdx.y == 0)
+        check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, blockIdx.x, a.status);
+    return find_tile(a.cu, a.n_seqs, a.n_tokens, a.max_len, TB, blockIdx.x, threadIdx.x & 31, t) &&
+           t->len < a.skip_len;
+}
+
+// ------------------------------------------------------------------ forward
+constexpr int FWD_SMEM = 5 * TILE * 2;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const Args a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    T* sq = reinterpret_cast<T*>(smem);
+    T* sk = sq + TILE;
+    T* sv = sk + 2 * TILE;
+    __shared__ uint32_t bits[2][2];
+    SeqTile t;
+    if (!block_tile(a, &t)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.y, hk = h / a.group;
+    int kt0, kt1;
+    visible_tiles(a, t, &kt0, &kt1);
+    load_tile(sq, a.io.q, h, a, t, t.row0);
+    load_tile(sk, a.io.k, hk, a, t, kt0 * TB);
+    load_tile(sv, a.io.v, hk, a, t, kt0 * TB);
+    key_bits(bits[0], a, t, kt0 * TB);
+    copy_commit();
+
+    const float sl2 = a.scale * LOG2E;
+    const int i0 = t.row0 + warp * 16 + (lane >> 2), i1 = i0 + 8;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float o[8][4];
+    clear(o);
+    uint32_t qa[4][4];
+    for (int kt = kt0; kt < kt1; kt++) {
+        const int b = (kt - kt0) & 1;
+        if (kt + 1 < kt1) {
+            load_tile(sk + (b ^ 1) * TILE, a.io.k, hk, a, t, (kt + 1) * TB);
+            load_tile(sv + (b ^ 1) * TILE, a.io.v, hk, a, t, (kt + 1) * TB);
+            key_bits(bits[b ^ 1], a, t, (kt + 1) * TB);
+        }
+        copy_commit();
+        copy_wait<1>();
+        __syncthreads();
+        if (kt == kt0) load_a(qa, sq, warp, lane);
+        float s[8][4];
+        mma_nt<T>(s, qa, sk + b * TILE, lane);
+        const uint64_t there = bits[b][0] | (uint64_t)bits[b][1] << 32;
+        if (there != ~0ull || edge(a.window, t.row0, kt * TB)) {
+            // element (j, e) of this thread is key kt * 64 + 8 j + 2 (lane & 3) + e
+            const int c0 = 2 * (lane & 3), k0 = kt * TB + c0;
+            const uint64_t w = there >> c0;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const bool ok = (w >> (8 * j + e)) & 1;
+                    const int key = k0 + 8 * j + e;
+                    if (!ok || (a.window >= 0 && abs(i0 - key) > a.window)) s[j][e] = -INFINITY;
+                    if (!ok || (a.window >= 0 && abs(i1 - key) > a.window)) s[j][2 + e] = -INFINITY;
+                }
+        }
+        float x0 = s[0][0], x1 = s[0][2];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
+            x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+        }
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float u0 = n0 == -INFINITY ? 0.f : n0 * sl2, u1 = n1 == -INFINITY ? 0.f : n1 * sl2;
+        const float a0 = ex2_approx(m0 * sl2 - u0), a1 = ex2_approx(m1 * sl2 - u1);
+        m0 = n0;
+        m1 = n1;
+        float r0 = 0.f, r1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            s[j][0] = ex2_approx(fmaf(s[j][0], sl2, -u0));
+            s[j][1] = ex2_approx(fmaf(s[j][1], sl2, -u0));
+            s[j][2] = ex2_approx(fmaf(s[j][2], sl2, -u1));
+            s[j][3] = ex2_approx(fmaf(s[j][3], sl2, -u1));
+            r0 += s[j][0] + s[j][1];
+            r1 += s[j][2] + s[j][3];
+            o[j][0] *= a0;
+            o[j][1] *= a0;
+            o[j][2] *= a1;
+            o[j][3] *= a1;
+        }
+        l0 = l0 * a0 + r0;
+        l1 = l1 * a1 + r1;
+        mma_nn<T>(o, s, sv + b * TILE, lane);
+        __syncthreads();  // every warp is done with this buffer before it is refilled
+    }
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
+    store_rows<T>(a.io.out, h, t, t.row0 + warp * 16, lane, o, p0 ? 1.f / l0 : 0.f, p1 ? 1.f / l1 : 0.f);
+    if (a.io.lse && (lane & 3) == 0) {
+        float* g = a.io.lse + (long long)h * a.n_tokens + t.start;
+        if (i0 < t.len) g[i0] = p0 ? m0 * a.scale + logf(l0) : -INFINITY;
+        if (i1 < t.len) g[i1] = p1 ? m1 * a.scale + logf(l1) : -INFINITY;
+    }
+}
+
+// ------------------------------------------------------------------ dQ (and delta)
+constexpr int DQ_SMEM = 6 * TILE * 2;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const Args a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    T* sq = reinterpret_cast<T*>(smem);
+    T* sdo = sq + TILE;
+    T* sk = sdo + TILE;
+    T* sv = sk + 2 * TILE;
+    __shared__ uint32_t bits[2][2];
+    __shared__ float sdelta[TB];
+    SeqTile t;
+    if (!block_tile(a, &t)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.y, hk = h / a.group;
+    int kt0, kt1;
+    visible_tiles(a, t, &kt0, &kt1);
+    load_tile(sq, a.io.q, h, a, t, t.row0);
+    load_tile(sdo, a.io.dout, h, a, t, t.row0);
+    load_tile(sk, a.io.k, hk, a, t, kt0 * TB);
+    load_tile(sv, a.io.v, hk, a, t, kt0 * TB);
+    key_bits(bits[0], a, t, kt0 * TB);
+    copy_commit();
+    {  // delta: two threads to a row, 32 elements each
+        const int r = threadIdx.x >> 1, i = t.row0 + r, c0 = (threadIdx.x & 1) * 32;
+        const bool ok = present(a, t, i);
+        float acc = 0.f;
+        uint4 ov[4];
+        if (ok) {
+            const T* g = static_cast<const T*>(a.io.out.p) + (t.start + i) * a.io.out.ld + h * 64 + c0;
+#pragma unroll
+            for (int c = 0; c < 4; c++) ov[c] = *reinterpret_cast<const uint4*>(g + 8 * c);
+        }
+        copy_wait<0>();
+        __syncthreads();
+        if (ok) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const T* x = reinterpret_cast<const T*>(&ov[c]);
+                const uint4 dv = *reinterpret_cast<const uint4*>(sdo + swz(r, c0 + 8 * c));
+                const T* y = reinterpret_cast<const T*>(&dv);
+#pragma unroll
+                for (int e = 0; e < 8; e++) acc = fmaf(to_float(x[e]), to_float(y[e]), acc);
+            }
+        }
+        acc += __shfl_xor_sync(0xffffffffu, acc, 1);
+        if ((threadIdx.x & 1) == 0) {
+            sdelta[r] = acc;
+            if (i < t.len) a.io.delta[(long long)h * a.n_tokens + t.start + i] = acc;
+        }
+        __syncthreads();
+    }
+    const float sl2 = a.scale * LOG2E;
+    const int i0 = t.row0 + warp * 16 + (lane >> 2), i1 = i0 + 8;
+    const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
+    const float* lse = a.io.lse + (long long)h * a.n_tokens + t.start;
+    // absent rows have q = dO = 0: any finite lse gives them dS = 0
+    const float e0 = p0 ? lse[i0] * LOG2E : 0.f, e1 = p1 ? lse[i1] * LOG2E : 0.f;
+    const float d0 = sdelta[warp * 16 + (lane >> 2)], d1 = sdelta[warp * 16 + (lane >> 2) + 8];
+    uint32_t qa[4][4], da[4][4];
+    load_a(qa, sq, warp, lane);
+    load_a(da, sdo, warp, lane);
+    float dq[8][4];
+    clear(dq);
+    for (int kt = kt0; kt < kt1; kt++) {
+        const int b = (kt - kt0) & 1;
+        if (kt + 1 < kt1) {
+            load_tile(sk + (b ^ 1) * TILE, a.io.k, hk, a, t, (kt + 1) * TB);
+            load_tile(sv + (b ^ 1) * TILE, a.io.v, hk, a, t, (kt + 1) * TB);
+            key_bits(bits[b ^ 1], a, t, (kt + 1) * TB);
+        }
+        copy_commit();
+        copy_wait<1>();
+        __syncthreads();
+        float s[8][4], dp[8][4];
+        mma_nt<T>(s, qa, sk + b * TILE, lane);
+        mma_nt<T>(dp, da, sv + b * TILE, lane);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                s[j][e] = ex2_approx(fmaf(s[j][e], sl2, -e0)) * (dp[j][e] - d0);
+                s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -e1)) * (dp[j][2 + e] - d1);
+            }
+        const uint64_t there = bits[b][0] | (uint64_t)bits[b][1] << 32;
+        if (there != ~0ull || edge(a.window, t.row0, kt * TB)) {
+            const int c0 = 2 * (lane & 3), k0 = kt * TB + c0;
+            const uint64_t w = there >> c0;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const bool ok = (w >> (8 * j + e)) & 1;
+                    const int key = k0 + 8 * j + e;
+                    if (!ok || (a.window >= 0 && abs(i0 - key) > a.window)) s[j][e] = 0.f;
+                    if (!ok || (a.window >= 0 && abs(i1 - key) > a.window)) s[j][2 + e] = 0.f;
+                }
+        }
+        mma_nn<T>(dq, s, sk + b * TILE, lane);
+        __syncthreads();
+    }
+    store_rows<T>(a.io.dq, h, t, t.row0 + warp * 16, lane, dq, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+}
+
+// ------------------------------------------------------------------ dK, dV
+constexpr int DKV_SMEM = 6 * TILE * 2 + 2 * 2 * TB * 4;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const Args a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    T* sk = reinterpret_cast<T*>(smem);
+    T* sv = sk + TILE;
+    T* sq = sv + TILE;
+    T* sdo = sq + 2 * TILE;
+    float* slse = reinterpret_cast<float*>(sdo + 2 * TILE);  // [2][64]
+    float* sdelta = slse + 2 * TB;
+    SeqTile t;
+    if (!block_tile(a, &t)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hk = blockIdx.y;
+    int qt0, qt1;
+    visible_tiles(a, t, &qt0, &qt1);  // the window is symmetric
+    const int nqt = qt1 - qt0, total = nqt * a.group;
+    auto load_q = [&](int it, int b) {
+        const int h = hk * a.group + it / nqt, row0 = (qt0 + it % nqt) * TB;
+        load_tile(sq + b * TILE, a.io.q, h, a, t, row0);
+        load_tile(sdo + b * TILE, a.io.dout, h, a, t, row0);
+        const int r = threadIdx.x & 63;
+        const bool ok = present(a, t, row0 + r);
+        const long long at = (long long)h * a.n_tokens + t.start + (ok ? row0 + r : 0);
+        copy4((threadIdx.x < 64 ? slse : sdelta) + b * TB + r, (threadIdx.x < 64 ? a.io.lse : a.io.delta) + at, ok);
+    };
+    load_tile(sk, a.io.k, hk, a, t, t.row0);
+    load_tile(sv, a.io.v, hk, a, t, t.row0);
+    load_q(0, 0);
+    copy_commit();
+    const float sl2 = a.scale * LOG2E;
+    const int j0 = t.row0 + warp * 16 + (lane >> 2), j1 = j0 + 8;
+    uint32_t ka[4][4], va[4][4];
+    float dk[8][4], dv[8][4];
+    clear(dk);
+    clear(dv);
+    for (int it = 0; it < total; it++) {
+        const int b = it & 1;
+        if (it + 1 < total) load_q(it + 1, b ^ 1);
+        copy_commit();
+        copy_wait<1>();
+        __syncthreads();
+        if (it == 0) {
+            load_a(ka, sk, warp, lane);
+            load_a(va, sv, warp, lane);
+        }
+        const int row0 = (qt0 + it % nqt) * TB;
+        // transposed: rows are keys, columns queries
+        float s[8][4], dp[8][4];
+        mma_nt<T>(s, ka, sq + b * TILE, lane);
+        const int c0 = 2 * (lane & 3);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float2 e = *reinterpret_cast<const float2*>(slse + b * TB + 8 * j + c0);
+            s[j][0] = ex2_approx(fmaf(s[j][0], sl2, -e.x * LOG2E));
+            s[j][1] = ex2_approx(fmaf(s[j][1], sl2, -e.y * LOG2E));
+            s[j][2] = ex2_approx(fmaf(s[j][2], sl2, -e.x * LOG2E));
+            s[j][3] = ex2_approx(fmaf(s[j][3], sl2, -e.y * LOG2E));
+        }
+        if (edge(a.window, row0, t.row0)) {
+            const int q0 = row0 + c0;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    if (abs(q0 + 8 * j + e - j0) > a.window) s[j][e] = 0.f;
+                    if (abs(q0 + 8 * j + e - j1) > a.window) s[j][2 + e] = 0.f;
+                }
+        }
+        mma_nn<T>(dv, s, sdo + b * TILE, lane);
+        mma_nt<T>(dp, va, sdo + b * TILE, lane);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float2 d = *reinterpret_cast<const float2*>(sdelta + b * TB + 8 * j + c0);
+            s[j][0] *= dp[j][0] - d.x;
+            s[j][1] *= dp[j][1] - d.y;
+            s[j][2] *= dp[j][2] - d.x;
+            s[j][3] *= dp[j][3] - d.y;
+        }
+        mma_nn<T>(dk, s, sq + b * TILE, lane);
+        __syncthreads();
+    }
+    const bool p0 = present(a, t, j0), p1 = present(a, t, j1);
+    store_rows<T>(a.io.dk, hk, t, t.row0 + warp * 16, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+    store_rows<T>(a.io.dv, hk, t, t.row0 + warp * 16, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
+}
+
+Args make_args(const laya_attention& a, const AttnIO& io) {
+    Args g;
+    g.cu = a.cu_seqlens;
+    g.mask = a.token_mask;
+    g.status = a.status;
+    g.n_seqs = (int)a.n_seqs;
+    g.n_tokens = (int)a.n_tokens;
+    g.max_len = (int)a.max_len;
+    g.group = (int)(a.n_heads / a.n_kv_heads);
+    g.window = a.window;
+    g.scale = a.scale;
+    g.skip_len = INT_MAX;
+    g.io = io;
+    return g;
+}
+
+cudaError_t launch(void (*kernel)(Args), unsigned heads, int smem, const Args& g, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), heads);
+    kernel<<<grid, THREADS, smem, stream>>>(g);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
+    return launch(a.elem_dtype == LAYA_DT_BF16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>,
+                  a.n_heads, FWD_SMEM, make_args(a, io), stream);
+}
+
+cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
+    const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
+    const Args g = make_args(a, io);
+    cudaError_t e = launch(bf16 ? attention_dq_kernel<__nv_bfloat16> : attention_dq_kernel<__half>, a.n_heads,
+                           DQ_SMEM, g, stream);
+    if (e == cudaSuccess)
+        e = launch(bf16 ? attention_dkv_kernel<__nv_bfloat16> : attention_dkv_kernel<__half>, a.n_kv_heads, DKV_SMEM,
+                   g, stream);
+    return e;
+}
+
+}  // namespace laya

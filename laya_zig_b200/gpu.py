@@ -74,6 +74,25 @@ class _Batch(ctypes.Structure):
                 ("n_tokens", ctypes.c_uint32), ("n_markers", ctypes.c_uint32), ("max_len", ctypes.c_uint32)]
 
 
+class _RopePlan(ctypes.Structure):
+    _fields_ = [("turn", ctypes.c_uint64 * 128), ("head_dim", ctypes.c_uint32), ("rot_dim", ctypes.c_uint32),
+                ("layout", ctypes.c_int32), ("magnitude", ctypes.c_float)]
+
+
+class _Attention(ctypes.Structure):
+    _fields_ = [("cu_seqlens", ctypes.c_void_p), ("token_mask", ctypes.c_void_p), ("status", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32), ("max_len", ctypes.c_uint32),
+                ("n_heads", ctypes.c_uint32), ("n_kv_heads", ctypes.c_uint32), ("window", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("elem_dtype", ctypes.c_int32)]
+
+
+class _Policy(ctypes.Structure):
+    _fields_ = [("cu_options", ctypes.c_void_p), ("qtypes", ctypes.c_void_p), ("status", ctypes.c_void_p),
+                ("n_decisions", ctypes.c_uint32), ("n_options", ctypes.c_uint32), ("max_options", ctypes.c_uint32),
+                ("temperature", ctypes.c_float * 3), ("clip_low", ctypes.c_float), ("clip_high", ctypes.c_float),
+                ("kl_coef", ctypes.c_float), ("entropy_coef", ctypes.c_float), ("elem_dtype", ctypes.c_int32)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError("liblaya_gpu.so is not built (%s); run `python -m laya_zig_b200.build`" % LIB_PATH)
@@ -112,6 +131,22 @@ def _load():
     L.laya_gpu_format_dump.restype = I
     L.laya_gpu_decision_tail_noalloc.argtypes = [P, P, P, P, P, U, U, P, P, P, P]
     L.laya_gpu_decision_tail_noalloc.restype = I
+    S, F, B = ctypes.c_int64, ctypes.c_float, ctypes.c_double
+    L.laya_gpu_op_status.argtypes = [P, P]
+    L.laya_gpu_op_status.restype = I
+    L.laya_gpu_rope_plan.argtypes = [U, U, B, I, B, U, B, B, F, ctypes.POINTER(_RopePlan)]
+    L.laya_gpu_rope_plan.restype = I
+    L.laya_gpu_rope.argtypes = [ctypes.POINTER(_RopePlan), P, S, P, S, U, U, P, U, P, I, I, P, P]
+    L.laya_gpu_rope.restype = I
+    L.laya_gpu_attention.argtypes = [ctypes.POINTER(_Attention), P, S, P, S, P, S, P, S, P, P]
+    L.laya_gpu_attention.restype = I
+    L.laya_gpu_attention_backward_workspace.argtypes = [ctypes.POINTER(_Attention)]
+    L.laya_gpu_attention_backward_workspace.restype = ctypes.c_uint64
+    L.laya_gpu_attention_backward.argtypes = [ctypes.POINTER(_Attention), P, S, P, S, P, S, P, S, P, P, S, P, S, P, S,
+                                              P, S, P, ctypes.c_uint64, P]
+    L.laya_gpu_attention_backward.restype = I
+    L.laya_gpu_policy_loss.argtypes = [ctypes.POINTER(_Policy)] + [P] * 12
+    L.laya_gpu_policy_loss.restype = I
     return L
 
 
@@ -391,3 +426,113 @@ def linear(x_ptr: int, w_ptr: int, bias_ptr: int, out_ptr: int, M: int, N: int, 
     rc = lib.laya_gpu_linear(x_ptr, w_ptr, bias_ptr or None, out_ptr, M, N, K, DT[dtype], stream or None)
     if rc != LAYA_OK:
         raise _error(rc, lib.laya_gpu_last_error(None).decode())
+
+
+# ---------------------------------------------------------------------------
+# Operators of a training step (include/laya_gpu.h has their definitions).
+# Everything is a raw device pointer of the current device (e.g. a torch
+# tensor's data_ptr()), strides count elements, 0 stands for NULL; calls are
+# asynchronous on `stream`. `status_ptr` is one int32 of device memory, zero
+# at first: op_status() waits and raises if a kernel's check failed.
+
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def _op_check(rc: int) -> None:
+    if rc != LAYA_OK:
+        raise _error(rc, lib.laya_gpu_last_error(None).decode())
+
+
+def op_status(status_ptr: int, stream: int = 0) -> None:
+    """Wait for `stream`; raise if an operator that was given this status
+    word recorded a failed check or a wait that ran out; clear the word."""
+    _op_check(lib.laya_gpu_op_status(status_ptr, stream or None))
+
+
+class RopePlan:
+    """Frequencies of a rotary embedding: made once, used by every rope().
+    `factor` stretches it to longer contexts, for all pairs alike or, with
+    `original_len`, for those that turn seldom within it."""
+
+    def __init__(self, head_dim: int = 64, rot_dim: Optional[int] = None, theta: float = 160000.0,
+                 layout: str = "half", factor: float = 1.0, original_len: int = 0, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, magnitude: float = 1.0):
+        if layout not in ROPE_LAYOUTS:
+            raise LayaError(ERR_ARG, "rope_plan: layout %s" % layout)
+        self.c = _RopePlan()
+        _op_check(lib.laya_gpu_rope_plan(head_dim, head_dim if rot_dim is None else rot_dim, theta,
+                                         ROPE_LAYOUTS[layout], factor, original_len, beta_fast, beta_slow, magnitude,
+                                         ctypes.byref(self.c)))
+
+
+def rope(plan: RopePlan, x_ptr: int, x_stride: int, y_ptr: int, y_stride: int, n_tokens: int, heads: int,
+         status_ptr: int, cu_seqlens_ptr: int = 0, n_seqs: int = 0, positions_ptr: int = 0, inverse: bool = False,
+         dtype: str = "BF16", stream: int = 0) -> None:
+    """Rotate `heads` adjacent heads of every row (queries and keys side by
+    side in a packed projection, say); inverse=True is the gradient."""
+    _op_check(lib.laya_gpu_rope(ctypes.byref(plan.c), x_ptr or None, x_stride, y_ptr or None, y_stride, n_tokens,
+                                heads, cu_seqlens_ptr or None, n_seqs, positions_ptr or None, int(inverse), DT[dtype],
+                                status_ptr or None, stream or None))
+
+
+class AttentionShape:
+    """What attention() and attention_backward() need to know besides the rows."""
+
+    def __init__(self, cu_seqlens_ptr: int, n_seqs: int, n_tokens: int, max_len: int, n_heads: int, n_kv_heads: int,
+                 status_ptr: int, window: int = -1, scale: float = 0.125, dtype: str = "BF16",
+                 token_mask_ptr: int = 0):
+        self.c = _Attention(cu_seqlens_ptr or None, token_mask_ptr or None, status_ptr or None, n_seqs, n_tokens,
+                            max_len, n_heads, n_kv_heads, window, scale, DT[dtype])
+
+
+def attention(shape: AttentionShape, q_ptr: int, q_stride: int, k_ptr: int, k_stride: int, v_ptr: int, v_stride: int,
+              out_ptr: int, out_stride: int, lse_ptr: int = 0, stream: int = 0) -> None:
+    """Attention over packed sequences; lse[n_heads][n_tokens] is what the
+    backward pass needs."""
+    _op_check(lib.laya_gpu_attention(ctypes.byref(shape.c), q_ptr or None, q_stride, k_ptr or None, k_stride,
+                                     v_ptr or None, v_stride, out_ptr or None, out_stride, lse_ptr or None,
+                                     stream or None))
+
+
+def attention_backward_workspace(shape: AttentionShape) -> int:
+    """Bytes of workspace for attention_backward()."""
+    n = lib.laya_gpu_attention_backward_workspace(ctypes.byref(shape.c))
+    if n == 0 and shape.c.n_tokens:
+        raise _error(ERR_ARG, lib.laya_gpu_last_error(None).decode())
+    return n
+
+
+def attention_backward(shape: AttentionShape, q_ptr: int, q_stride: int, k_ptr: int, k_stride: int, v_ptr: int,
+                       v_stride: int, out_ptr: int, out_stride: int, lse_ptr: int, dout_ptr: int, dout_stride: int,
+                       dq_ptr: int, dq_stride: int, dk_ptr: int, dk_stride: int, dv_ptr: int, dv_stride: int,
+                       workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
+    """Gradients of sum(out * dout) with respect to q, k and v, from the
+    out and lse that attention() left."""
+    _op_check(lib.laya_gpu_attention_backward(ctypes.byref(shape.c), q_ptr or None, q_stride, k_ptr or None, k_stride,
+                                              v_ptr or None, v_stride, out_ptr or None, out_stride, lse_ptr or None,
+                                              dout_ptr or None, dout_stride, dq_ptr or None, dq_stride,
+                                              dk_ptr or None, dk_stride, dv_ptr or None, dv_stride,
+                                              workspace_ptr or None, workspace_bytes, stream or None))
+
+
+class PolicyBatch:
+    """Decisions of policy_loss(): option offsets, question types (NULL: all
+    0), tempering and coefficients."""
+
+    def __init__(self, cu_options_ptr: int, n_decisions: int, n_options: int, max_options: int, status_ptr: int,
+                 qtypes_ptr: int = 0, temperature: Sequence[float] = (1.0, 1.0, 1.0), clip_low: float = 0.2,
+                 clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0, dtype: str = "F32"):
+        self.c = _Policy(cu_options_ptr or None, qtypes_ptr or None, status_ptr or None, n_decisions, n_options,
+                         max_options, (ctypes.c_float * 3)(*temperature), clip_low, clip_high, kl_coef, entropy_coef,
+                         DT[dtype])
+
+
+def policy_loss(batch: PolicyBatch, logits_ptr: int, ref_logits_ptr: int, actions_ptr: int, advantages_ptr: int,
+                old_logp_ptr: int, grad_ptr: int = 0, loss_ptr: int = 0, logp_ptr: int = 0, kl_ptr: int = 0,
+                entropy_ptr: int = 0, dlogits_ptr: int = 0, stream: int = 0) -> None:
+    """The clipped policy loss of each decision and, with dlogits_ptr, its
+    gradient times grad (0: 1)."""
+    _op_check(lib.laya_gpu_policy_loss(ctypes.byref(batch.c), logits_ptr or None, ref_logits_ptr or None,
+                                       actions_ptr or None, advantages_ptr or None, old_logp_ptr or None,
+                                       grad_ptr or None, loss_ptr or None, logp_ptr or None, kl_ptr or None,
+                                       entropy_ptr or None, dlogits_ptr or None, stream or None))
