@@ -12,8 +12,8 @@
 // g = -r A while the unclipped term is the smaller one, else 0.
 //
 // A decision's options are read once and stay in registers (a group of G
-// lanes, V options each, G * V >= max_options); sums are warp shuffles in a
-// fixed order. Above 1,024 options a block takes a decision and reads it
+// threads, V options each, G * V >= max_options); sums are shuffles, over a
+// block joined in shared memory, in a fixed order. Above 1,024 options a block takes a decision and reads it
 // three times. The bytes are 3 per option and element byte; what bounds the
 // small ones is the launch.
 #include "operators.cuh"
@@ -21,38 +21,53 @@
 namespace laya {
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Scalars {
     const int* cu;
     const uint32_t* qtypes;
     int n, G;
     int max_k;
+    float scale[3];   // log2(e) / temperature: logits -> z in units of log 2
     float inv_t[3];
     float lo, hi, kl_coef, ent_coef;
     int* status;
 };
 
-template <int G>
-__device__ __forceinline__ float group_max(float v) {
+// Sums or maxima of two values over the G threads of a decision, in a fixed
+// order: part of a warp, a warp, or the whole block.
+template <int G, bool MAX>
+__device__ __forceinline__ void group_reduce(float& a, float& b, float2* buf) {
+    auto join = [](float u, float v) { return MAX ? fmaxf(u, v) : u + v; };
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-template <int G>
-__device__ __forceinline__ float group_sum(float v) {
+    for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) {
+        const float u = __shfl_xor_sync(0xffffffffu, a, o), v = __shfl_xor_sync(0xffffffffu, b, o);
+        a = join(a, u);
+        b = join(b, v);
+    }
+    if (G > 32) {
+        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = make_float2(a, b);
+        __syncthreads();
+        a = buf[0].x;
+        b = buf[0].y;
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+        for (int w = 1; w < G / 32; w++) {
+            a = join(a, buf[w].x);
+            b = join(b, buf[w].y);
+        }
+    }
 }
 
 // What one thread needs of its decision besides the options.
 struct Decision {
     int start, k, action;
-    float adv, old_logp, grad, inv_t;
+    float adv, old_logp, grad, inv_t, scale;
+    float taken;  // z of the action
     bool ok;
 };
 
+template <typename T>
 __device__ __forceinline__ Decision load_decision(const Scalars& s, const PolicyIO& io, int i) {
     Decision d;
     const int start = s.cu[i], end = s.cu[i + 1];
@@ -65,8 +80,10 @@ __device__ __forceinline__ Decision load_decision(const Scalars& s, const Policy
     d.grad = io.grad ? io.grad[i] : 1.f;
     const bool run = run_ok(start, end, s.G, s.max_k);
     d.ok = run && q <= 2u && (d.k == 0 || (d.action >= 0 && d.action < d.k));
-    d.inv_t = s.inv_t[q <= 2u ? q : 0u];
+    d.inv_t = q == 1u ? s.inv_t[1] : q == 2u ? s.inv_t[2] : s.inv_t[0];
+    d.scale = q == 1u ? s.scale[1] : q == 2u ? s.scale[2] : s.scale[0];
     if (!run) d.k = 0;  // nothing of it can be addressed
+    d.taken = d.ok && d.k > 0 ? to_float(static_cast<const T*>(io.logits)[start + d.action]) * d.scale : 0.f;
     return d;
 }
 
@@ -96,157 +113,173 @@ __device__ __forceinline__ void store_scalars(const PolicyIO& io, int i, const R
     if (io.entropy) io.entropy[i] = r.ent;
 }
 
-// One option's share of the KL, from its log probabilities.
-__device__ __forceinline__ float kl_term(float lp, float p, float lr) {
-    const float d = lp - lr;
-    // p (d + e^-d - 1); away from 0 the plain difference of probabilities
-    return p > 0.f ? p * d + (fabsf(d) < 0.5f ? p * expm1f(-d) : expf(lr) - p) : expf(lr);
+// One option's share of the KL in units of log 2, from its log2
+// probabilities: p d - p + ref. For |d| < 1/4 that is p times the series of
+// d + e^-d - 1 = d^2 (1/2 - d/6 + d^2/24 - ...), six terms of it (the next is
+// below 2^-23 of the sum); from there on the plain differences, whose
+// rounding is below 2^-20 of it. In units of log 2: a = log 2 times d.
+__device__ __forceinline__ float kl_term(float d, float p, float lr) {
+    constexpr float L = LN2;
+    float g = fmaf(d, -L * L * L * L * L * L / 5040.f, L * L * L * L * L / 720.f);
+    g = fmaf(d, g, -L * L * L * L / 120.f);
+    g = fmaf(d, g, L * L * L / 24.f);
+    g = fmaf(d, g, -L * L / 6.f);
+    g = fmaf(d, g, L / 2.f);
+    const float near = p * d * (d * g);
+    const float far = fmaf(p, d, (ex2_approx(lr) - p) * (1.f / L));
+    return !(p == 0.f) && fabsf(d) < 0.25f / L ? near : p == 0.f ? ex2_approx(lr) * (1.f / L) : far;
+}
+
+// dloss/dz of one option, times the weights: p (c0 + c1 d + c2 lp), plus
+// own for the option that was taken.
+struct Slope {
+    float own, c0, c1, c2;
+};
+__device__ __forceinline__ Slope slope(const Scalars& s, const Decision& d, const Result& r) {
+    const float w = d.grad * d.inv_t;
+    Slope c;
+    c.own = r.g * w;
+    c.c0 = w * (-r.g - s.kl_coef * r.kl + s.ent_coef * r.ent);
+    c.c1 = w * s.kl_coef * LN2;
+    c.c2 = w * s.ent_coef * LN2;
+    return c;
 }
 
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io) {
+    static_assert(G <= 32 || G == THREADS, "a decision is part of a warp, a warp or a block");
+    __shared__ float2 buf[3][THREADS / 32];  // one row for each block-wide reduction
     const int group = threadIdx.x / G, l = threadIdx.x % G;
     const long long at = (long long)blockIdx.x * (THREADS / G) + group;
     const bool live = at < s.n;
     const int i = live ? (int)at : s.n - 1;  // whole warps take part in the shuffles
-    Decision d = load_decision(s, io, i);
+    Decision d = load_decision<T>(s, io, i);
     if (live && !d.ok && l == 0) atomicOr(s.status, ERR_BAD_INDEX);
     const T* x = static_cast<const T*>(io.logits) + d.start;
     const T* xr = static_cast<const T*>(io.ref) + d.start;
     const int k = d.k;
-    float z[V], zr[V];
-    float m = -INFINITY, mr = -INFINITY;
+    // thread l holds options l, l + G, ..; all loads are under way before the
+    // first is used
+    float z[V], zr[V], p[V];
+    {
+        T raw[V], rawr[V];
 #pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int j = l + v * G;
-        z[v] = j < k ? to_float(x[j]) * d.inv_t : -INFINITY;
-        zr[v] = io.ref && j < k ? to_float(xr[j]) * d.inv_t : -INFINITY;
+        for (int v = 0; v < V; v++)
+            if (l + v * G < k) raw[v] = x[l + v * G];
+        if (io.ref) {
+#pragma unroll
+            for (int v = 0; v < V; v++)
+                if (l + v * G < k) rawr[v] = xr[l + v * G];
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            z[v] = l + v * G < k ? to_float(raw[v]) * d.scale : -INFINITY;
+            zr[v] = io.ref && l + v * G < k ? to_float(rawr[v]) * d.scale : -INFINITY;
+        }
     }
+    float m = -INFINITY, mr = -INFINITY;
 #pragma unroll
     for (int v = 0; v < V; v++) {
         m = fmaxf(m, z[v]);
         mr = fmaxf(mr, zr[v]);
     }
-    m = group_max<G>(m);
-    mr = group_max<G>(mr);
+    group_reduce<G, true>(m, mr, buf[0]);
     const float mz = m == -INFINITY ? 0.f : m, mrz = mr == -INFINITY ? 0.f : mr;
     float sum = 0.f, sumr = 0.f;
+    // ex2.approx here and below: 2^-22 relative, of exponents whose own
+    // rounding is small for every term that carries weight in a sum
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        sum += expf(z[v] - mz);
-        sumr += expf(zr[v] - mrz);
+        if (v * G >= k) break;  // of the whole group
+        sum += ex2_approx(z[v] - mz);
+        if (io.ref) sumr += ex2_approx(zr[v] - mrz);
     }
-    sum = group_sum<G>(sum);
-    sumr = group_sum<G>(sumr);
+    group_reduce<G, false>(sum, sumr, buf[1]);
     const bool some = d.ok && !(sum == 0.f);  // an option that is not ruled out
-    const float lse = mz + logf(sum), lser = mrz + logf(sumr);
-    float ent = 0.f, kl = 0.f, lpa = 0.f;
+    const float lse = mz + log2f(sum), lser = mrz + log2f(sumr);
+    float ent = 0.f, kl = 0.f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const int j = l + v * G;
-        z[v] -= lse;  // log p
-        const float p = expf(z[v]);
-        if (p > 0.f) ent -= p * z[v];
-        if (j == d.action) lpa = z[v];
-        if (io.ref && j < k) {
+        if (v * G >= k) break;
+        z[v] -= lse;  // log2 p
+        p[v] = ex2_approx(z[v]);
+        if (!(p[v] == 0.f)) ent = fmaf(-p[v], z[v], ent);
+        if (io.ref && l + v * G < k) {
             zr[v] -= lser;
-            kl += kl_term(z[v], p, zr[v]);
+            const float dv = z[v] - zr[v];
+            kl += kl_term(dv, p[v], zr[v]);
+            zr[v] = dv;
         }
     }
-    ent = group_sum<G>(ent);
-    kl = group_sum<G>(kl);
-    lpa = group_sum<G>(lpa);  // one lane holds it
-    Result r = some ? finish(s, d, lpa, kl, ent) : Result{};
+    group_reduce<G, false>(ent, kl, buf[2]);
+    Result r = some ? finish(s, d, (d.taken - lse) * LN2, kl * LN2, ent * LN2) : Result{};
     if (!live) return;
     if (l == 0) store_scalars(io, i, r);
     if (io.dlogits) {
         T* dx = static_cast<T*>(io.dlogits) + d.start;
-        const float w = d.grad * d.inv_t;
+        const Slope c = slope(s, d, r);
 #pragma unroll
         for (int v = 0; v < V; v++) {
+            if (v * G >= k) break;
             const int j = l + v * G;
-            if (j >= k) continue;
-            float g = 0.f;
-            if (some && !(z[v] == -INFINITY)) {  // not ruled out
-                const float lp = z[v], p = expf(lp);
-                g = r.g * ((j == d.action ? 1.f : 0.f) - p);
-                if (!(p == 0.f)) {
-                    if (io.ref) g += s.kl_coef * p * (lp - zr[v] - r.kl);
-                    g += s.ent_coef * p * (lp + r.ent);
-                }
-                g *= w;
-            }
-            dx[j] = from_float<T>(g);
+            float g = fmaf(c.c2, z[v], c.c0);
+            if (io.ref) g = fmaf(c.c1, zr[v], g);
+            g = p[v] == 0.f ? 0.f : p[v] * g;  // an option that is ruled out has log p = -inf
+            if (j == d.action) g += c.own;
+            if (j < k) dx[j] = from_float<T>(some ? g : 0.f);
         }
     }
-}
-
-__device__ __forceinline__ float block_reduce(float v, bool is_max, float* buf) {
-    v = is_max ? warp_max(v) : warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float r = buf[0];
-    for (int w = 1; w < THREADS / 32; w++) r = is_max ? fmaxf(r, buf[w]) : r + buf[w];
-    return r;
 }
 
 // A decision of any number of options: a block reads it three times.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyIO io) {
-    __shared__ float buf[THREADS / 32];
+    __shared__ float2 buf[3][THREADS / 32];
     for (long long at = blockIdx.x; at < s.n; at += gridDim.x) {
         const int i = (int)at;
-        Decision d = load_decision(s, io, i);
+        Decision d = load_decision<T>(s, io, i);
         if (!d.ok && threadIdx.x == 0) atomicOr(s.status, ERR_BAD_INDEX);
         const T* x = static_cast<const T*>(io.logits) + d.start;
         const T* xr = static_cast<const T*>(io.ref) + d.start;
         const int k = d.k;
         float m = -INFINITY, mr = -INFINITY;
         for (int j = threadIdx.x; j < k; j += THREADS) {
-            m = fmaxf(m, to_float(x[j]) * d.inv_t);
-            if (io.ref) mr = fmaxf(mr, to_float(xr[j]) * d.inv_t);
+            m = fmaxf(m, to_float(x[j]) * d.scale);
+            if (io.ref) mr = fmaxf(mr, to_float(xr[j]) * d.scale);
         }
-        m = block_reduce(m, true, buf);
-        mr = block_reduce(mr, true, buf);
+        group_reduce<THREADS, true>(m, mr, buf[0]);
         const float mz = m == -INFINITY ? 0.f : m, mrz = mr == -INFINITY ? 0.f : mr;
         float sum = 0.f, sumr = 0.f;
         for (int j = threadIdx.x; j < k; j += THREADS) {
-            sum += expf(to_float(x[j]) * d.inv_t - mz);
-            if (io.ref) sumr += expf(to_float(xr[j]) * d.inv_t - mrz);
+            sum += ex2_approx(to_float(x[j]) * d.scale - mz);
+            if (io.ref) sumr += ex2_approx(to_float(xr[j]) * d.scale - mrz);
         }
-        sum = block_reduce(sum, false, buf);
-        sumr = block_reduce(sumr, false, buf);
+        group_reduce<THREADS, false>(sum, sumr, buf[1]);
         const bool some = d.ok && !(sum == 0.f);
-        const float lse = mz + logf(sum), lser = mrz + logf(sumr);
-        float ent = 0.f, kl = 0.f, lpa = 0.f;
+        const float lse = mz + log2f(sum), lser = mrz + log2f(sumr);
+        float ent = 0.f, kl = 0.f;
         for (int j = threadIdx.x; j < k; j += THREADS) {
-            const float lp = to_float(x[j]) * d.inv_t - lse, p = expf(lp);
-            if (p > 0.f) ent -= p * lp;
-            if (j == d.action) lpa = lp;
-            if (io.ref) kl += kl_term(lp, p, to_float(xr[j]) * d.inv_t - lser);
+            const float lp = to_float(x[j]) * d.scale - lse, p = ex2_approx(lp);
+            if (!(p == 0.f)) ent = fmaf(-p, lp, ent);
+            if (io.ref) {
+                const float lr = to_float(xr[j]) * d.scale - lser;
+                kl += kl_term(lp - lr, p, lr);
+            }
         }
-        ent = block_reduce(ent, false, buf);
-        kl = block_reduce(kl, false, buf);
-        lpa = block_reduce(lpa, false, buf);
-        const Result r = some ? finish(s, d, lpa, kl, ent) : Result{};
+        group_reduce<THREADS, false>(ent, kl, buf[2]);
+        const Result r = some ? finish(s, d, (d.taken - lse) * LN2, kl * LN2, ent * LN2) : Result{};
+        __syncthreads();  // buf is free for the next decision
         if (threadIdx.x == 0) store_scalars(io, i, r);
         if (io.dlogits) {
             T* dx = static_cast<T*>(io.dlogits) + d.start;
-            const float w = d.grad * d.inv_t;
+            const Slope c = slope(s, d, r);
             for (int j = threadIdx.x; j < k; j += THREADS) {
-                float g = 0.f;
-                const float lp = to_float(x[j]) * d.inv_t - lse;
-                if (some && !(lp == -INFINITY)) {
-                    const float p = expf(lp);
-                    g = r.g * ((j == d.action ? 1.f : 0.f) - p);
-                    if (!(p == 0.f)) {
-                        if (io.ref) g += s.kl_coef * p * (lp - (to_float(xr[j]) * d.inv_t - lser) - r.kl);
-                        g += s.ent_coef * p * (lp + r.ent);
-                    }
-                    g *= w;
-                }
-                dx[j] = from_float<T>(g);
+                const float lp = to_float(x[j]) * d.scale - lse, p = ex2_approx(lp);
+                float g = fmaf(c.c2, lp, c.c0);
+                if (io.ref) g = fmaf(c.c1, lp - (to_float(xr[j]) * d.scale - lser), g);
+                g = p == 0.f ? 0.f : p * g;
+                if (j == d.action) g += c.own;
+                dx[j] = from_float<T>(some ? g : 0.f);
             }
         }
     }
@@ -263,7 +296,7 @@ template <typename T>
 cudaError_t launch_t(const Scalars& s, const PolicyIO& io, cudaStream_t stream) {
     if (s.max_k <= 16) return launch_g<T, 8, 2>(s, io, stream);
     if (s.max_k <= 128) return launch_g<T, 32, 4>(s, io, stream);
-    if (s.max_k <= 1024) return launch_g<T, 32, 32>(s, io, stream);
+    if (s.max_k <= 1024) return launch_g<T, THREADS, 8>(s, io, stream);
     policy_wide_kernel<T><<<(unsigned)(s.n < 148 * 8 ? s.n : 148 * 8), THREADS, 0, stream>>>(s, io);
     return cudaGetLastError();
 }
@@ -277,7 +310,10 @@ cudaError_t launch_policy(const laya_policy& p, const PolicyIO& io, cudaStream_t
     s.n = (int)p.n_decisions;
     s.G = (int)p.n_options;
     s.max_k = (int)p.max_options;
-    for (int i = 0; i < 3; i++) s.inv_t[i] = 1.f / fmaxf(1e-3f, p.temperature[i]);
+    for (int i = 0; i < 3; i++) {
+        s.inv_t[i] = 1.f / fmaxf(1e-3f, p.temperature[i]);
+        s.scale[i] = (float)(1.4426950408889634 / fmaxf(1e-3f, p.temperature[i]));
+    }
     s.lo = 1.f - p.clip_low;
     s.hi = 1.f + p.clip_high;
     s.kl_coef = p.kl_coef;

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int PAIRS = LAYA_ROPE_MAX_HEAD_DIM / 2;
+constexpr int BATCH = 4;  // pieces a lane has in flight
 
 template <typename T>
 struct Chunk {
@@ -55,6 +56,38 @@ __global__ void __launch_bounds__(WARPS * 32) rope_kernel(const __grid_constant_
             if (!run_ok(cu[s], cu[s + 1], n_tokens, n_tokens)) atomicOr(status, ERR_BAD_INDEX);
     }
     if (t >= n_tokens) return;
+    const T* xr = x + t * x_stride;
+    T* yr = y + t * y_stride;
+    const bool copy = x != y;  // elements that no pair holds
+    // The row in pieces: 16 bytes, or two of the pair's halves. The first
+    // batch is on its way before the token's position is known.
+    constexpr int N = Chunk<T>::N;
+    const int rot_items = HALF ? (int)plan.rot_dim / (2 * N) : (int)plan.rot_dim / N;
+    const int items = rot_items + (copy ? (int)(plan.head_dim - plan.rot_dim) / N : 0);
+    int h = VEC ? lane / items : 0, it = VEC ? lane % items : 0;
+    const int dh = VEC ? 32 / items : 0, di = VEC ? 32 % items : 0;
+    Chunk<T> a[BATCH], b[BATCH];
+    int at[BATCH], piece[BATCH];
+    auto load_batch = [&]() {
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            at[u] = -1;
+            piece[u] = it;
+            if (h < heads) {
+                at[u] = h * (int)plan.head_dim +
+                        (it >= rot_items ? (int)plan.rot_dim + (it - rot_items) * N : it * N);
+                a[u] = load_chunk(xr + at[u]);
+                if (HALF && it < rot_items) b[u] = load_chunk(xr + at[u] + plan.rot_dim / 2);
+            }
+            h += dh;
+            it += di;
+            if (it >= items) {
+                it -= items;
+                h++;
+            }
+        }
+    };
+    if constexpr (VEC) load_batch();
     int pos;
     if (positions) {
         pos = positions[t];
@@ -75,46 +108,37 @@ __global__ void __launch_bounds__(WARPS * 32) rope_kernel(const __grid_constant_
     }
     __syncwarp();
     const float2* tab = table[warp];
-    const T* xr = x + t * x_stride;
-    T* yr = y + t * y_stride;
-    const bool copy = x != y;  // elements that no pair holds
     if constexpr (VEC) {
-        constexpr int N = Chunk<T>::N;
-        const int rot_items = HALF ? half / N : rot / N;
-        const int rest = copy ? (hd - rot) / N : 0;
-        const int items = rot_items + rest;
-        const int total = items * heads;
-#pragma unroll 4
-        for (int w = lane; w < total; w += 32) {
-            const int h = w / items, i = w - h * items;
-            const long long at = (long long)h * hd;
-            if (i >= rot_items) {
-                const long long o = at + rot + (i - rot_items) * N;
-                store_chunk(yr + o, load_chunk(xr + o));
-            } else if (HALF) {
-                const long long o = at + i * N;
-                Chunk<T> a = load_chunk(xr + o), b = load_chunk(xr + o + half);
+        while (true) {
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    const float2 cs = tab[i * N + j];
-                    const float u = to_float(a.e[j]), v = to_float(b.e[j]);
-                    a.e[j] = from_float<T>(u * cs.x - v * cs.y);
-                    b.e[j] = from_float<T>(u * cs.y + v * cs.x);
-                }
-                store_chunk(yr + o, a);
-                store_chunk(yr + o + half, b);
-            } else {
-                const long long o = at + i * N;
-                Chunk<T> a = load_chunk(xr + o);
+            for (int u = 0; u < BATCH; u++) {
+                if (at[u] < 0) continue;
+                const int i = piece[u];
+                if (i >= rot_items) {
+                    store_chunk(yr + at[u], a[u]);
+                } else if (HALF) {
 #pragma unroll
-                for (int j = 0; j < N; j += 2) {
-                    const float2 cs = tab[(i * N + j) / 2];
-                    const float u = to_float(a.e[j]), v = to_float(a.e[j + 1]);
-                    a.e[j] = from_float<T>(u * cs.x - v * cs.y);
-                    a.e[j + 1] = from_float<T>(u * cs.y + v * cs.x);
+                    for (int j = 0; j < N; j++) {
+                        const float2 cs = tab[i * N + j];
+                        const float p = to_float(a[u].e[j]), q = to_float(b[u].e[j]);
+                        a[u].e[j] = from_float<T>(p * cs.x - q * cs.y);
+                        b[u].e[j] = from_float<T>(p * cs.y + q * cs.x);
+                    }
+                    store_chunk(yr + at[u], a[u]);
+                    store_chunk(yr + at[u] + half, b[u]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j += 2) {
+                        const float2 cs = tab[(i * N + j) / 2];
+                        const float p = to_float(a[u].e[j]), q = to_float(a[u].e[j + 1]);
+                        a[u].e[j] = from_float<T>(p * cs.x - q * cs.y);
+                        a[u].e[j + 1] = from_float<T>(p * cs.y + q * cs.x);
+                    }
+                    store_chunk(yr + at[u], a[u]);
                 }
-                store_chunk(yr + o, a);
             }
+            if (h >= heads) break;
+            load_batch();
         }
     } else {
         const int rest = copy ? hd - rot : 0;

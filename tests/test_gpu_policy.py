@@ -120,12 +120,11 @@ def _check(lens, dtype="F32", klc=0.1, entc=0.03, use_ref=True, use_q=True, use_
             own = torch.zeros(k, dtype=torch.float64)
             own[int(act[i])] = 1
             eg = el * (own + p) * 2 + (klc + entc) * p * (6 * ee + 4 * e * size)
-            # f32 probabilities below 2^-126 have an absolute error: expf's two
-            # steps of 2^-149 and half a step for the rounding, so 2^-147
-            # covers one; it is multiplied by r A, by kl_coef (d - KL) and by
-            # entropy_coef (lp + H), whose factors do not pass 2 size, and
-            # each product rounds at 2^-150 again
-            eg = eg + 2.0 ** -147 * (ra + (abs(klc) + abs(entc)) * 2 * size + 1)
+            # ex2.approx.ftz gives 0 below 2^-126: an absolute error of 2^-126
+            # for a probability, which is multiplied by r A, by kl_coef (d -
+            # KL) and by entropy_coef (lp + H), whose factors do not pass 2
+            # size
+            eg = eg + 2.0 ** -126 * (ra + (abs(klc) + abs(entc)) * 2 * size + 1)
             assert ((d - g).abs() <= w / t * eg + (u + 2.0 ** -20) * g.abs() + t0 +
                     2.0 ** -22 * w / t * ra * (own + p)).all(), (i, k)
     return got
