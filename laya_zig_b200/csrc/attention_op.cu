@@ -20,9 +20,7 @@
 // they hold enters a product: zero rows of Q and dO add nothing to dK and dV,
 // zero rows of K nothing to dQ, and the scores of such keys are masked where
 // the softmax sums them.
-#include <climits>
-
-#include "operators.cuh"
+#include "attention_op.cuh"
 
 namespace laya {
 namespace {
@@ -30,19 +28,6 @@ namespace {
 constexpr int TB = 64;  // rows per tile
 constexpr int THREADS = 128;
 constexpr int TILE = TB * 64;  // elements
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-struct Args {
-    const int* cu;
-    const uint8_t* mask;
-    int* status;
-    int n_seqs, n_tokens, max_len;
-    int group;  // query heads per key head
-    int window;
-    float scale;
-    int skip_len;  // sequences of at least this many tokens are another kernel's
-    AttnIO io;
-};
 
 // element offset of (row, col) in a 64 x 64 16-bit tile whose 16-byte chunks
 // are XORed by row: ldmatrix row fetches never share a bank
@@ -78,42 +63,9 @@ __device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-
-// 16 (or 4) bytes from global to shared memory, zeros where !ok
-__device__ __forceinline__ void copy16(void* s, const void* g, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(s)), "l"(g), "r"(ok ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void copy4(void* s, const void* g, bool ok) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(s)), "l"(g), "r"(ok ? 4 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// Is token `i` of the sequence (any integer) there?
-__device__ __forceinline__ bool present(const Args& a, const SeqTile& t, int i) {
-    return i >= 0 && i < t.len && (!a.mask || a.mask[t.start + i] != 0);
-}
-
 // Rows row0 .. row0 + 63 of the sequence, 64 elements each, into a tile.
 template <typename T>
-__device__ __forceinline__ void load_tile(T* s, const AttnRows& rows, int head, const Args& a, const SeqTile& t,
+__device__ __forceinline__ void load_tile(T* s, const AttnRows& rows, int head, const AttnArgs& a, const SeqTile& t,
                                           int row0) {
     const T* g = static_cast<const T*>(rows.p) + head * 64;
 #pragma unroll
@@ -126,7 +78,7 @@ __device__ __forceinline__ void load_tile(T* s, const AttnRows& rows, int head, 
 }
 
 // Bits of the tile's 64 keys that are there.
-__device__ __forceinline__ void key_bits(uint32_t* bits, const Args& a, const SeqTile& t, int row0) {
+__device__ __forceinline__ void key_bits(uint32_t* bits, const AttnArgs& a, const SeqTile& t, int row0) {
     const int w = threadIdx.x >> 5;
     if (w < 2) {
         const uint32_t b = __ballot_sync(0xffffffffu, present(a, t, row0 + (int)threadIdx.x));
@@ -200,34 +152,17 @@ __device__ __forceinline__ void store_rows(const AttnRows& rows, int head, const
     }
 }
 
-// Tiles [t0, t1) of the sequence that rows row0 .. row0 + 63 see.
-__device__ __forceinline__ void visible_tiles(const Args& a, const SeqTile& t, int* t0, int* t1) {
-    int lo = 0, hi = t.len;
-    if (a.window >= 0) {
-        lo = max(0, t.row0 - a.window);
-        hi = (int)min((long long)t.len, (long long)t.row0 + TB + a.window);
-    }
-    *t0 = lo / TB;
-    *t1 = (hi + TB - 1) / TB;
-}
-
-// Does some pair of the two tiles lie outside the window?
-__device__ __forceinline__ bool edge(int window, int row0, int col0) {
-    return window >= 0 && (row0 + TB - 1 - col0 > window || col0 + TB - 1 - row0 > window);
-}
-
-__device__ __forceinline__ bool block_tile(const Args& a, SeqTile* t) {
+__device__ __forceinline__ bool block_tile(const AttnArgs& a, SeqTile* t) {
     if (threadIdx.x == 0 && blockIdx.y == 0)
         check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, blockIdx.x, a.status);
-    return find_tile(a.cu, a.n_seqs, a.n_tokens, a.max_len, TB, blockIdx.x, threadIdx.x & 31, t) &&
-           t->len < a.skip_len;
+    return find_tile(a.cu, a.n_seqs, a.n_tokens, a.max_len, TB, blockIdx.x, threadIdx.x & 31, t);
 }
 
 // ------------------------------------------------------------------ forward
 constexpr int FWD_SMEM = 5 * TILE * 2;
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const AttnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     T* sq = reinterpret_cast<T*>(smem);
     T* sk = sq + TILE;
@@ -238,7 +173,7 @@ __global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const Args a)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int h = blockIdx.y, hk = h / a.group;
     int kt0, kt1;
-    visible_tiles(a, t, &kt0, &kt1);
+    visible_tiles(a, t, TB, TB, &kt0, &kt1);
     load_tile(sq, a.io.q, h, a, t, t.row0);
     load_tile(sk, a.io.k, hk, a, t, kt0 * TB);
     load_tile(sv, a.io.v, hk, a, t, kt0 * TB);
@@ -265,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const Args a)
         float s[8][4];
         mma_nt<T>(s, qa, sk + b * TILE, lane);
         const uint64_t there = bits[b][0] | (uint64_t)bits[b][1] << 32;
-        if (there != ~0ull || edge(a.window, t.row0, kt * TB)) {
+        if (there != ~0ull || edge(a.window, t.row0, TB, kt * TB, TB)) {
             // element (j, e) of this thread is key kt * 64 + 8 j + 2 (lane & 3) + e
             const int c0 = 2 * (lane & 3), k0 = kt * TB + c0;
             const uint64_t w = there >> c0;
@@ -330,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const Args a)
 constexpr int DQ_SMEM = 6 * TILE * 2;
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const AttnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     T* sq = reinterpret_cast<T*>(smem);
     T* sdo = sq + TILE;
@@ -343,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const Args a) 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int h = blockIdx.y, hk = h / a.group;
     int kt0, kt1;
-    visible_tiles(a, t, &kt0, &kt1);
+    visible_tiles(a, t, TB, TB, &kt0, &kt1);
     load_tile(sq, a.io.q, h, a, t, t.row0);
     load_tile(sdo, a.io.dout, h, a, t, t.row0);
     load_tile(sk, a.io.k, hk, a, t, kt0 * TB);
@@ -412,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const Args a) 
                 s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -e1)) * (dp[j][2 + e] - d1);
             }
         const uint64_t there = bits[b][0] | (uint64_t)bits[b][1] << 32;
-        if (there != ~0ull || edge(a.window, t.row0, kt * TB)) {
+        if (there != ~0ull || edge(a.window, t.row0, TB, kt * TB, TB)) {
             const int c0 = 2 * (lane & 3), k0 = kt * TB + c0;
             const uint64_t w = there >> c0;
 #pragma unroll
@@ -435,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const Args a) 
 constexpr int DKV_SMEM = 6 * TILE * 2 + 2 * 2 * TB * 4;
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const AttnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     T* sk = reinterpret_cast<T*>(smem);
     T* sv = sk + TILE;
@@ -448,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const Args a)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int hk = blockIdx.y;
     int qt0, qt1;
-    visible_tiles(a, t, &qt0, &qt1);  // the window is symmetric
+    visible_tiles(a, t, TB, TB, &qt0, &qt1);
     const int nqt = qt1 - qt0, total = nqt * a.group;
     auto load_q = [&](int it, int b) {
         const int h = hk * a.group + it / nqt, row0 = (qt0 + it % nqt) * TB;
@@ -492,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const Args a)
             s[j][2] = ex2_approx(fmaf(s[j][2], sl2, -e.x * LOG2E));
             s[j][3] = ex2_approx(fmaf(s[j][3], sl2, -e.y * LOG2E));
         }
-        if (edge(a.window, row0, t.row0)) {
+        if (edge(a.window, row0, TB, t.row0, TB)) {
             const int q0 = row0 + c0;
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -520,8 +455,8 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const Args a)
     store_rows<T>(a.io.dv, hk, t, t.row0 + warp * 16, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
 }
 
-Args make_args(const laya_attention& a, const AttnIO& io) {
-    Args g;
+AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
+    AttnArgs g;
     g.cu = a.cu_seqlens;
     g.mask = a.token_mask;
     g.status = a.status;
@@ -531,12 +466,11 @@ Args make_args(const laya_attention& a, const AttnIO& io) {
     g.group = (int)(a.n_heads / a.n_kv_heads);
     g.window = a.window;
     g.scale = a.scale;
-    g.skip_len = INT_MAX;
     g.io = io;
     return g;
 }
 
-cudaError_t launch(void (*kernel)(Args), unsigned heads, int smem, const Args& g, cudaStream_t stream) {
+cudaError_t launch(void (*kernel)(AttnArgs), unsigned heads, int smem, const AttnArgs& g, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), heads);
@@ -546,14 +480,28 @@ cudaError_t launch(void (*kernel)(Args), unsigned heads, int smem, const Args& g
 
 }  // namespace
 
+// Calls whose longest sequence has at least this many tokens go to tcgen05
+// (LAYA_ATTN_OP_TC_MIN_LEN in the environment overrides).
+static uint32_t tc_min_len() {
+    static const uint32_t v = [] {
+        const char* e = getenv("LAYA_ATTN_OP_TC_MIN_LEN");
+        return e && *e ? (uint32_t)strtoul(e, nullptr, 10) : 65u;
+    }();
+    return v;
+}
+
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
+    if (a.max_len >= tc_min_len())
+        return launch_attention_fwd_tc(a.elem_dtype == LAYA_DT_BF16, (int)a.n_heads, make_args(a, io), stream);
     return launch(a.elem_dtype == LAYA_DT_BF16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>,
                   a.n_heads, FWD_SMEM, make_args(a, io), stream);
 }
 
 cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
     const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
-    const Args g = make_args(a, io);
+    const AttnArgs g = make_args(a, io);
+    if (a.max_len >= tc_min_len())
+        return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
     cudaError_t e = launch(bf16 ? attention_dq_kernel<__nv_bfloat16> : attention_dq_kernel<__half>, a.n_heads,
                            DQ_SMEM, g, stream);
     if (e == cudaSuccess)

@@ -1,0 +1,76 @@
+// attention_op.cuh -- what the attention operator's kernels share.
+// attention_op.cu: 64 x 64 tiles on mma.sync; attention_op_tc.cu: tcgen05.
+#pragma once
+#include "operators.cuh"
+
+namespace laya {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnArgs {
+    const int* cu;
+    const uint8_t* mask;
+    int* status;
+    int n_seqs, n_tokens, max_len;
+    int group;  // query heads per key head
+    int window;
+    float scale;
+    AttnIO io;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// 16 (or 4) bytes from global to shared memory, zeros where !ok
+__device__ __forceinline__ void copy16(void* s, const void* g, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(s)), "l"(g), "r"(ok ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(void* s, const void* g, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(s)), "l"(g), "r"(ok ? 4 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Is token `i` of the sequence (any integer) there?
+__device__ __forceinline__ bool present(const AttnArgs& a, const SeqTile& t, int i) {
+    return i >= 0 && i < t.len && (!a.mask || a.mask[t.start + i] != 0);
+}
+
+// Tiles [t0, t1) of `tile` rows of the sequence that rows row0 .. row0 + rows
+// - 1 see (the window is symmetric: keys of queries or queries of keys).
+__device__ __forceinline__ void visible_tiles(const AttnArgs& a, const SeqTile& t, int rows, int tile, int* t0,
+                                              int* t1) {
+    int lo = 0, hi = t.len;
+    if (a.window >= 0) {
+        lo = max(0, t.row0 - a.window);
+        hi = (int)min((long long)t.len, (long long)t.row0 + rows + a.window);
+    }
+    *t0 = lo / tile;
+    *t1 = (hi + tile - 1) / tile;
+}
+
+// Does some pair of rows row0 .. + rows - 1 and col0 .. + cols - 1 lie outside the window?
+__device__ __forceinline__ bool edge(int window, int row0, int rows, int col0, int cols) {
+    return window >= 0 && (row0 + rows - 1 - col0 > window || col0 + cols - 1 - row0 > window);
+}
+
+// attention_op_tc.cu
+cudaError_t launch_attention_fwd_tc(bool bf16, int n_heads, const AttnArgs& a, cudaStream_t stream);
+cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, const AttnArgs& a, cudaStream_t stream);
+
+}  // namespace laya

@@ -35,6 +35,10 @@ struct GemmArgs {
 CUresult make_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint32_t box_rows,
                       bool bf16);
 
+// The same with rows `stride` elements apart (a multiple of 8; base 16-byte aligned).
+CUresult make_tmap_rows(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t stride,
+                        uint32_t box_rows, bool bf16);
+
 // Output tensor map of an epilogue: [rows][inner] row-major, elements of
 // `elem_bytes` (2: 16-bit of the GEMM's type, 4: f32), box of 32 rows x
 // 128 bytes with 128-byte swizzle. The epilogue writes it with TMA stores

@@ -22,7 +22,7 @@ namespace laya {
 namespace {
 
 constexpr int THREADS = 128;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LN2 = 0.6931471805599453f;
 
 struct Scalars {
     const int* cu;
