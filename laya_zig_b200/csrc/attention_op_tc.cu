@@ -1,32 +1,38 @@
 // attention_op_tc.cu -- the attention operator on tcgen05: forward, dQ, and
 // dK with dV (the formulas are in attention_op.cu).
 //
-// One CTA takes 128 rows (queries, or keys for dK and dV) of one head, one to
-// a TMEM lane, and walks the other side in tiles of 64:
+// Two CTAs to an SM walk over the call's items, an item being 128 rows
+// (queries, or keys for dK and dV) of one head, one row to a TMEM lane, which
+// go through the other side in tiles of 64:
 //
-//   warps 0-3  the softmax's arithmetic: thread t owns row t, reads its 64
-//              scores from TMEM, and writes P or dS back as 16-bit pairs over
-//              the scores it has read. A lane's columns are its thread's
+//   warps 0-7  the softmax's arithmetic, in two groups of four warps that take
+//              the tiles in turn: thread t of a group owns row t, reads its 64
+//              scores from TMEM, and writes P or dS back as 16-bit pairs into
+//              the columns it has read. A lane's columns are its thread's
 //              alone, so that needs no barrier among the threads, and the
 //              next product takes P or dS from TMEM as its A operand.
-//   warp 4     loads: TMA boxes of 64 rows x 128 bytes into a ring of STAGES
-//              tile pairs. A box of the packed rows also brings the rows of
-//              absent tokens and of the next sequence; in tiles that have
-//              such rows the warp overwrites them with zeros once the box has
-//              landed, while the next one is on its way, before it hands the
-//              stage over. (The 128-row tile needs none of that: its rows
-//              are the MMA's M index, and nothing crosses from one to another.)
-//   warp 5     owns TMEM and issues the MMAs.
+//   warp 8     finds the items and loads: TMA boxes of 64 rows x 128 bytes
+//              into a ring of STAGES tile pairs. A box of the packed rows also
+//              brings the rows of absent tokens and of the next sequence; in
+//              tiles that have such rows the warp overwrites them with zeros
+//              once the box has landed, while the next one is on its way,
+//              before it hands the stage over. (The 128-row tile needs none
+//              of that: its rows are the MMA's M index, and nothing crosses
+//              from one to another.)
+//   warp 9     owns TMEM and issues the MMAs.
 //
-// TMEM holds 256 columns a CTA (two S tiles, or S and dP; one or two 64-wide
-// accumulators), so two CTAs share an SM: while one waits for a product the
-// other has the SFU, which bounds all three kernels (a 128 x 64 tile costs
-// 512 cycles of ex2 an SM sub-partition, its products 320 to 640).
+// The next item is found and loaded while the present one is computed: at
+// 175-180 tokens an item has three tiles, and finding it, setting up and the
+// first loads took a third of a CTA's time when every item had its own.
+//
+// TMEM holds 256 columns a CTA, four groups to an SM in all: while one waits
+// for a product the others have the SFU (a 128 x 64 tile costs 512 cycles of
+// ex2 an SM sub-partition, its products 320 to 640).
 //
 // TMEM is only overwritten by a product after the barrier that says its last
 // reader is done: MMAs to different accumulators are not taken to be ordered.
-// Every wait is bounded (common.cuh); a CTA that gives up records it, waits
-// for its own copies and MMAs, frees TMEM and leaves.
+// Every wait is bounded; a CTA that gives up records it, waits for its own
+// copies and MMAs, frees TMEM and leaves.
 #include <type_traits>
 
 #include "attention_op.cuh"
@@ -35,42 +41,99 @@
 namespace laya {
 namespace {
 
-constexpr int ROWS = 128;  // rows per CTA, one TMEM lane each
+constexpr int ROWS = 128;  // rows per item, one TMEM lane each
 constexpr int STEP = 64;   // rows of the other side per tile
-constexpr int STAGES = 3;
-constexpr int THREADS = 192;
+constexpr int MAX_STAGES = 3;
 constexpr int BIG = ROWS * 64 * 2;    // 16 KB
 constexpr int SMALL = STEP * 64 * 2;  // 8 KB
-constexpr uint32_t COLS = 256;
+
+// A CTA with G softmax groups, SUMS 64-wide accumulators in TMEM and EXTRA
+// floats in shared memory.
+template <int G_, int BIGS_, int STAGE_BYTES_, int COLS_, int EXTRA_>
+struct Shape {
+    static constexpr int G = G_, BIGS = BIGS_, STAGE_BYTES = STAGE_BYTES_, COLS = COLS_, EXTRA = EXTRA_;
+    static constexpr int STAGES = G == 1 ? 2 : 3;
+    static constexpr int SOFTMAX = G * ROWS;  // threads of the groups
+    static constexpr int LOADER = 4 * G, MMA = 4 * G + 1, THREADS = SOFTMAX + 64;
+    static constexpr int CTAS = G == 1 ? 3 : 2;  // on an SM
+};
+
+// What the loading warp found; n < 0: there is no further item.
+struct Item {
+    int start, len, row0;  // the sequence and the item's first row in it
+    int head;              // of the 128 rows
+    int t0, n;             // its tiles
+};
 
 struct Bars {
-    uint64_t full[STAGES], empty[STAGES], landed[STAGES];
-    uint64_t s_full[2], dp_full;  // products ready for the softmax warps
-    uint64_t p_full, ds_full;     // operands ready for the MMA warp
-    uint64_t done[2];             // the products that read them are complete
-    uint64_t all_done;
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], landed[MAX_STAGES];
+    uint64_t item_full[2], item_empty[2];
+    uint64_t big_full, big_empty;
+    // one of each for each group of softmax warps
+    uint64_t s_full[2], dp_full[2];  // products to read
+    uint64_t s_read[2];              // S has been read: its columns may take dP
+    uint64_t p_full[2];              // P (and dS) written: operands of the next products
+    uint64_t done[2];                // which are complete: the columns may take S again
+    uint64_t acc_full[2], acc_free[2];  // an item's accumulators
+    uint64_t sync[2];                // among the softmax threads
+    uint64_t drained;
     uint32_t tmem;
     int abort;
 };
 
-// Per stage: two words of presence bits (keys), or 64 values each of -lse *
-// log2 e and delta (queries).
-struct Extra {
-    float lse[STAGES][STEP], delta[STAGES][STEP];
-    uint32_t bits[STAGES][2];
+struct Slots {
+    uint32_t bits[MAX_STAGES][2];  // presence of a stage's rows (keys)
+    Item item[2];
 };
-
-constexpr int smem_bytes(int big_tiles) {
-    return big_tiles * BIG + STAGES * 2 * SMALL + (int)sizeof(Bars) + (int)sizeof(Extra) + 16 + 1024;
-}
 
 struct Frame {
-    uint8_t* smem;  // big tiles, then the ring
-    uint8_t* ring;
+    uint8_t* big;    // the 128-row tiles
+    uint8_t* ring;   // STAGES pairs of 64-row tiles
+    uint8_t* stage;  // 2 KB (forward: 4 KB) a softmax warp
     Bars* bar;
-    Extra* extra;
+    Slots* slots;
+    float* extra;  // 16-byte aligned
     uint32_t tmem;
 };
+
+template <typename C>
+constexpr int smem_bytes() {
+    return C::BIGS * BIG + C::STAGES * 2 * SMALL + 4 * C::G * C::STAGE_BYTES + C::EXTRA * 4 + (int)sizeof(Bars) +
+           (int)sizeof(Slots) + 1024;
+}
+
+// mbar_wait (common.cuh), looking at the clock and the abort word only every
+// 32 tries: reading the clock takes some hundred cycles, which a barrier that
+// is about to complete would wait for.
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, int* err, int* abort) {
+    unsigned long long t0 = 0;
+    for (unsigned tries = 1;; tries++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((tries & 31) != 0) continue;
+        if (*(volatile int*)abort) return false;
+        const unsigned long long now = globaltimer();
+        if (tries == 32) t0 = now;
+        if (now - t0 > WAIT_LIMIT_NS) {
+            atomicOr(err, ERR_WAIT_TIMEOUT);
+            *(volatile int*)abort = 1;
+            return false;
+        }
+    }
+}
+
+// Has the phase completed? Unlike mbar_try_wait this returns at once (that one
+// may sleep for thousands of cycles).
+__device__ __forceinline__ bool ready(uint64_t* b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err) {
     const unsigned long long t0 = globaltimer();
@@ -81,7 +144,7 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err) 
         }
 }
 
-// ------------------------------------------------------------------ loads
+// ------------------------------------------------------------------ items and loads
 
 // Presence bits of N * 32 rows of the sequence from row0.
 template <int N>
@@ -90,33 +153,40 @@ __device__ __forceinline__ void row_bits(uint32_t (&bits)[N], const AttnArgs& a,
     for (int i = 0; i < N; i++) bits[i] = __ballot_sync(0xffffffffu, present(a, t, row0 + i * 32 + lane));
 }
 
-// The loading warp's side of the ring. A stage is full when its boxes have
-// landed, zeroed where they must be, and every lane has arrived (32 lanes, and
-// lane 0 once more: with the bytes it expects, or for them).
-struct Ring {
+// The loading warp: items in order, their tiles into the ring. A stage is full
+// when its boxes have landed, zeroed where they must be, and every lane has
+// arrived (32 lanes, and lane 0 once more: with the bytes it expects, or for
+// them).
+template <typename C>
+struct Loader {
+    static constexpr int STAGES = C::STAGES;
     const Frame& f;
     const AttnArgs& a;
-    const CUtensorMap *m0, *m1;
     int lane;
-    int issued = 0;
+    int items = 0, issued = 0;
     int patch = -1;  // the stage that waits for its zeros
     uint32_t patch_bits[2] = {0, 0};
     uint32_t landed_parity = 0;  // one bit a stage
 
+    __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+        if (__all_sync(0xffffffffu, ready(bar, parity))) return true;
+        fill();  // a warp that has to wait first hands over what it holds
+        return __all_sync(0xffffffffu, wait_one(bar, parity, a.status, &f.bar->abort));
+    }
     __device__ __forceinline__ void fill() {
         if (patch < 0) return;
         Bars* bar = f.bar;
-        const bool ok = mbar_wait(&bar->landed[patch], landed_parity >> patch & 1, a.status, &bar->abort);
+        const bool ok = wait_one(&bar->landed[patch], landed_parity >> patch & 1, a.status, &bar->abort);
         landed_parity ^= 1u << patch;
         if (ok) {
             uint8_t* s = f.ring + patch * 2 * SMALL;
             const uint4 zero = make_uint4(0, 0, 0, 0);
+            // 16 lanes a row (both tiles), two rows at a time
+            uint8_t* to = s + (lane >> 3 & 1) * SMALL + (lane >> 4) * 128 + (lane & 7) * 16;
+            const uint32_t there0 = patch_bits[0] >> (lane >> 4), there1 = patch_bits[1] >> (lane >> 4);
 #pragma unroll
-            for (int w = 0; w < 2; w++)
-                for (uint32_t gone = ~patch_bits[w]; gone; gone &= gone - 1) {
-                    const int r = w * 32 + __ffs(gone) - 1;  // 16 lanes a row: both tiles
-                    if (lane < 16) *reinterpret_cast<uint4*>(s + (lane >> 3) * SMALL + r * 128 + (lane & 7) * 16) = zero;
-                }
+            for (int i = 0; i < 32; i++)
+                if (!((i < 16 ? there0 : there1) >> (2 * i & 31) & 1)) *reinterpret_cast<uint4*>(to + i * 256) = zero;
         }
         fence_proxy_async();
         __syncwarp();
@@ -124,33 +194,43 @@ struct Ring {
         mbar_arrive(&bar->full[patch]);
         patch = -1;
     }
-    // Room for the next stage; a warp that has to wait first hands over what it holds.
-    __device__ __forceinline__ bool room() {
-        const int s = issued % STAGES;
-        const uint32_t parity = ((issued / STAGES) & 1) ^ 1;
-        if (__all_sync(0xffffffffu, mbar_try_wait(&f.bar->empty[s], parity))) return true;
-        fill();
-        return __all_sync(0xffffffffu, mbar_wait(&f.bar->empty[s], parity, a.status, &f.bar->abort));
+    // The next item for everyone, and its 128-row tiles (columns `col`) once
+    // the one before has no use for the old ones.
+    __device__ __forceinline__ bool item(const Item& it, const CUtensorMap* b0, const CUtensorMap* b1) {
+        Bars* bar = f.bar;
+        const int s = items & 1;
+        if (!wait(&bar->item_empty[s], ((items >> 1) & 1) ^ 1)) return false;
+        if (lane == 0) {
+            f.slots->item[s] = it;
+            mbar_arrive(&bar->item_full[s]);
+        }
+        if (it.n >= 0) {
+            if (!wait(&bar->big_empty, (items & 1) ^ 1)) return false;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&bar->big_full, C::BIGS * BIG);
+                const int row = it.start + it.row0;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    tma_load_2d(f.big + i * SMALL, b0, &bar->big_full, it.head * 64, row + i * STEP);
+                    if (C::BIGS > 1) tma_load_2d(f.big + BIG + i * SMALL, b1, &bar->big_full, it.head * 64, row + i * STEP);
+                }
+            }
+        }
+        items++;
+        return true;
     }
-    // Rows `row` of both arrays (columns `col0`, `col1`) into the next stage;
-    // with the first go `big` tiles of rows `big_row` (columns `big0`, `big1`).
-    __device__ __forceinline__ void load(int col0, int col1, int row, const uint32_t (&bits)[2], const CUtensorMap* big0,
-                                         const CUtensorMap* big1, int big_col, int big_row) {
+    __device__ __forceinline__ bool room() { return wait(&f.bar->empty[issued % STAGES], ((issued / STAGES) & 1) ^ 1); }
+    // Rows `row` of both arrays (column `col`) into the next stage.
+    __device__ __forceinline__ void tile(const CUtensorMap* m0, const CUtensorMap* m1, int col, int row,
+                                         const uint32_t (&bits)[2]) {
         Bars* bar = f.bar;
         const int s = issued % STAGES;
         const bool whole = (bits[0] & bits[1]) == ~0u;
         if (lane == 0) {
             uint64_t* b = whole ? &bar->full[s] : &bar->landed[s];
-            const bool first = issued == 0;
-            mbar_arrive_expect_tx(b, 2 * SMALL + (first ? (big1 ? 2 : 1) * BIG : 0));
-            if (first) {
-                for (int i = 0; i < 2; i++) {
-                    tma_load_2d(f.smem + i * SMALL, big0, b, big_col, big_row + i * STEP);
-                    if (big1) tma_load_2d(f.smem + BIG + i * SMALL, big1, b, big_col, big_row + i * STEP);
-                }
-            }
-            tma_load_2d(f.ring + 2 * s * SMALL, m0, b, col0, row);
-            tma_load_2d(f.ring + (2 * s + 1) * SMALL, m1, b, col1, row);
+            mbar_arrive_expect_tx(b, 2 * SMALL);
+            tma_load_2d(f.ring + 2 * s * SMALL, m0, b, col, row);
+            tma_load_2d(f.ring + (2 * s + 1) * SMALL, m1, b, col, row);
         }
         issued++;
         fill();
@@ -162,10 +242,45 @@ struct Ring {
             patch_bits[1] = bits[1];
         }
     }
-    // Every box has landed before shared memory goes away.
-    __device__ __forceinline__ void finish() {
+    // Every box has landed before shared memory goes away. `big`: of this many
+    // items the 128-row tiles were asked for.
+    __device__ __forceinline__ void finish(int big) {
         fill();
         for (int j = max(0, issued - STAGES); j < issued; j++) drain(&f.bar->full[j % STAGES], (j / STAGES) & 1, a.status);
+        if (big > 0) drain(&f.bar->big_full, (big - 1) & 1, a.status);
+    }
+};
+
+// Item w of the call (heads first, then tiles of 128 rows): false if it names no rows.
+__device__ __forceinline__ bool find_item(const AttnArgs& a, long long w, int heads, int lane, SeqTile* t, int* head) {
+    const long long x = w / heads;
+    *head = (int)(w - x * heads);
+    if (lane == 0 && *head == 0) check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, x, a.status);
+    return find_tile(a.cu, a.n_seqs, a.n_tokens, a.max_len, ROWS, x, lane, t);
+}
+
+// The k-th item, for every other warp: its slot, until it arrives on item_empty.
+__device__ __forceinline__ bool next_item(const Frame& f, const AttnArgs& a, int k) {
+    Bars* b = f.bar;
+    return wait_one(&b->item_full[k & 1], (k >> 1) & 1, a.status, &b->abort) && f.slots->item[k & 1].n >= 0;
+}
+
+// A softmax group's place: the ring stage of its next tile with that stage's
+// parity, and the parity of the group's own barriers. With two groups its
+// tiles are every other one, whichever items they belong to.
+template <typename C>
+struct Turn {
+    static_assert(C::G <= C::STAGES, "next() wraps at most once");
+    int stage;
+    uint32_t full = 0, own = 0;
+    __device__ __forceinline__ explicit Turn(int group) : stage(group) {}
+    __device__ __forceinline__ void next() {
+        own ^= 1;
+        stage += C::G;
+        if (stage >= C::STAGES) {
+            stage -= C::STAGES;
+            full ^= 1;
+        }
     }
 };
 
@@ -174,6 +289,10 @@ struct Ring {
 __device__ __forceinline__ void load64(uint32_t taddr, float (&v)[64]) {
     tmem_ld32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
     tmem_ld32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+    tc_wait_ld();
+}
+__device__ __forceinline__ void load32(uint32_t taddr, float (&v)[32]) {
+    tmem_ld32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
     tc_wait_ld();
 }
 
@@ -186,15 +305,46 @@ __device__ __forceinline__ void store_pairs(uint32_t taddr, const float* v) {
     tmem_st16(taddr, p);
 }
 
-// A thread's accumulator row (64 columns), times f (0: zeros), to global memory.
+// Two f32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+          "l"(*reinterpret_cast<uint64_t*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// A warp's 32 rows of 32 accumulators, times f (a row's own; 0: zeros), to
+// global memory by way of 2 KB of shared memory: 64 bytes to a row and 8 rows
+// to an instruction instead of 16 bytes to each of 32. g is the first row's
+// address; rows at `rows` and past it are not written.
 template <typename T>
-__device__ __forceinline__ void store_row(uint32_t taddr, T* dst, bool write, float f) {
-    float v[64];
-    load64(taddr, v);
-    if (!write) return;
-    uint4* d = reinterpret_cast<uint4*>(dst);
+__device__ __forceinline__ void store_rows(uint8_t* stage, const float* v, float f, T* g, long long ld, int rows,
+                                           int lane) {
+    __syncwarp();
 #pragma unroll
-    for (int c = 0; c < 8; c++) {
+    for (int c = 0; c < 4; c++) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (f != 0.f) {
             u.x = pack2<T>(v[8 * c] * f, v[8 * c + 1] * f);
@@ -202,21 +352,46 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, bool write, fl
             u.z = pack2<T>(v[8 * c + 4] * f, v[8 * c + 5] * f);
             u.w = pack2<T>(v[8 * c + 6] * f, v[8 * c + 7] * f);
         }
-        d[c] = u;
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)) = u;
+    }
+    __syncwarp();
+    const int c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = i * 8 + (lane >> 2);
+        const uint4 u = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+        if (r < rows) *reinterpret_cast<uint4*>(g + r * ld + c * 8) = u;
     }
 }
 
 // v[i] = to where key col0 + i is not there or lies outside row's window.
 __device__ __forceinline__ void mask_row(float (&v)[64], const uint32_t (&bits)[2], int window, int row, int col0,
                                          float to) {
-    const unsigned span = window >= 0 ? 2u * (unsigned)window : 0xffffffffu;
-    const unsigned d = (unsigned)(col0 - row) + (window >= 0 ? (unsigned)window : 0u);
+    if ((bits[0] & bits[1]) != ~0u) {
 #pragma unroll
-    for (int i = 0; i < 64; i++)
-        if (!(bits[i / 32] >> (i & 31) & 1) || (window >= 0 && d + i > span)) v[i] = to;
+        for (int i = 0; i < 64; i++) v[i] = bits[i / 32] & 1u << (i & 31) ? v[i] : to;
+    }
+    if (window >= 0) {  // col0 + i - (row - window) in [0, 2 window], as one unsigned comparison
+        const unsigned span = 2u * (unsigned)window, d = (unsigned)(col0 - row) + (unsigned)window;
+#pragma unroll
+        for (int i = 0; i < 64; i++) v[i] = d + i <= span ? v[i] : to;
+    }
 }
 
 // ------------------------------------------------------------------ MMAs
+
+// One lane of the warp, chosen by the hardware. Code under it keeps the MMAs'
+// operands in uniform registers; under `lane == 0` four MMAs and two commits
+// took 530 cycles to issue instead of 180.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
 
 template <typename T>
 constexpr uint32_t IDESC = idesc_f16(ROWS, STEP, std::is_same<T, __nv_bfloat16>::value);
@@ -230,45 +405,80 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b) {
         tc_mma_f16(d, sw128_desc(a) + 2 * ks, sw128_desc(b) + 2 * ks, IDESC<T>, ks != 0);
 }
 
-// D (128 x 64) += P . B, P (128 x 64, 16-bit pairs) in TMEM, B's 64 rows summed over.
+// D (128 x 64) += P . B, P (128 x 64, 16-bit pairs, 16 of them every `step`
+// columns) in TMEM, B's 64 rows summed over.
 template <typename T>
-__device__ __forceinline__ void mma_sum(uint32_t d, uint32_t p, uint32_t b, bool accumulate) {
+__device__ __forceinline__ void mma_sum(uint32_t d, uint32_t p, int step, uint32_t b, bool accumulate) {
 #pragma unroll
     for (int ks = 0; ks < 4; ks++)
-        tc_mma_f16_ts(d, p + 8 * ks, sw128_desc(b + ks * 2048), IDESC<T> | B_MN, accumulate || ks != 0);
+        tc_mma_f16_ts(d, p + step * ks, sw128_desc(b + ks * 2048), IDESC<T> | B_MN, accumulate || ks != 0);
 }
+
+// The MMA lane takes whatever is ready next, S, dP or a sum, each kind in the
+// order of the tiles (so an accumulator's order does not depend on timing).
+struct Poll {
+    Bars* bar;
+    int* err;
+    unsigned idle = 0;  // polls since something was ready
+    unsigned long long t0 = 0;
+
+    // False once nothing has been ready for WAIT_LIMIT_NS, or a warp gave up.
+    __device__ __forceinline__ bool go_on(bool moved) {
+        if (moved) {
+            idle = 0;
+            return true;
+        }
+        if ((++idle & 255) != 0) return true;
+        if (*(volatile int*)&bar->abort) return false;
+        const unsigned long long now = globaltimer();
+        if (idle == 256) t0 = now;
+        if (now - t0 <= WAIT_LIMIT_NS) return true;
+        atomicOr(err, ERR_WAIT_TIMEOUT);
+        *(volatile int*)&bar->abort = 1;
+        return false;
+    }
+};
 
 // ------------------------------------------------------------------ CTA frame
 
-template <int BIG_TILES>
+template <typename C>
 __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
     Frame f;
-    f.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    f.ring = f.smem + BIG_TILES * BIG;
-    f.bar = reinterpret_cast<Bars*>(f.ring + STAGES * 2 * SMALL);
-    f.extra = reinterpret_cast<Extra*>(
-        (reinterpret_cast<uintptr_t>(f.bar) + sizeof(Bars) + 15) & ~uintptr_t(15));
+    f.big = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    f.ring = f.big + C::BIGS * BIG;
+    f.stage = f.ring + C::STAGES * 2 * SMALL;
+    f.extra = reinterpret_cast<float*>(f.stage + 4 * C::G * C::STAGE_BYTES);
+    f.bar = reinterpret_cast<Bars*>(f.extra + C::EXTRA);
+    f.slots = reinterpret_cast<Slots*>(f.bar + 1);
+    f.stage += (warp & (4 * C::G - 1)) * C::STAGE_BYTES;
     if (threadIdx.x == 0) {
         Bars* b = f.bar;
-        for (int s = 0; s < STAGES; s++) {
+        for (int s = 0; s < MAX_STAGES; s++) {
             mbar_init(&b->full[s], 33);
             mbar_init(&b->empty[s], 1);
             mbar_init(&b->landed[s], 1);
         }
+        mbar_init(&b->big_full, 1);
+        mbar_init(&b->big_empty, 1);
         for (int s = 0; s < 2; s++) {
+            mbar_init(&b->item_full[s], 1);
+            mbar_init(&b->item_empty[s], C::SOFTMAX + 1);
             mbar_init(&b->s_full[s], 1);
+            mbar_init(&b->dp_full[s], 1);
+            mbar_init(&b->s_read[s], ROWS);
+            mbar_init(&b->p_full[s], ROWS);
             mbar_init(&b->done[s], 1);
+            mbar_init(&b->acc_full[s], 1);
+            mbar_init(&b->acc_free[s], C::SOFTMAX);
+            mbar_init(&b->sync[s], C::SOFTMAX);
         }
-        mbar_init(&b->dp_full, 1);
-        mbar_init(&b->p_full, ROWS);
-        mbar_init(&b->ds_full, ROWS);
-        mbar_init(&b->all_done, 1);
+        mbar_init(&b->drained, 1);
         b->abort = 0;
         fence_barrier_init();
         fence_proxy_async();
     }
-    if (warp == 5) {
-        tmem_alloc(&f.bar->tmem, COLS);
+    if (warp == C::MMA) {
+        tmem_alloc(&f.bar->tmem, C::COLS);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -278,455 +488,619 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
     return f;
 }
 
+template <typename C>
 __device__ __forceinline__ void close_frame(const Frame& f, int warp) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 5) tmem_dealloc(f.tmem, COLS);
-}
-
-__device__ __forceinline__ bool block_tile(const AttnArgs& a, SeqTile* t) {
-    if (threadIdx.x == 0 && blockIdx.y == 0)
-        check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, blockIdx.x, a.status);
-    return find_tile(a.cu, a.n_seqs, a.n_tokens, a.max_len, ROWS, blockIdx.x, threadIdx.x & 31, t);
+    if (warp == C::MMA) tmem_dealloc(f.tmem, C::COLS);
 }
 
 // Warp-wide wait of the softmax warps.
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, const AttnArgs& a, Bars* b) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.status, &b->abort));
+    return __all_sync(0xffffffffu, wait_one(bar, parity, a.status, &b->abort));
 }
 
 // ------------------------------------------------------------------ forward
-constexpr int FWD_SMEM = smem_bytes(1);
+// TMEM: S of group g at column 64 g (P over it); O of group g at 64 (G + g).
+// Two groups exchange halves of their rows of O at an item's end.
+template <int G>
+using Fwd = Shape<G, 1, G == 1 ? 2048 : 4096, 128 * G, G == 1 ? 0 : 4 * ROWS>;
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 2)
+template <typename T, typename C>
+__global__ void __launch_bounds__(C::THREADS, C::CTAS)
     attention_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                             const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap,
-                            const AttnArgs a) {
+                            const AttnArgs a, int heads, long long work) {
     extern __shared__ uint8_t raw[];
-    SeqTile t;
-    if (!block_tile(a, &t)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.y, hk = h / a.group;
-    int kt0, kt1;
-    visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
-    const int n = kt1 - kt0;
-    const Frame f = open_frame<1>(raw, warp);
+    const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
-    // TMEM: S 0, 1 at columns 0, 64 (P over them); O at 128
+    constexpr int G = C::G, STAGES = C::STAGES;
 
-    if (warp == 4) {
-        Ring ring{f, a, &mk, &mv, lane};
-        for (int j = 0; j < n; j++) {
-            uint32_t bits[2];
-            row_bits(bits, a, t, (kt0 + j) * STEP, lane);
-            if (!ring.room()) break;
-            if (lane < 2) f.extra->bits[j % STAGES][lane] = lane ? bits[1] : bits[0];
-            ring.load(hk * 64, hk * 64, t.start + (kt0 + j) * STEP, bits, &mq, nullptr, h * 64, t.start + t.row0);
-        }
-        ring.finish();
-    } else if (warp == 5) {
-        if (lane == 0) {
-            const uint32_t q = smem_u32(f.smem), kv = smem_u32(f.ring);
-            bool ok = true;
-            auto scores = [&](int j) {
-                const int s = j % STAGES;
-                ok = mbar_wait(&bar->full[s], (j / STAGES) & 1, a.status, &bar->abort);
-                if (!ok) return;
-                tc_fence_after();
-                mma_rows<T>(f.tmem + (j & 1) * 64, q, kv + 2 * s * SMALL);
-                tc_commit(&bar->s_full[j & 1]);
-            };
-            scores(0);
-            if (ok && n > 1) scores(1);
-            for (int j = 0; j < n && ok; j++) {
-                const int s = j % STAGES;
-                ok = mbar_wait(&bar->p_full, j & 1, a.status, &bar->abort);
+    if (warp == C::LOADER) {
+        Loader<C> ld{f, a, lane};
+        bool ok = true;
+        for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
+            SeqTile t;
+            int h;
+            if (!find_item(a, w, heads, lane, &t, &h)) continue;
+            int kt0, kt1;
+            visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
+            uint32_t next[2];
+            row_bits(next, a, t, kt0 * STEP, lane);
+            ok = ld.item(Item{t.start, t.len, t.row0, h, kt0, kt1 - kt0}, &mq, nullptr);
+            for (int j = kt0; j < kt1 && ok; j++) {
+                const uint32_t bits[2] = {next[0], next[1]};
+                if (j + 1 < kt1) row_bits(next, a, t, (j + 1) * STEP, lane);
+                ok = ld.room();
                 if (!ok) break;
-                tc_fence_after();
-                mma_sum<T>(f.tmem + 128, f.tmem + (j & 1) * 64, kv + (2 * s + 1) * SMALL, j != 0);
-                tc_commit(&bar->empty[s]);
-                tc_commit(&bar->done[0]);
-                if (j + 2 < n) {
-                    ok = mbar_wait(&bar->done[0], j & 1, a.status, &bar->abort);
-                    if (ok) scores(j + 2);
-                }
+                if (lane < 2) f.slots->bits[ld.issued % C::STAGES][lane] = lane ? bits[1] : bits[0];
+                ld.tile(&mk, &mv, h / a.group * 64, t.start + j * STEP, bits);
             }
-            tc_commit(&bar->all_done);
-            drain(&bar->all_done, 0, a.status);
+            ld.fill();  // before the search for the next item
+        }
+        const int big = ld.items;
+        if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mq, nullptr);
+        ld.finish(big);
+    } else if (warp == C::MMA) {
+        if (elect_one()) {
+            const uint32_t q = smem_u32(f.big), kv = smem_u32(f.ring);
+            Poll poll{bar, a.status};
+            int c = 0;  // tiles of the items before
+            for (int k = 0; next_item(f, a, k); k++) {
+                const int end = c + f.slots->item[k & 1].n;
+                mbar_arrive(&bar->item_empty[k & 1]);
+                int sc = c, pv = c;  // the next tile of each product
+                bool big = false, moved = true;
+                while (pv < end && poll.go_on(moved)) {
+                    moved = false;
+                    if (!big) big = moved = ready(&bar->big_full, k & 1);
+                    if (big && sc < end && sc < pv + G && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
+                        (sc < G || ready(&bar->done[sc % G], (sc / G - 1) & 1))) {
+                        tc_fence_after();
+                        mma_rows<T>(f.tmem + sc % G * 64, q, kv + 2 * (sc % STAGES) * SMALL);
+                        tc_commit(&bar->s_full[sc % G]);
+                        if (++sc == end) tc_commit(&bar->big_empty);
+                        moved = true;
+                    }
+                    if (pv < sc && ready(&bar->p_full[pv % G], (pv / G) & 1) &&
+                        (k == 0 || pv > c || ready(&bar->acc_free[0], (k - 1) & 1))) {
+                        const int s = pv % STAGES, g = pv % G;
+                        tc_fence_after();
+                        mma_sum<T>(f.tmem + (G + g) * 64, f.tmem + g * 64, 8, kv + (2 * s + 1) * SMALL, pv >= c + G);
+                        tc_commit(&bar->empty[s]);
+                        tc_commit(&bar->done[g]);
+                        if (++pv == end) tc_commit(&bar->acc_full[0]);
+                        moved = true;
+                    }
+                }
+                if (pv < end) break;
+                c = end;
+            }
+            tc_commit(&bar->drained);
+            drain(&bar->drained, 0, a.status);
         }
         __syncwarp();
     } else {
-        const int i = t.row0 + threadIdx.x;  // query
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const uint32_t t_o = f.tmem + lanes + 128;
+        const int g = warp >> 2, r = threadIdx.x & (ROWS - 1);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = f.tmem + lanes + g * 64, t_o = t_s + G * 64;
         const float sl2 = a.scale * LOG2E;
         constexpr float RESCALE = 8.0f;  // exponent growth that moves the reference point
-        float m = -INFINITY, l = 0.f;
+        // halves of the rows of O that the groups exchange, 32 columns a warp's 32 rows
+        float* give = reinterpret_cast<float*>(f.stage + (g ? -4 : 4) * C::STAGE_BYTES) + lane;
+        const float* take = reinterpret_cast<const float*>(f.stage) + lane;
+        Turn<C> turn(g);
+        int ahead = g;  // the group's next tile, counted from the item's first
         bool ok = true;
-        for (int j = 0; j < n; j++) {
-            const uint32_t t_s = f.tmem + lanes + (j & 1) * 64;
-            const int s = j % STAGES;
-            ok = wait_all(&bar->full[s], (j / STAGES) & 1, a, bar) && wait_all(&bar->s_full[j & 1], (j >> 1) & 1, a, bar);
-            if (!ok) break;
-            tc_fence_after();
-            float v[64];
-            load64(t_s, v);
-            const uint32_t bits[2] = {f.extra->bits[s][0], f.extra->bits[s][1]};
-            if ((bits[0] & bits[1]) != ~0u || edge(a.window, t.row0, ROWS, (kt0 + j) * STEP, STEP))
-                mask_row(v, bits, a.window, i, (kt0 + j) * STEP, -INFINITY);
-            float mx[8];
-#pragma unroll
-            for (int c = 0; c < 8; c++) mx[c] = fmaxf(v[c], v[c + 8]);
-#pragma unroll
-            for (int c = 16; c < 64; c++) mx[c & 7] = fmaxf(mx[c & 7], v[c]);
-            const float top =
-                fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-            // The reference point moves when the maximum has grown by more
-            // than 2^8 (p stays below 2^8 otherwise): then O and l shrink.
-            float alpha = 1.f;
-            const bool move = j == 0 || (top - m) * sl2 > RESCALE;
-            if (move) {
-                alpha = ex2_approx((m - top) * sl2);  // m = -inf: 0 (NaN if top is -inf too, of an l and O of 0)
-                alpha = m == -INFINITY ? 0.f : alpha;
-                m = top;
-                l *= alpha;
-            }
-            const float u = m == -INFINITY ? 0.f : m * sl2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 64; c++) {
-                v[c] = ex2_approx(fmaf(v[c], sl2, -u));
-                sum[c & 3] += v[c];
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            store_pairs<T>(t_s, v);
-            store_pairs<T>(t_s + 16, v + 32);
-            if (j > 0) {
-                ok = wait_all(&bar->done[0], (j - 1) & 1, a, bar);
+        for (int k = 0; ok; k++) {
+            if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
+            const Item& it = f.slots->item[k & 1];
+            if (G == 2) mbar_arrive(&bar->sync[0]);  // through with the last item's exchange
+            const int n = it.n, row0 = it.row0, t0 = it.t0;
+            const bool mine = ahead < n;  // the item has a tile for this group
+            float m = -INFINITY, l = 0.f;
+            bool first = true;
+            for (; ahead < n; ahead += C::G, turn.next(), first = false) {
+                const int col0 = (t0 + ahead) * STEP;
+                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) && wait_all(&bar->s_full[g], turn.own, a, bar);
                 if (!ok) break;
-                if (__any_sync(0xffffffffu, move)) {
-                    tc_fence_after();
+                tc_fence_after();
+                float v[64];
+                load64(t_s, v);
+                const uint32_t bits[2] = {f.slots->bits[turn.stage][0], f.slots->bits[turn.stage][1]};
+                if ((bits[0] & bits[1]) != ~0u || edge(a.window, row0, ROWS, col0, STEP))
+                    mask_row(v, bits, a.window, row0 + r, col0, -INFINITY);
+                float mx[4];
 #pragma unroll
-                    for (int c = 0; c < 64; c += 32) {
-                        uint32_t r[32];
-                        tmem_ld32(t_o + c, r);
+                for (int e = 0; e < 4; e++) mx[e] = v[e];
+#pragma unroll
+                for (int e = 4; e < 60; e += 8)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) mx[x] = max3(mx[x], v[e + x], v[e + 4 + x]);
+                const float top = fmaxf(max3(max3(mx[0], v[60], v[61]), mx[1], mx[2]), max3(mx[3], v[62], v[63]));
+                // The reference point moves when the maximum has grown by more
+                // than 2^8 (p stays below 2^8 otherwise): then O and l shrink.
+                // S was asked for when P V of the group's tile before was
+                // complete, so O is at rest here.
+                float alpha = 1.f;
+                const bool move = first || (top - m) * sl2 > RESCALE;
+                if (move) {
+                    alpha = m == -INFINITY ? 0.f : ex2_approx((m - top) * sl2);
+                    m = top;
+                    l *= alpha;
+                }
+                if (!first && __any_sync(0xffffffffu, move)) {
+#pragma unroll
+                    for (int e = 0; e < 64; e += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(t_o + e, o);
                         tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-                        tmem_st32(t_o + c, r);
+                        for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+                        tmem_st16(t_o + e, o);
                     }
                 }
+                const float u = m == -INFINITY ? 0.f : m * sl2;
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+#pragma unroll
+                    for (int e = half * 32; e < half * 32 + 32; e += 2) {
+                        const float2 x = fma2(make_float2(v[e], v[e + 1]), make_float2(sl2, sl2), make_float2(-u, -u));
+                        v[e] = ex2_approx(x.x);
+                        v[e + 1] = ex2_approx(x.y);
+                        sum[e / 2 & 1] = add2(sum[e / 2 & 1], make_float2(v[e], v[e + 1]));
+                    }
+                    store_pairs<T>(t_s + half * 16, v + half * 32);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bar->p_full[g]);
             }
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bar->p_full);
-        }
-        if (ok) ok = wait_all(&bar->all_done, 0, a, bar);
-        if (ok) {
+            ahead -= n;
+            ok = ok && wait_all(&bar->acc_full[0], k & 1, a, bar);
+            if (!ok) break;
             tc_fence_after();
-            const bool there = present(a, t, i), write = i < t.len;
-            T* out = static_cast<T*>(a.io.out.p) + ((long long)t.start + (write ? i : 0)) * a.io.out.ld + h * 64;
-            store_row<T>(t_o, out, write, there ? 1.f / l : 0.f);
-            if (a.io.lse && write)
-                a.io.lse[(long long)h * a.n_tokens + t.start + i] = there ? m * a.scale + logf(l) : -INFINITY;
+            const SeqTile t{it.start, it.len, row0};
+            const bool there = present(a, t, row0 + r);
+            const int row = row0 + (warp & 3) * 32;  // the warp's first
+            T* out = static_cast<T*>(a.io.out.p) + ((long long)t.start + row) * a.io.out.ld + it.head * 64;
+            float top = m, sum = l;
+            if constexpr (G == 1) {
+                float o[64];
+                load64(t_o, o);
+                tc_fence_before();
+                mbar_arrive(&bar->acc_free[0]);
+                const float by = there ? 1.f / l : 0.f;
+                store_rows<T>(f.stage, o, by, out, a.io.out.ld, t.len - row, lane);
+                store_rows<T>(f.stage, o + 32, by, out + 32, a.io.out.ld, t.len - row, lane);
+            } else {
+                // The groups' halves of the row are joined: each takes 32
+                // columns of both. A group without a tile (n is 1) takes the
+                // other's.
+                ok = wait_all(&bar->sync[0], k & 1, a, bar);
+                if (!ok) break;
+                const bool two = n > 1;
+                float o[32];
+                if (two) {
+                    load32(t_o + (1 - g) * 32, o);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) give[e * 32] = o[e];
+                }
+                load32(f.tmem + lanes + 128 + (mine ? g : 1 - g) * 64 + g * 32, o);
+                tc_fence_before();
+                mbar_arrive(&bar->acc_free[0]);
+                float2* ml = reinterpret_cast<float2*>(f.extra) + r;  // [group][row]
+                ml[g * ROWS] = make_float2(m, l);
+                mbar_arrive(&bar->sync[1]);
+                ok = wait_all(&bar->sync[1], k & 1, a, bar);
+                if (!ok) break;
+                const float2 other = ml[(1 - g) * ROWS];
+                top = fmaxf(m, other.x);
+                const float u = top == -INFINITY ? 0.f : top;
+                const float f0 = ex2_approx((m - u) * sl2), f1 = ex2_approx((other.x - u) * sl2);
+                sum = l * f0 + other.y * f1;
+                if (two) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = fmaf(o[e], f0, take[e * 32] * f1);
+                }
+                store_rows<T>(f.stage, o, there ? 1.f / sum : 0.f, out + g * 32, a.io.out.ld, t.len - row, lane);
+            }
+            if (a.io.lse && g == 0 && row0 + r < t.len)
+                a.io.lse[(long long)it.head * a.n_tokens + t.start + row0 + r] =
+                    there ? top * a.scale + logf(sum) : -INFINITY;
+            mbar_arrive(&bar->item_empty[k & 1]);
         }
     }
-    close_frame(f, warp);
+    close_frame<C>(f, warp);
+}
+
+// The MMA lane of either backward kernel: S = A0 . R0^T, dP = A1 . R1^T (A:
+// 128-row tiles, R: the ring's), then the sums over the tile's rows.
+template <typename T, typename C, int ACCS, typename Sum>
+__device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a, Sum sums) {
+    constexpr int G = C::G, STAGES = C::STAGES;
+    Bars* bar = f.bar;
+    const uint32_t big0 = smem_u32(f.big), big1 = big0 + BIG, ring = smem_u32(f.ring);
+    Poll poll{bar, a.status};
+    int c = 0;  // tiles of the items before
+    for (int k = 0; next_item(f, a, k); k++) {
+        const int end = c + f.slots->item[k & 1].n, acc = k % ACCS;
+        mbar_arrive(&bar->item_empty[k & 1]);
+        int sc = c, dp = c, sum = c;  // the next tile of each product
+        bool big = false, moved = true;
+        while (sum < end && poll.go_on(moved)) {
+            moved = false;
+            if (!big) big = moved = ready(&bar->big_full, k & 1);
+            if (dp < sc && ready(&bar->s_read[dp % G], (dp / G) & 1)) {
+                tc_fence_after();
+                mma_rows<T>(f.tmem + dp % G * 64, big1, ring + (2 * (dp % STAGES) + 1) * SMALL);
+                tc_commit(&bar->dp_full[dp % G]);
+                if (++dp == end) tc_commit(&bar->big_empty);
+                moved = true;
+            }
+            if (sum < dp && ready(&bar->p_full[sum % G], (sum / G) & 1) &&
+                (k < ACCS || sum > c || ready(&bar->acc_free[acc], (k / ACCS - 1) & 1))) {
+                const int s = sum % STAGES, g = sum % G;
+                tc_fence_after();
+                sums(f.tmem + g * 64, ring + 2 * s * SMALL, acc, sum > c);
+                tc_commit(&bar->empty[s]);
+                tc_commit(&bar->done[g]);
+                if (++sum == end) tc_commit(&bar->acc_full[acc]);
+                moved = true;
+            }
+            if (big && sc < end && sc < sum + G && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
+                (sc < G || ready(&bar->done[sc % G], (sc / G - 1) & 1))) {
+                tc_fence_after();
+                mma_rows<T>(f.tmem + sc % G * 64, big0, ring + 2 * (sc % STAGES) * SMALL);
+                tc_commit(&bar->s_full[sc % G]);
+                sc++;
+                moved = true;
+            }
+        }
+        if (sum < end) break;
+        c = end;
+    }
+    tc_commit(&bar->drained);
+    drain(&bar->drained, 0, a.status);
 }
 
 // ------------------------------------------------------------------ dQ (and delta)
-constexpr int DQ_SMEM = smem_bytes(2);
+// TMEM: S of group g at column 64 g (dP over it, dS over that); dQ at 64 G, with
+// two groups the next item's at 192
+template <int G>
+using Dq = Shape<G, 2, 2048, 128 * G, G == 1 ? 0 : 4 * ROWS>;
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 2)
+template <typename T, typename C>
+__global__ void __launch_bounds__(C::THREADS, C::CTAS)
     attention_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
-                           const AttnArgs a) {
+                           const AttnArgs a, int heads, long long work) {
     extern __shared__ uint8_t raw[];
-    SeqTile t;
-    if (!block_tile(a, &t)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.y, hk = h / a.group;
-    int kt0, kt1;
-    visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
-    const int n = kt1 - kt0;
-    const Frame f = open_frame<2>(raw, warp);
+    const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
-    // TMEM: S 0, 1 at columns 0, 64 (dS over them); dP at 128; dQ at 192
+    constexpr int G = C::G, ACCS = G;  // accumulators in turn
 
-    if (warp == 4) {
-        Ring ring{f, a, &mk, &mv, lane};
-        for (int j = 0; j < n; j++) {
-            uint32_t bits[2];
-            row_bits(bits, a, t, (kt0 + j) * STEP, lane);
-            if (!ring.room()) break;
-            if (lane < 2) f.extra->bits[j % STAGES][lane] = lane ? bits[1] : bits[0];
-            ring.load(hk * 64, hk * 64, t.start + (kt0 + j) * STEP, bits, &mq, &mdo, h * 64, t.start + t.row0);
-        }
-        ring.finish();
-    } else if (warp == 5) {
-        if (lane == 0) {
-            const uint32_t q = smem_u32(f.smem), dout = q + BIG, kv = smem_u32(f.ring);
-            bool ok = true;
-            auto scores = [&](int j) {
-                const int s = j % STAGES;
-                ok = mbar_wait(&bar->full[s], (j / STAGES) & 1, a.status, &bar->abort);
-                if (!ok) return;
-                tc_fence_after();
-                mma_rows<T>(f.tmem + (j & 1) * 64, q, kv + 2 * s * SMALL);
-                tc_commit(&bar->s_full[j & 1]);
-            };
-            auto dp = [&](int j) {
-                mma_rows<T>(f.tmem + 128, dout, kv + (2 * (j % STAGES) + 1) * SMALL);
-                tc_commit(&bar->dp_full);
-            };
-            scores(0);
-            if (ok) dp(0);
-            if (ok && n > 1) scores(1);
-            for (int j = 0; j < n && ok; j++) {
-                const int s = j % STAGES;
-                ok = mbar_wait(&bar->ds_full, j & 1, a.status, &bar->abort);
+    if (warp == C::LOADER) {
+        Loader<C> ld{f, a, lane};
+        bool ok = true;
+        for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
+            SeqTile t;
+            int h;
+            if (!find_item(a, w, heads, lane, &t, &h)) continue;
+            int kt0, kt1;
+            visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
+            uint32_t next[2];
+            row_bits(next, a, t, kt0 * STEP, lane);
+            ok = ld.item(Item{t.start, t.len, t.row0, h, kt0, kt1 - kt0}, &mq, &mdo);
+            for (int j = kt0; j < kt1 && ok; j++) {
+                const uint32_t bits[2] = {next[0], next[1]};
+                if (j + 1 < kt1) row_bits(next, a, t, (j + 1) * STEP, lane);
+                ok = ld.room();
                 if (!ok) break;
-                tc_fence_after();
-                if (j + 1 < n) dp(j + 1);  // dP(j) has been read
-                mma_sum<T>(f.tmem + 192, f.tmem + (j & 1) * 64, kv + 2 * s * SMALL, j != 0);
-                tc_commit(&bar->empty[s]);
-                tc_commit(&bar->done[0]);
-                if (j + 2 < n) {
-                    ok = mbar_wait(&bar->done[0], j & 1, a.status, &bar->abort);
-                    if (ok) scores(j + 2);
-                }
+                if (lane < 2) f.slots->bits[ld.issued % C::STAGES][lane] = lane ? bits[1] : bits[0];
+                ld.tile(&mk, &mv, h / a.group * 64, t.start + j * STEP, bits);
             }
-            tc_commit(&bar->all_done);
-            drain(&bar->all_done, 0, a.status);
+            ld.fill();  // before the search for the next item
         }
+        const int big = ld.items;
+        if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mq, &mdo);
+        ld.finish(big);
+    } else if (warp == C::MMA) {
+        if (elect_one())
+            backward_mmas<T, C, ACCS>(f, a, [&](uint32_t p, uint32_t kv, int acc, bool more) {
+                mma_sum<T>(f.tmem + (G + acc) * 64, p, 8, kv, more);
+            });
         __syncwarp();
     } else {
-        const int r = threadIdx.x, i = t.row0 + r;  // query
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const int g = warp >> 2, r = threadIdx.x & (ROWS - 1);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = f.tmem + lanes + g * 64;
         const float sl2 = a.scale * LOG2E;
-        const bool there = present(a, t, i);
-        const long long at = (long long)h * a.n_tokens + t.start + i;
-        // absent rows have q = dO = 0: any finite lse gives them dS = 0
-        const float e = there ? a.io.lse[at] * LOG2E : 0.f;
-        uint4 o[8];
-        if (there) {
-            const uint4* g = reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.out.p) +
-                                                            ((long long)t.start + i) * a.io.out.ld + h * 64);
+        Turn<C> turn(g);
+        int ahead = g;  // the group's next tile, counted from the item's first
+        bool ok = true;
+        for (int k = 0; ok; k++) {
+            if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
+            const Item& it = f.slots->item[k & 1];
+            const int n = it.n, t0 = it.t0, i = it.row0 + r;  // query
+            const SeqTile t{it.start, it.len, it.row0};
+            const bool there = present(a, t, i);
+            const long long at = (long long)it.head * a.n_tokens + t.start + i;
+            // absent rows are not stored: any finite lse will do
+            const float e = there ? a.io.lse[at] * LOG2E : 0.f;
+            // delta: 8 / G lanes to a row, 4 G rows at a time, so that a row's
+            // elements are read together; then each row's sum to its thread
+            constexpr int LANES = 8 / G, STEPS = 32 / (32 / LANES);
+            float delta = 0.f;
+            {
+                const int row0 = (warp & 3) * 32 + lane / LANES, ch = g * LANES + lane % LANES;
+                uint4 o[STEPS];
+                uint32_t here = 0;
 #pragma unroll
-            for (int c = 0; c < 8; c++) o[c] = g[c];
-        }
-        bool ok = wait_all(&bar->full[0], 0, a, bar);  // dO came with the first keys
-        float delta = 0.f;
-        if (ok) {
-            if (there) {
+                for (int x = 0; x < STEPS; x++) {
+                    const int row = t.row0 + row0 + x * (32 / LANES);
+                    if (present(a, t, row)) {
+                        here |= 1u << x;
+                        o[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.out.p) +
+                                                               ((long long)t.start + row) * a.io.out.ld + it.head * 64 +
+                                                               ch * 8);
+                    }
+                }
+                ok = wait_all(&bar->big_full, k & 1, a, bar);
+                if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    const uint4 d = *reinterpret_cast<const uint4*>(f.smem + BIG + r * 128 + ((c ^ (r & 7)) << 4));
-                    const T* x = reinterpret_cast<const T*>(&o[c]);
-                    const T* y = reinterpret_cast<const T*>(&d);
+                for (int x = 0; x < STEPS; x++) {
+                    const int row = row0 + x * (32 / LANES);
+                    float sum = 0.f;
+                    if (here >> x & 1) {
+                        const uint4 d = *reinterpret_cast<const uint4*>(f.big + BIG + row * 128 + ((ch ^ (row & 7)) << 4));
+                        const T* u = reinterpret_cast<const T*>(&o[x]);
+                        const T* v = reinterpret_cast<const T*>(&d);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) delta = fmaf(to_float(x[k]), to_float(y[k]), delta);
+                        for (int z = 0; z < 8; z++) sum = fmaf(to_float(u[z]), to_float(v[z]), sum);
+                    }
+#pragma unroll
+                    for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                    const float mine = __shfl_sync(0xffffffffu, sum, lane % (32 / LANES) * LANES);
+                    if (lane / (32 / LANES) == x) delta = mine;
                 }
             }
-            if (i < t.len) a.io.delta[at] = delta;
-        }
-        for (int j = 0; j < n && ok; j++) {
-            const uint32_t t_s = f.tmem + lanes + (j & 1) * 64;
-            const int s = j % STAGES;
-            ok = wait_all(&bar->full[s], (j / STAGES) & 1, a, bar) && wait_all(&bar->s_full[j & 1], (j >> 1) & 1, a, bar);
-            if (!ok) break;
-            tc_fence_after();
-            float v[64];
-            load64(t_s, v);
-#pragma unroll
-            for (int c = 0; c < 64; c++) v[c] = ex2_approx(fmaf(v[c], sl2, -e));
-            const uint32_t bits[2] = {f.extra->bits[s][0], f.extra->bits[s][1]};
-            if ((bits[0] & bits[1]) != ~0u || edge(a.window, t.row0, ROWS, (kt0 + j) * STEP, STEP))
-                mask_row(v, bits, a.window, i, (kt0 + j) * STEP, 0.f);
-            ok = wait_all(&bar->dp_full, j & 1, a, bar);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float d[32];
-                tmem_ld32(f.tmem + lanes + 128 + half * 32, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
-                tc_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 32; c++) d[c] = v[half * 32 + c] * (d[c] - delta);
-                store_pairs<T>(t_s + half * 16, d);
+            if constexpr (G == 2) {
+                float* part = f.extra + (k & 1) * 2 * ROWS + r;  // [item's turn][group][row]
+                part[g * ROWS] = delta;
+                mbar_arrive(&bar->sync[0]);
+                ok = wait_all(&bar->sync[0], k & 1, a, bar);
+                if (!ok) break;
+                delta = part[0] + part[ROWS];
             }
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bar->ds_full);
-        }
-        if (ok) ok = wait_all(&bar->all_done, 0, a, bar);
-        if (ok) {
+            if (g == 0 && i < t.len) a.io.delta[at] = delta;
+            for (; ahead < n; ahead += C::G, turn.next()) {
+                const int col0 = (t0 + ahead) * STEP;
+                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) && wait_all(&bar->s_full[g], turn.own, a, bar);
+                if (!ok) break;
+                tc_fence_after();
+                float v[64];
+                load64(t_s, v);
+                tc_fence_before();
+                mbar_arrive(&bar->s_read[g]);
+#pragma unroll
+                for (int x = 0; x < 64; x += 2) {
+                    const float2 y = fma2(make_float2(v[x], v[x + 1]), make_float2(sl2, sl2), make_float2(-e, -e));
+                    v[x] = ex2_approx(y.x);
+                    v[x + 1] = ex2_approx(y.y);
+                }
+                const uint32_t bits[2] = {f.slots->bits[turn.stage][0], f.slots->bits[turn.stage][1]};
+                if ((bits[0] & bits[1]) != ~0u || edge(a.window, i - r, ROWS, col0, STEP))
+                    mask_row(v, bits, a.window, i, col0, 0.f);
+                ok = wait_all(&bar->dp_full[g], turn.own, a, bar);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int x = 0; x < 64; x += 16) {
+                    uint32_t d[16], ds[8];
+                    tmem_ld16(t_s + x, d);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int z = 0; z < 8; z++) {
+                        const float2 y = mul2(make_float2(v[x + 2 * z], v[x + 2 * z + 1]),
+                                              add2(make_float2(__uint_as_float(d[2 * z]), __uint_as_float(d[2 * z + 1])),
+                                                   make_float2(-delta, -delta)));
+                        ds[z] = pack2<T>(y.x, y.y);
+                    }
+                    tmem_st8(t_s + x / 2, ds);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bar->p_full[g]);
+            }
+            ahead -= n;
+            if (ok) ok = wait_all(&bar->acc_full[k % ACCS], (k / ACCS) & 1, a, bar);
+            if (!ok) break;
             tc_fence_after();
-            const bool write = i < t.len;
-            T* dq = static_cast<T*>(a.io.dq.p) + ((long long)t.start + (write ? i : 0)) * a.io.dq.ld + h * 64;
-            store_row<T>(f.tmem + lanes + 192, dq, write, there ? a.scale : 0.f);
+            // each group stores 64 / G columns
+            float d[64 / G];
+            const uint32_t t_acc = f.tmem + lanes + (G + k % ACCS) * 64 + g * 32;
+            if constexpr (G == 1)
+                load64(t_acc, d);
+            else
+                load32(t_acc, d);
+            tc_fence_before();
+            mbar_arrive(&bar->acc_free[k % ACCS]);
+            const int row = it.row0 + (warp & 3) * 32;  // the warp's first
+            const float by = there ? a.scale : 0.f;
+            T* dq = static_cast<T*>(a.io.dq.p) + ((long long)it.start + row) * a.io.dq.ld + it.head * 64 + g * 32;
+            store_rows<T>(f.stage, d, by, dq, a.io.dq.ld, it.len - row, lane);
+            if constexpr (G == 1) store_rows<T>(f.stage, d + 32, by, dq + 32, a.io.dq.ld, it.len - row, lane);
+            mbar_arrive(&bar->item_empty[k & 1]);
         }
     }
-    close_frame(f, warp);
+    close_frame<C>(f, warp);
 }
 
 // ------------------------------------------------------------------ dK, dV
-constexpr int DKV_SMEM = smem_bytes(2);
+// TMEM: S^T of group 0, 1 at columns 0, 64 (dP^T over it, P^T and dS^T over
+// that, 8 columns of each in turn); dV at 128; dK at 192. extra: -lse * log2 e
+// and -delta of each stage's queries.
+using Dkv = Shape<2, 2, 2048, 256, 2 * MAX_STAGES * STEP>;
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 2)
+template <typename T, typename C>
+__global__ void __launch_bounds__(C::THREADS, C::CTAS)
     attention_dkv_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                           const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
-                           const AttnArgs a) {
+                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
+                            const AttnArgs a, int heads, long long work) {
     extern __shared__ uint8_t raw[];
-    SeqTile t;
-    if (!block_tile(a, &t)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int hk = blockIdx.y;
-    int qt0, qt1;
-    visible_tiles(a, t, ROWS, STEP, &qt0, &qt1);
-    const int nq = qt1 - qt0, n = nq * a.group;  // the query tiles of every head of the group
-    const Frame f = open_frame<2>(raw, warp);
+    const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
-    // TMEM: S^T at column 0 (P^T over it); dP^T at 64 (dS^T over it); dV at 128; dK at 192
 
-    if (warp == 4) {
-        Ring ring{f, a, &mq, &mdo, lane};
-        for (int j = 0; j < n; j++) {
-            const int h = hk * a.group + j / nq, row0 = (qt0 + j % nq) * STEP;
-            uint32_t bits[2];
-            row_bits(bits, a, t, row0, lane);
-            // statistics of rows lane and lane + 32 (0 for rows that are not there: q = dO = 0)
-            const long long g = (long long)h * a.n_tokens + t.start + row0 + lane;
-            const bool b0 = bits[0] >> lane & 1, b1 = bits[1] >> lane & 1;
-            const float l0 = b0 ? a.io.lse[g] : 0.f, l1 = b1 ? a.io.lse[g + 32] : 0.f;
-            const float d0 = b0 ? a.io.delta[g] : 0.f, d1 = b1 ? a.io.delta[g + 32] : 0.f;
-            if (!ring.room()) break;
-            const int s = j % STAGES;
-            f.extra->lse[s][lane] = -LOG2E * l0;
-            f.extra->lse[s][lane + 32] = -LOG2E * l1;
-            f.extra->delta[s][lane] = d0;
-            f.extra->delta[s][lane + 32] = d1;
-            ring.load(h * 64, h * 64, t.start + row0, bits, &mk, &mv, hk * 64, t.start + t.row0);
-        }
-        ring.finish();
-    } else if (warp == 5) {
-        if (lane == 0) {
-            const uint32_t k = smem_u32(f.smem), v = k + BIG, qd = smem_u32(f.ring);
-            bool ok = mbar_wait(&bar->full[0], 0, a.status, &bar->abort);
-            if (ok) {
-                tc_fence_after();
-                mma_rows<T>(f.tmem, k, qd);
-                tc_commit(&bar->s_full[0]);
-                mma_rows<T>(f.tmem + 64, v, qd + SMALL);
-                tc_commit(&bar->dp_full);
-            }
+    if (warp == C::LOADER) {
+        Loader<C> ld{f, a, lane};
+        bool ok = true;
+        for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
+            SeqTile t;
+            int hk;
+            if (!find_item(a, w, heads, lane, &t, &hk)) continue;
+            int qt0, qt1;
+            visible_tiles(a, t, ROWS, STEP, &qt0, &qt1);
+            // the query tiles of every head of the group
+            const int n = (qt1 - qt0) * a.group;
+            uint32_t next[2];
+            row_bits(next, a, t, qt0 * STEP, lane);
+            ok = ld.item(Item{t.start, t.len, t.row0, hk, qt0, n}, &mk, &mv);
+            int h = hk * a.group, q = qt0;
             for (int j = 0; j < n && ok; j++) {
-                const int s = j % STAGES, s1 = (j + 1) % STAGES;
-                ok = mbar_wait(&bar->p_full, j & 1, a.status, &bar->abort);
-                if (!ok) break;
-                tc_fence_after();
-                mma_sum<T>(f.tmem + 128, f.tmem, qd + (2 * s + 1) * SMALL, j != 0);
-                tc_commit(&bar->done[0]);
-                if (j + 1 < n) {
-                    ok = mbar_wait(&bar->full[s1], ((j + 1) / STAGES) & 1, a.status, &bar->abort) &&
-                         mbar_wait(&bar->done[0], j & 1, a.status, &bar->abort);
-                    if (!ok) break;
-                    tc_fence_after();
-                    mma_rows<T>(f.tmem, k, qd + 2 * s1 * SMALL);
-                    tc_commit(&bar->s_full[0]);
+                const uint32_t bits[2] = {next[0], next[1]};
+                const int row0 = q * STEP;
+                // statistics of rows lane and lane + 32 (0 for rows that are not there: q = dO = 0)
+                const long long at = (long long)h * a.n_tokens + t.start + row0 + lane;
+                const bool b0 = bits[0] >> lane & 1, b1 = bits[1] >> lane & 1;
+                const float l0 = b0 ? a.io.lse[at] : 0.f, l1 = b1 ? a.io.lse[at + 32] : 0.f;
+                const float d0 = b0 ? a.io.delta[at] : 0.f, d1 = b1 ? a.io.delta[at + 32] : 0.f;
+                const int head = h;
+                if (++q == qt1) {
+                    q = qt0;
+                    h++;
                 }
-                ok = mbar_wait(&bar->ds_full, j & 1, a.status, &bar->abort);
+                if (j + 1 < n) row_bits(next, a, t, q * STEP, lane);
+                ok = ld.room();
                 if (!ok) break;
-                tc_fence_after();
-                mma_sum<T>(f.tmem + 192, f.tmem + 64, qd + 2 * s * SMALL, j != 0);
-                tc_commit(&bar->empty[s]);
-                tc_commit(&bar->done[1]);
-                if (j + 1 < n) {
-                    ok = mbar_wait(&bar->done[1], j & 1, a.status, &bar->abort);
-                    if (!ok) break;
-                    tc_fence_after();
-                    mma_rows<T>(f.tmem + 64, v, qd + (2 * s1 + 1) * SMALL);
-                    tc_commit(&bar->dp_full);
-                }
+                const int s = ld.issued % C::STAGES;
+                float* stat = f.extra + s * 2 * STEP + lane;
+                stat[0] = -LOG2E * l0;
+                stat[32] = -LOG2E * l1;
+                stat[STEP] = -d0;
+                stat[STEP + 32] = -d1;
+                ld.tile(&mq, &mdo, head * 64, t.start + row0, bits);
             }
-            tc_commit(&bar->all_done);
-            drain(&bar->all_done, 0, a.status);
+            ld.fill();  // before the search for the next item
         }
+        const int big = ld.items;
+        if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mk, &mv);
+        ld.finish(big);
+    } else if (warp == C::MMA) {
+        if (elect_one())
+            backward_mmas<T, C, 1>(f, a, [&](uint32_t p, uint32_t qd, int, bool more) {
+                mma_sum<T>(f.tmem + 128, p, 16, qd + SMALL, more);
+                mma_sum<T>(f.tmem + 192, p + 8, 16, qd, more);
+            });
         __syncwarp();
     } else {
-        const int i = t.row0 + threadIdx.x;  // key
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const uint32_t t_s = f.tmem + lanes, t_dp = t_s + 64;
+        const int g = warp >> 2, r = threadIdx.x & (ROWS - 1);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = f.tmem + lanes + g * 64;
         const float sl2 = a.scale * LOG2E;
+        Turn<C> turn(g);
+        int ahead = g;  // the group's next tile, counted from the item's first
         bool ok = true;
-        for (int j = 0; j < n; j++) {
-            const int s = j % STAGES;
-            ok = wait_all(&bar->full[s], (j / STAGES) & 1, a, bar) && wait_all(&bar->s_full[0], j & 1, a, bar);
-            if (!ok) break;
-            tc_fence_after();
-            float v[64];
-            load64(t_s, v);
-            const float4* lse = reinterpret_cast<const float4*>(f.extra->lse[s]);
+        for (int k = 0; ok; k++) {
+            if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
+            const Item& it = f.slots->item[k & 1];
+            const int n = it.n, i = it.row0 + r;  // key
+            for (; ahead < n; ahead += C::G, turn.next()) {
+                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) && wait_all(&bar->s_full[g], turn.own, a, bar);
+                if (!ok) break;
+                tc_fence_after();
+                float v[64];
+                load64(t_s, v);
+                tc_fence_before();
+                mbar_arrive(&bar->s_read[g]);
+                const float4* lse = reinterpret_cast<const float4*>(f.extra + turn.stage * 2 * STEP);
 #pragma unroll
-            for (int c = 0; c < 16; c++) {
-                const float4 e = lse[c];
-                v[4 * c] = ex2_approx(fmaf(v[4 * c], sl2, e.x));
-                v[4 * c + 1] = ex2_approx(fmaf(v[4 * c + 1], sl2, e.y));
-                v[4 * c + 2] = ex2_approx(fmaf(v[4 * c + 2], sl2, e.z));
-                v[4 * c + 3] = ex2_approx(fmaf(v[4 * c + 3], sl2, e.w));
-            }
-            const int row0 = (qt0 + j % nq) * STEP;
-            if (edge(a.window, row0, STEP, t.row0, ROWS)) {
-                const uint32_t all[2] = {~0u, ~0u};
-                mask_row(v, all, a.window, i, row0, 0.f);
-            }
-            store_pairs<T>(t_s, v);
-            store_pairs<T>(t_s + 16, v + 32);
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bar->p_full);
-            ok = wait_all(&bar->dp_full, j & 1, a, bar);
-            if (!ok) break;
-            tc_fence_after();
-            const float4* delta = reinterpret_cast<const float4*>(f.extra->delta[s]);
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float d[32];
-                tmem_ld32(t_dp + half * 32, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
-                tc_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    const float4 e = delta[half * 8 + c];
-                    const float* p = &v[half * 32 + 4 * c];
-                    d[4 * c] = p[0] * (d[4 * c] - e.x);
-                    d[4 * c + 1] = p[1] * (d[4 * c + 1] - e.y);
-                    d[4 * c + 2] = p[2] * (d[4 * c + 2] - e.z);
-                    d[4 * c + 3] = p[3] * (d[4 * c + 3] - e.w);
+                for (int x = 0; x < 16; x++) {
+                    const float4 e = lse[x];
+                    const float2 y = fma2(make_float2(v[4 * x], v[4 * x + 1]), make_float2(sl2, sl2), make_float2(e.x, e.y));
+                    const float2 z =
+                        fma2(make_float2(v[4 * x + 2], v[4 * x + 3]), make_float2(sl2, sl2), make_float2(e.z, e.w));
+                    v[4 * x] = ex2_approx(y.x);
+                    v[4 * x + 1] = ex2_approx(y.y);
+                    v[4 * x + 2] = ex2_approx(z.x);
+                    v[4 * x + 3] = ex2_approx(z.y);
                 }
-                store_pairs<T>(t_dp + half * 16, d);
+                if (a.window >= 0) {
+                    const int row0 = (it.t0 + ahead % (n / a.group)) * STEP;
+                    if (edge(a.window, row0, STEP, i - r, ROWS)) {
+                        const uint32_t all[2] = {~0u, ~0u};
+                        mask_row(v, all, a.window, i, row0, 0.f);
+                    }
+                }
+                ok = wait_all(&bar->dp_full[g], turn.own, a, bar);
+                if (!ok) break;
+                tc_fence_after();
+                const float4* delta = lse + STEP / 4;
+#pragma unroll
+                for (int x = 0; x < 64; x += 16) {
+                    uint32_t d[16], w[16];  // 16 of dP, then 16 of P and 16 of dS in pairs
+                    tmem_ld16(t_s + x, d);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int z = 0; z < 4; z++) {
+                        const float4 e = delta[x / 4 + z];
+                        const float2 p0 = make_float2(v[x + 4 * z], v[x + 4 * z + 1]);
+                        const float2 p1 = make_float2(v[x + 4 * z + 2], v[x + 4 * z + 3]);
+                        const float2 y0 = add2(make_float2(__uint_as_float(d[4 * z]), __uint_as_float(d[4 * z + 1])),
+                                               make_float2(e.x, e.y));
+                        const float2 y1 = add2(make_float2(__uint_as_float(d[4 * z + 2]), __uint_as_float(d[4 * z + 3])),
+                                               make_float2(e.z, e.w));
+                        const float2 s0 = mul2(p0, y0), s1 = mul2(p1, y1);
+                        w[2 * z] = pack2<T>(p0.x, p0.y);
+                        w[2 * z + 1] = pack2<T>(p1.x, p1.y);
+                        w[8 + 2 * z] = pack2<T>(s0.x, s0.y);
+                        w[9 + 2 * z] = pack2<T>(s1.x, s1.y);
+                    }
+                    tmem_st16(t_s + x, w);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bar->p_full[g]);
             }
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bar->ds_full);
-        }
-        if (ok) ok = wait_all(&bar->all_done, 0, a, bar);
-        if (ok) {
+            ahead -= n;
+            if (ok) ok = wait_all(&bar->acc_full[0], k & 1, a, bar);
+            if (!ok) break;
             tc_fence_after();
-            const bool there = present(a, t, i), write = i < t.len;
-            const long long row = (long long)t.start + (write ? i : 0);
-            store_row<T>(t_s + 192, static_cast<T*>(a.io.dk.p) + row * a.io.dk.ld + hk * 64, write,
-                         there ? a.scale : 0.f);
-            store_row<T>(t_s + 128, static_cast<T*>(a.io.dv.p) + row * a.io.dv.ld + hk * 64, write, there ? 1.f : 0.f);
+            // group 0 stores dV, group 1 dK
+            float d[64];
+            load64(f.tmem + lanes + 128 + g * 64, d);
+            tc_fence_before();
+            mbar_arrive(&bar->acc_free[0]);
+            const SeqTile t{it.start, it.len, it.row0};
+            const float by = !present(a, t, i) ? 0.f : g ? a.scale : 1.f;
+            const AttnRows& out = g ? a.io.dk : a.io.dv;
+            const int row = it.row0 + (warp & 3) * 32;  // the warp's first
+            T* to = static_cast<T*>(out.p) + ((long long)it.start + row) * out.ld + it.head * 64;
+            store_rows<T>(f.stage, d, by, to, out.ld, it.len - row, lane);
+            store_rows<T>(f.stage, d + 32, by, to + 32, out.ld, it.len - row, lane);
+            mbar_arrive(&bar->item_empty[k & 1]);
         }
     }
-    close_frame(f, warp);
+    close_frame<C>(f, warp);
 }
 
-using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnArgs);
+using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnArgs, int, long long);
 
 struct Maps {
     CUtensorMap q, k, v, dout;
@@ -736,12 +1110,29 @@ bool map_rows(CUtensorMap* m, const AttnRows& r, int heads, const AttnArgs& a, b
     return make_tmap_rows(m, r.p, (uint64_t)heads * 64, (uint64_t)a.n_tokens, (uint64_t)r.ld, STEP, bf16) == CUDA_SUCCESS;
 }
 
-cudaError_t launch(Kernel kernel, unsigned heads, int smem, const Maps& m, const AttnArgs& a, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+        return 148;
+    return sms;
+}
+
+template <typename C>
+cudaError_t launch(Kernel kernel, int heads, const Maps& m, const AttnArgs& a, int sms, cudaStream_t stream) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<C>());
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)seq_tiles(a.n_tokens, a.n_seqs, ROWS), heads);
-    kernel<<<grid, THREADS, smem, stream>>>(m.q, m.k, m.v, m.dout, a);
+    const long long work = seq_tiles(a.n_tokens, a.n_seqs, ROWS) * heads, most = (long long)C::CTAS * sms;
+    kernel<<<(unsigned)(work < most ? work : most), C::THREADS, smem_bytes<C>(), stream>>>(m.q, m.k, m.v, m.dout, a,
+                                                                                          heads, work);
     return cudaGetLastError();
+}
+
+// One group a CTA or two?
+bool solo(int heads, const AttnArgs& a, int sms) {
+    const char* e = getenv("SOLO");
+    if (e) return e[0] == '1';
+    return a.max_len <= 1024;
 }
 
 }  // namespace
@@ -753,8 +1144,12 @@ cudaError_t launch_attention_fwd_tc(bool bf16, int n_heads, const AttnArgs& a, c
         !map_rows(&m.v, a.io.v, kv, a, bf16))
         return cudaErrorInvalidValue;
     m.dout = m.q;  // not used
-    return launch(bf16 ? attention_fwd_tc_kernel<__nv_bfloat16> : attention_fwd_tc_kernel<__half>, n_heads, FWD_SMEM,
-                  m, a, stream);
+    const int sms = sm_count();
+    if (solo(n_heads, a, sms))
+        return launch<Fwd<1>>(bf16 ? attention_fwd_tc_kernel<__nv_bfloat16, Fwd<1>> : attention_fwd_tc_kernel<__half, Fwd<1>>,
+                              n_heads, m, a, sms, stream);
+    return launch<Fwd<2>>(bf16 ? attention_fwd_tc_kernel<__nv_bfloat16, Fwd<2>> : attention_fwd_tc_kernel<__half, Fwd<2>>,
+                          n_heads, m, a, sms, stream);
 }
 
 cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, const AttnArgs& a, cudaStream_t stream) {
@@ -762,11 +1157,16 @@ cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, cons
     if (!map_rows(&m.q, a.io.q, n_heads, a, bf16) || !map_rows(&m.k, a.io.k, n_kv_heads, a, bf16) ||
         !map_rows(&m.v, a.io.v, n_kv_heads, a, bf16) || !map_rows(&m.dout, a.io.dout, n_heads, a, bf16))
         return cudaErrorInvalidValue;
-    cudaError_t e = launch(bf16 ? attention_dq_tc_kernel<__nv_bfloat16> : attention_dq_tc_kernel<__half>, n_heads,
-                           DQ_SMEM, m, a, stream);
+    const int sms = sm_count();
+    cudaError_t e =
+        solo(n_heads, a, sms)
+            ? launch<Dq<1>>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq<1>> : attention_dq_tc_kernel<__half, Dq<1>>,
+                            n_heads, m, a, sms, stream)
+            : launch<Dq<2>>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq<2>> : attention_dq_tc_kernel<__half, Dq<2>>,
+                            n_heads, m, a, sms, stream);
     if (e == cudaSuccess)
-        e = launch(bf16 ? attention_dkv_tc_kernel<__nv_bfloat16> : attention_dkv_tc_kernel<__half>, n_kv_heads,
-                   DKV_SMEM, m, a, stream);
+        e = launch<Dkv>(bf16 ? attention_dkv_tc_kernel<__nv_bfloat16, Dkv> : attention_dkv_tc_kernel<__half, Dkv>,
+                        n_kv_heads, m, a, sms, stream);
     return e;
 }
 
