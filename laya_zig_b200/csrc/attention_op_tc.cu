@@ -345,14 +345,14 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, const float* v, float
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (f != 0.f) {
-            u.x = pack2<T>(v[8 * c] * f, v[8 * c + 1] * f);
-            u.y = pack2<T>(v[8 * c + 2] * f, v[8 * c + 3] * f);
-            u.z = pack2<T>(v[8 * c + 4] * f, v[8 * c + 5] * f);
-            u.w = pack2<T>(v[8 * c + 6] * f, v[8 * c + 7] * f);
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 x = mul2(make_float2(v[8 * c + 2 * e], v[8 * c + 2 * e + 1]), make_float2(f, f));
+            u[e] = f == 0.f ? 0u : pack2<T>(x.x, x.y);  // whatever the accumulator holds
         }
-        *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)) = u;
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)) =
+            make_uint4(u[0], u[1], u[2], u[3]);
     }
     __syncwarp();
     const int c = lane & 3;
@@ -768,11 +768,39 @@ __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a,
     drain(&bar->drained, 0, a.status);
 }
 
-// ------------------------------------------------------------------ dQ (and delta)
+// ------------------------------------------------------------------ delta
+// delta[h][t] = sum_d dO O, a thread to 8 elements, 8 lanes to a row of a head.
+// Bound by memory (both arrays once). Inside the dQ kernel, whose warps are
+// few, it took a third of an item's time at 175-180 tokens.
+constexpr int DELTA_THREADS = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const AttnArgs a, int heads) {
+    const int n = a.n_seqs;
+    const int first = max(a.cu[0], 0), last = min(a.cu[n], a.n_tokens);  // rows past either are not the call's
+    const long long at = ((long long)blockIdx.x * DELTA_THREADS + threadIdx.x) / 8;
+    const int c = threadIdx.x & 7;
+    const int t = (int)(at / heads), h = (int)(at - (long long)t * heads);
+    const bool ok = t >= first && t < last && (!a.mask || a.mask[t] != 0);
+    float sum = 0.f;
+    if (ok) {
+        const uint4 o = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.out.p) + t * a.io.out.ld + h * 64 + c * 8);
+        const uint4 d = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.dout.p) + t * a.io.dout.ld + h * 64 + c * 8);
+        const T* x = reinterpret_cast<const T*>(&o);
+        const T* y = reinterpret_cast<const T*>(&d);
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum = fmaf(to_float(x[k]), to_float(y[k]), sum);
+    }
+#pragma unroll
+    for (int k = 1; k < 8; k *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if (ok && c == 0) a.io.delta[(long long)h * a.n_tokens + t] = sum;
+}
+
+// ------------------------------------------------------------------ dQ
 // TMEM: S of group g at column 64 g (dP over it, dS over that); dQ at 64 G, with
 // two groups the next item's at 192
 template <int G>
-using Dq = Shape<G, 2, 2048, 128 * G, G == 1 ? 0 : 4 * ROWS>;
+using Dq = Shape<G, 2, 2048, 128 * G, 0>;
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS)
@@ -831,54 +859,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
             const SeqTile t{it.start, it.len, it.row0};
             const bool there = present(a, t, i);
             const long long at = (long long)it.head * a.n_tokens + t.start + i;
-            // absent rows are not stored: any finite lse will do
-            const float e = there ? a.io.lse[at] * LOG2E : 0.f;
-            // delta: 8 / G lanes to a row, 4 G rows at a time, so that a row's
-            // elements are read together; then each row's sum to its thread
-            constexpr int LANES = 8 / G, STEPS = 32 / (32 / LANES);
-            float delta = 0.f;
-            {
-                const int row0 = (warp & 3) * 32 + lane / LANES, ch = g * LANES + lane % LANES;
-                uint4 o[STEPS];
-                uint32_t here = 0;
-#pragma unroll
-                for (int x = 0; x < STEPS; x++) {
-                    const int row = t.row0 + row0 + x * (32 / LANES);
-                    if (present(a, t, row)) {
-                        here |= 1u << x;
-                        o[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.out.p) +
-                                                               ((long long)t.start + row) * a.io.out.ld + it.head * 64 +
-                                                               ch * 8);
-                    }
-                }
-                ok = wait_all(&bar->big_full, k & 1, a, bar);
-                if (!ok) break;
-#pragma unroll
-                for (int x = 0; x < STEPS; x++) {
-                    const int row = row0 + x * (32 / LANES);
-                    float sum = 0.f;
-                    if (here >> x & 1) {
-                        const uint4 d = *reinterpret_cast<const uint4*>(f.big + BIG + row * 128 + ((ch ^ (row & 7)) << 4));
-                        const T* u = reinterpret_cast<const T*>(&o[x]);
-                        const T* v = reinterpret_cast<const T*>(&d);
-#pragma unroll
-                        for (int z = 0; z < 8; z++) sum = fmaf(to_float(u[z]), to_float(v[z]), sum);
-                    }
-#pragma unroll
-                    for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                    const float mine = __shfl_sync(0xffffffffu, sum, lane % (32 / LANES) * LANES);
-                    if (lane / (32 / LANES) == x) delta = mine;
-                }
-            }
-            if constexpr (G == 2) {
-                float* part = f.extra + (k & 1) * 2 * ROWS + r;  // [item's turn][group][row]
-                part[g * ROWS] = delta;
-                mbar_arrive(&bar->sync[0]);
-                ok = wait_all(&bar->sync[0], k & 1, a, bar);
-                if (!ok) break;
-                delta = part[0] + part[ROWS];
-            }
-            if (g == 0 && i < t.len) a.io.delta[at] = delta;
+            // absent rows are not stored: any finite values will do
+            const float e = there ? a.io.lse[at] * LOG2E : 0.f, delta = there ? a.io.delta[at] : 0.f;
             for (; ahead < n; ahead += C::G, turn.next()) {
                 const int col0 = (t0 + ahead) * STEP;
                 ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) && wait_all(&bar->s_full[g], turn.own, a, bar);
@@ -1158,8 +1140,15 @@ cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, cons
         !map_rows(&m.v, a.io.v, n_kv_heads, a, bf16) || !map_rows(&m.dout, a.io.dout, n_heads, a, bf16))
         return cudaErrorInvalidValue;
     const int sms = sm_count();
-    cudaError_t e =
-        solo(n_heads, a, sms)
+    const long long threads = (long long)a.n_tokens * n_heads * 8;
+    const unsigned blocks = (unsigned)((threads + DELTA_THREADS - 1) / DELTA_THREADS);
+    if (bf16)
+        attention_delta_kernel<__nv_bfloat16><<<blocks, DELTA_THREADS, 0, stream>>>(a, n_heads);
+    else
+        attention_delta_kernel<__half><<<blocks, DELTA_THREADS, 0, stream>>>(a, n_heads);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    e = solo(n_heads, a, sms)
             ? launch<Dq<1>>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq<1>> : attention_dq_tc_kernel<__half, Dq<1>>,
                             n_heads, m, a, sms, stream)
             : launch<Dq<2>>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq<2>> : attention_dq_tc_kernel<__half, Dq<2>>,
