@@ -296,15 +296,6 @@ __device__ __forceinline__ void load32(uint32_t taddr, float (&v)[32]) {
     tc_wait_ld();
 }
 
-// 32 values as 16-bit pairs into 16 columns.
-template <typename T>
-__device__ __forceinline__ void store_pairs(uint32_t taddr, const float* v) {
-    uint32_t p[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) p[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-    tmem_st16(taddr, p);
-}
-
 // Two f32 operations an instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     uint64_t d;
@@ -333,6 +324,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+// The two values of a 16-bit pair.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t p);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p) {
+    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t p) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&p));
 }
 
 // A warp's 32 rows of 32 accumulators, times f (a row's own; 0: zeros), to
@@ -645,15 +648,17 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 const float u = m == -INFINITY ? 0.f : m * sl2;
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
+                for (int e = 0; e < 64; e += 16) {
+                    uint32_t p[8];
 #pragma unroll
-                    for (int e = half * 32; e < half * 32 + 32; e += 2) {
-                        const float2 x = fma2(make_float2(v[e], v[e + 1]), make_float2(sl2, sl2), make_float2(-u, -u));
-                        v[e] = ex2_approx(x.x);
-                        v[e + 1] = ex2_approx(x.y);
-                        sum[e / 2 & 1] = add2(sum[e / 2 & 1], make_float2(v[e], v[e + 1]));
+                    for (int x = 0; x < 8; x++) {
+                        const float2 y = fma2(make_float2(v[e + 2 * x], v[e + 2 * x + 1]), make_float2(sl2, sl2),
+                                              make_float2(-u, -u));
+                        const float2 q = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                        sum[x & 1] = add2(sum[x & 1], q);
+                        p[x] = pack2<T>(q.x, q.y);
                     }
-                    store_pairs<T>(t_s + half * 16, v + half * 32);
+                    tmem_st8(t_s + e / 2, p);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tc_wait_st();
@@ -870,15 +875,17 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 load64(t_s, v);
                 tc_fence_before();
                 mbar_arrive(&bar->s_read[g]);
-#pragma unroll
-                for (int x = 0; x < 64; x += 2) {
-                    const float2 y = fma2(make_float2(v[x], v[x + 1]), make_float2(sl2, sl2), make_float2(-e, -e));
-                    v[x] = ex2_approx(y.x);
-                    v[x + 1] = ex2_approx(y.y);
-                }
                 const uint32_t bits[2] = {f.slots->bits[turn.stage][0], f.slots->bits[turn.stage][1]};
                 if ((bits[0] & bits[1]) != ~0u || edge(a.window, i - r, ROWS, col0, STEP))
-                    mask_row(v, bits, a.window, i, col0, 0.f);
+                    mask_row(v, bits, a.window, i, col0, -INFINITY);
+                // P as 16-bit pairs, which is how it waits for dP: in 32 bits
+                // the row would not fit the thread's 96 registers
+                uint32_t p[32];
+#pragma unroll
+                for (int x = 0; x < 32; x++) {
+                    const float2 y = fma2(make_float2(v[2 * x], v[2 * x + 1]), make_float2(sl2, sl2), make_float2(-e, -e));
+                    p[x] = pack2<T>(ex2_approx(y.x), ex2_approx(y.y));
+                }
                 ok = wait_all(&bar->dp_full[g], turn.own, a, bar);
                 if (!ok) break;
                 tc_fence_after();
@@ -889,7 +896,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                     tc_wait_ld();
 #pragma unroll
                     for (int z = 0; z < 8; z++) {
-                        const float2 y = mul2(make_float2(v[x + 2 * z], v[x + 2 * z + 1]),
+                        const float2 y = mul2(unpack2<T>(p[x / 2 + z]),
                                               add2(make_float2(__uint_as_float(d[2 * z]), __uint_as_float(d[2 * z + 1])),
                                                    make_float2(-delta, -delta)));
                         ds[z] = pack2<T>(y.x, y.y);
@@ -1011,24 +1018,23 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 load64(t_s, v);
                 tc_fence_before();
                 mbar_arrive(&bar->s_read[g]);
+                if (a.window >= 0) {
+                    const int row0 = (it.t0 + ahead % (n / a.group)) * STEP;
+                    if (edge(a.window, row0, STEP, i - r, ROWS)) {
+                        const uint32_t all[2] = {~0u, ~0u};
+                        mask_row(v, all, a.window, i, row0, -INFINITY);
+                    }
+                }
                 const float4* lse = reinterpret_cast<const float4*>(f.extra + turn.stage * 2 * STEP);
+                uint32_t p[32];  // P in 16-bit pairs, as dV's product takes it; dS uses the same values
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
                     const float4 e = lse[x];
                     const float2 y = fma2(make_float2(v[4 * x], v[4 * x + 1]), make_float2(sl2, sl2), make_float2(e.x, e.y));
                     const float2 z =
                         fma2(make_float2(v[4 * x + 2], v[4 * x + 3]), make_float2(sl2, sl2), make_float2(e.z, e.w));
-                    v[4 * x] = ex2_approx(y.x);
-                    v[4 * x + 1] = ex2_approx(y.y);
-                    v[4 * x + 2] = ex2_approx(z.x);
-                    v[4 * x + 3] = ex2_approx(z.y);
-                }
-                if (a.window >= 0) {
-                    const int row0 = (it.t0 + ahead % (n / a.group)) * STEP;
-                    if (edge(a.window, row0, STEP, i - r, ROWS)) {
-                        const uint32_t all[2] = {~0u, ~0u};
-                        mask_row(v, all, a.window, i, row0, 0.f);
-                    }
+                    p[2 * x] = pack2<T>(ex2_approx(y.x), ex2_approx(y.y));
+                    p[2 * x + 1] = pack2<T>(ex2_approx(z.x), ex2_approx(z.y));
                 }
                 ok = wait_all(&bar->dp_full[g], turn.own, a, bar);
                 if (!ok) break;
@@ -1042,15 +1048,13 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
 #pragma unroll
                     for (int z = 0; z < 4; z++) {
                         const float4 e = delta[x / 4 + z];
-                        const float2 p0 = make_float2(v[x + 4 * z], v[x + 4 * z + 1]);
-                        const float2 p1 = make_float2(v[x + 4 * z + 2], v[x + 4 * z + 3]);
                         const float2 y0 = add2(make_float2(__uint_as_float(d[4 * z]), __uint_as_float(d[4 * z + 1])),
                                                make_float2(e.x, e.y));
                         const float2 y1 = add2(make_float2(__uint_as_float(d[4 * z + 2]), __uint_as_float(d[4 * z + 3])),
                                                make_float2(e.z, e.w));
-                        const float2 s0 = mul2(p0, y0), s1 = mul2(p1, y1);
-                        w[2 * z] = pack2<T>(p0.x, p0.y);
-                        w[2 * z + 1] = pack2<T>(p1.x, p1.y);
+                        w[2 * z] = p[x / 2 + 2 * z];
+                        w[2 * z + 1] = p[x / 2 + 2 * z + 1];
+                        const float2 s0 = mul2(unpack2<T>(w[2 * z]), y0), s1 = mul2(unpack2<T>(w[2 * z + 1]), y1);
                         w[8 + 2 * z] = pack2<T>(s0.x, s0.y);
                         w[9 + 2 * z] = pack2<T>(s1.x, s1.y);
                     }

@@ -78,7 +78,8 @@ def attention_bounds(q, k, v, scale, p, out, lse, u, t0, dout=None, grads=None):
     exp of that, ex2.approx (2^-22), the row sum or, in the backward pass, the
     rounding of lse times log2 e: relative e_p = 2 e_s + 2^-20 + 2^-22 |lse|.
     The product operands P and dS are rounded to 16 bits (u relative, t0
-    absolute among the subnormals), results once more. P enters the products
+    absolute among the subnormals), dS perhaps from the rounded P (so 2 u, and
+    t0 times |dP - delta|), results once more. P enters the products
     after exp2 of a difference from the row's maximum or from lse; both are
     <= 1 (or below 2^8 with its own relative rounding), so t0 counts 256
     times at most. ex2.approx.ftz gives 0 below 2^-126: an absolute error of
@@ -104,9 +105,9 @@ def attention_bounds(q, k, v, scale, p, out, lse, u, t0, dout=None, grads=None):
     delta = (dout * out).sum(-1).t()[..., None]
     # delta comes from the out the forward left, itself off by b["out"]
     e_delta = ((d_out * (b["out"] + 70 * F32 * out.abs())).sum(-1)).t()[..., None]
-    e_ds = p * (ep[..., None] * (dp - delta).abs() + 70 * F32 * dp_abs + e_delta) + u * (p * (dp - delta)).abs()
+    e_ds = p * (ep[..., None] * (dp - delta).abs() + 70 * F32 * dp_abs + e_delta) + 2 * u * (p * (dp - delta)).abs()
     flushed = 2.0 ** -126
-    e_ds = e_ds * (1 + 4 * u) + (t0 + flushed * (dp - delta).abs()) * seen
+    e_ds = e_ds * (1 + 4 * u) + (t0 + (t0 + flushed) * (dp - delta).abs()) * seen
 
     def shared(x):  # sum over the heads that share a key head
         return x.reshape(x.shape[0], k.shape[1], rep, 64).sum(2)
