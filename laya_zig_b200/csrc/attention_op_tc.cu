@@ -5,12 +5,15 @@
 // (queries, or keys for dK and dV) of one head, one row to a TMEM lane, which
 // go through the other side in tiles of 64:
 //
-//   warps 0-7  the softmax's arithmetic, in two groups of four warps that take
-//              the tiles in turn: thread t of a group owns row t, reads its 64
-//              scores from TMEM, and writes P or dS back as 16-bit pairs into
-//              the columns it has read. A lane's columns are its thread's
-//              alone, so that needs no barrier among the threads, and the
-//              next product takes P or dS from TMEM as its A operand.
+//   warps 0-7  the softmax's arithmetic, in two groups of four warps: thread t
+//              of either owns row t, of which group g reads columns 32 g .. 32
+//              g + 31 of the tile's scores from TMEM and writes P or dS back
+//              as 16-bit pairs into the columns it has read. A lane's columns
+//              of a group are its thread's alone, so that needs no barrier
+//              among the threads, and the next product takes P or dS from
+//              TMEM as its A operand. (In the forward each group has its own
+//              maximum, sum and O over its half of the keys; they are joined
+//              at the item's end.)
 //   warp 8     finds the items and loads: TMA boxes of 64 rows x 128 bytes
 //              into a ring of STAGES tile pairs. A box of the packed rows also
 //              brings the rows of absent tokens and of the next sequence; in
@@ -25,9 +28,10 @@
 // 175-180 tokens an item has three tiles, and finding it, setting up and the
 // first loads took a third of a CTA's time when every item had its own.
 //
-// TMEM holds 256 columns a CTA, four groups to an SM in all: while one waits
-// for a product the others have the SFU (a 128 x 64 tile costs 512 cycles of
-// ex2 an SM sub-partition, its products 320 to 640).
+// TMEM holds 256 columns a CTA: two buffers for scores, so that a tile's are
+// there when the tile before has been dealt with, and the accumulators. What
+// bounds the kernels then is the SFU, 512 cycles of ex2 an SM sub-partition
+// for a 128 x 64 tile (its products take 320 to 640).
 //
 // TMEM is only overwritten by a product after the barrier that says its last
 // reader is done: MMAs to different accumulators are not taken to be ordered.
@@ -43,19 +47,19 @@ namespace {
 
 constexpr int ROWS = 128;  // rows per item, one TMEM lane each
 constexpr int STEP = 64;   // rows of the other side per tile
-constexpr int MAX_STAGES = 3;
 constexpr int BIG = ROWS * 64 * 2;    // 16 KB
 constexpr int SMALL = STEP * 64 * 2;  // 8 KB
 
-// A CTA with G softmax groups, SUMS 64-wide accumulators in TMEM and EXTRA
-// floats in shared memory.
-template <int G_, int BIGS_, int STAGE_BYTES_, int COLS_, int EXTRA_>
+constexpr int STAGES = 3;
+constexpr int SOFTMAX = 256;  // threads of the two groups
+constexpr int LOADER = 8, MMA = 9, THREADS = SOFTMAX + 64;
+constexpr int CTAS = 2;  // on an SM
+constexpr uint32_t COLS = 256;
+
+// Of one kernel: 128-row tiles, staging bytes a softmax warp, floats besides.
+template <int BIGS_, int STAGE_BYTES_, int EXTRA_>
 struct Shape {
-    static constexpr int G = G_, BIGS = BIGS_, STAGE_BYTES = STAGE_BYTES_, COLS = COLS_, EXTRA = EXTRA_;
-    static constexpr int STAGES = G == 1 ? 2 : 3;
-    static constexpr int SOFTMAX = G * ROWS;  // threads of the groups
-    static constexpr int LOADER = 4 * G, MMA = 4 * G + 1, THREADS = SOFTMAX + 64;
-    static constexpr int CTAS = G == 1 ? 3 : 2;  // on an SM
+    static constexpr int BIGS = BIGS_, STAGE_BYTES = STAGE_BYTES_, EXTRA = EXTRA_;
 };
 
 // What the loading warp found; n < 0: there is no further item.
@@ -66,10 +70,10 @@ struct Item {
 };
 
 struct Bars {
-    uint64_t full[MAX_STAGES], empty[MAX_STAGES], landed[MAX_STAGES];
+    uint64_t full[STAGES], empty[STAGES], landed[STAGES];
     uint64_t item_full[2], item_empty[2];
     uint64_t big_full, big_empty;
-    // one of each for each group of softmax warps
+    // one of each for each score buffer
     uint64_t s_full[2], dp_full[2];  // products to read
     uint64_t s_read[2];              // S has been read: its columns may take dP
     uint64_t p_full[2];              // P (and dS) written: operands of the next products
@@ -82,7 +86,7 @@ struct Bars {
 };
 
 struct Slots {
-    uint32_t bits[MAX_STAGES][2];  // presence of a stage's rows (keys)
+    uint32_t bits[STAGES][2];  // presence of a stage's rows (keys)
     Item item[2];
 };
 
@@ -98,7 +102,7 @@ struct Frame {
 
 template <typename C>
 constexpr int smem_bytes() {
-    return C::BIGS * BIG + C::STAGES * 2 * SMALL + 4 * C::G * C::STAGE_BYTES + C::EXTRA * 4 + (int)sizeof(Bars) +
+    return C::BIGS * BIG + STAGES * 2 * SMALL + 8 * C::STAGE_BYTES + C::EXTRA * 4 + (int)sizeof(Bars) +
            (int)sizeof(Slots) + 1024;
 }
 
@@ -159,7 +163,6 @@ __device__ __forceinline__ void row_bits(uint32_t (&bits)[N], const AttnArgs& a,
 // them).
 template <typename C>
 struct Loader {
-    static constexpr int STAGES = C::STAGES;
     const Frame& f;
     const AttnArgs& a;
     int lane;
@@ -265,20 +268,16 @@ __device__ __forceinline__ bool next_item(const Frame& f, const AttnArgs& a, int
     return wait_one(&b->item_full[k & 1], (k >> 1) & 1, a.status, &b->abort) && f.slots->item[k & 1].n >= 0;
 }
 
-// A softmax group's place: the ring stage of its next tile with that stage's
-// parity, and the parity of the group's own barriers. With two groups its
-// tiles are every other one, whichever items they belong to.
-template <typename C>
+// The softmax warps' place in the ring and in the score buffers: both go on
+// from item to item.
 struct Turn {
-    static_assert(C::G <= C::STAGES, "next() wraps at most once");
-    int stage;
-    uint32_t full = 0, own = 0;
-    __device__ __forceinline__ explicit Turn(int group) : stage(group) {}
+    int stage = 0, buffer = 0;
+    uint32_t full = 0, own = 0;  // parities
     __device__ __forceinline__ void next() {
-        own ^= 1;
-        stage += C::G;
-        if (stage >= C::STAGES) {
-            stage -= C::STAGES;
+        own ^= buffer;
+        buffer ^= 1;
+        if (++stage == STAGES) {
+            stage = 0;
             full ^= 1;
         }
     }
@@ -326,18 +325,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// The two values of a 16-bit pair.
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t p);
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p) {
-    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t p) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&p));
-}
-
 // A warp's 32 rows of 32 accumulators, times f (a row's own; 0: zeros), to
 // global memory by way of 2 KB of shared memory: 64 bytes to a row and 8 rows
 // to an instruction instead of 16 bytes to each of 32. g is the first row's
@@ -367,17 +354,16 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, const float* v, float
     }
 }
 
-// v[i] = to where key col0 + i is not there or lies outside row's window.
-__device__ __forceinline__ void mask_row(float (&v)[64], const uint32_t (&bits)[2], int window, int row, int col0,
-                                         float to) {
-    if ((bits[0] & bits[1]) != ~0u) {
+// v[i] = -inf where column col0 + i is not there or lies outside row's window.
+__device__ __forceinline__ void mask_row(float (&v)[32], uint32_t bits, int window, int row, int col0) {
+    if (bits != ~0u) {
 #pragma unroll
-        for (int i = 0; i < 64; i++) v[i] = bits[i / 32] & 1u << (i & 31) ? v[i] : to;
+        for (int i = 0; i < 32; i++) v[i] = bits & 1u << i ? v[i] : -INFINITY;
     }
     if (window >= 0) {  // col0 + i - (row - window) in [0, 2 window], as one unsigned comparison
         const unsigned span = 2u * (unsigned)window, d = (unsigned)(col0 - row) + (unsigned)window;
 #pragma unroll
-        for (int i = 0; i < 64; i++) v[i] = d + i <= span ? v[i] : to;
+        for (int i = 0; i < 32; i++) v[i] = d + i <= span ? v[i] : -INFINITY;
     }
 }
 
@@ -408,12 +394,12 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b) {
         tc_mma_f16(d, sw128_desc(a) + 2 * ks, sw128_desc(b) + 2 * ks, IDESC<T>, ks != 0);
 }
 
-// D (128 x 64) += P . B, P (128 x 64, 16-bit pairs, 16 of them every `step`
-// columns) in TMEM, B's 64 rows summed over.
-template <typename T>
+// D (128 x 64) += P . B over N x 16 of B's rows; P: 16 rows' 16-bit pairs
+// every `step` columns of TMEM.
+template <typename T, int N>
 __device__ __forceinline__ void mma_sum(uint32_t d, uint32_t p, int step, uint32_t b, bool accumulate) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ks++)
+    for (int ks = 0; ks < N; ks++)
         tc_mma_f16_ts(d, p + step * ks, sw128_desc(b + ks * 2048), IDESC<T> | B_MN, accumulate || ks != 0);
 }
 
@@ -449,14 +435,14 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
     Frame f;
     f.big = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     f.ring = f.big + C::BIGS * BIG;
-    f.stage = f.ring + C::STAGES * 2 * SMALL;
-    f.extra = reinterpret_cast<float*>(f.stage + 4 * C::G * C::STAGE_BYTES);
+    f.stage = f.ring + STAGES * 2 * SMALL;
+    f.extra = reinterpret_cast<float*>(f.stage + 8 * C::STAGE_BYTES);
     f.bar = reinterpret_cast<Bars*>(f.extra + C::EXTRA);
     f.slots = reinterpret_cast<Slots*>(f.bar + 1);
-    f.stage += (warp & (4 * C::G - 1)) * C::STAGE_BYTES;
+    f.stage += (warp & 7) * C::STAGE_BYTES;
     if (threadIdx.x == 0) {
         Bars* b = f.bar;
-        for (int s = 0; s < MAX_STAGES; s++) {
+        for (int s = 0; s < STAGES; s++) {
             mbar_init(&b->full[s], 33);
             mbar_init(&b->empty[s], 1);
             mbar_init(&b->landed[s], 1);
@@ -465,23 +451,23 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
         mbar_init(&b->big_empty, 1);
         for (int s = 0; s < 2; s++) {
             mbar_init(&b->item_full[s], 1);
-            mbar_init(&b->item_empty[s], C::SOFTMAX + 1);
+            mbar_init(&b->item_empty[s], SOFTMAX + 1);
             mbar_init(&b->s_full[s], 1);
             mbar_init(&b->dp_full[s], 1);
-            mbar_init(&b->s_read[s], ROWS);
-            mbar_init(&b->p_full[s], ROWS);
+            mbar_init(&b->s_read[s], SOFTMAX);
+            mbar_init(&b->p_full[s], SOFTMAX);
             mbar_init(&b->done[s], 1);
             mbar_init(&b->acc_full[s], 1);
-            mbar_init(&b->acc_free[s], C::SOFTMAX);
-            mbar_init(&b->sync[s], C::SOFTMAX);
+            mbar_init(&b->acc_free[s], SOFTMAX);
+            mbar_init(&b->sync[s], SOFTMAX);
         }
         mbar_init(&b->drained, 1);
         b->abort = 0;
         fence_barrier_init();
         fence_proxy_async();
     }
-    if (warp == C::MMA) {
-        tmem_alloc(&f.bar->tmem, C::COLS);
+    if (warp == MMA) {
+        tmem_alloc(&f.bar->tmem, COLS);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -496,7 +482,7 @@ __device__ __forceinline__ void close_frame(const Frame& f, int warp) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == C::MMA) tmem_dealloc(f.tmem, C::COLS);
+    if (warp == MMA) tmem_dealloc(f.tmem, COLS);
 }
 
 // Warp-wide wait of the softmax warps.
@@ -504,14 +490,25 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, const A
     return __all_sync(0xffffffffu, wait_one(bar, parity, a.status, &b->abort));
 }
 
+// Presence bits of group g's 32 columns, col0 and on, of the present tile; the
+// ring is only asked about a tile that may lack some (its barrier is complete:
+// the tile's scores have been computed).
+__device__ __forceinline__ bool column_bits(const Frame& f, const AttnArgs& a, const Turn& turn, int g, int col0, int len,
+                                            uint32_t* bits) {
+    *bits = ~0u;
+    if (!a.mask && col0 + 32 <= len) return true;
+    if (!wait_all(&f.bar->full[turn.stage], turn.full, a, f.bar)) return false;
+    *bits = f.slots->bits[turn.stage][g];
+    return true;
+}
+
 // ------------------------------------------------------------------ forward
-// TMEM: S of group g at column 64 g (P over it); O of group g at 64 (G + g).
-// Two groups exchange halves of their rows of O at an item's end.
-template <int G>
-using Fwd = Shape<G, 1, G == 1 ? 2048 : 4096, 128 * G, G == 1 ? 0 : 4 * ROWS>;
+// TMEM: S at columns 0, 64 (P over it, a group's 16 columns at the start of its
+// 32); O of group 0, 1 at 128, 192. extra: either group's maximum and sum.
+using Fwd = Shape<1, 4096, 4 * ROWS>;
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(C::THREADS, C::CTAS)
+__global__ void __launch_bounds__(THREADS, CTAS)
     attention_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                             const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap,
                             const AttnArgs a, int heads, long long work) {
@@ -519,9 +516,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
-    constexpr int G = C::G, STAGES = C::STAGES;
 
-    if (warp == C::LOADER) {
+    if (warp == LOADER) {
         Loader<C> ld{f, a, lane};
         bool ok = true;
         for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
@@ -538,7 +534,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 if (j + 1 < kt1) row_bits(next, a, t, (j + 1) * STEP, lane);
                 ok = ld.room();
                 if (!ok) break;
-                if (lane < 2) f.slots->bits[ld.issued % C::STAGES][lane] = lane ? bits[1] : bits[0];
+                if (lane < 2) f.slots->bits[ld.issued % STAGES][lane] = lane ? bits[1] : bits[0];
                 ld.tile(&mk, &mv, h / a.group * 64, t.start + j * STEP, bits);
             }
             ld.fill();  // before the search for the next item
@@ -546,7 +542,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mq, nullptr);
         ld.finish(big);
-    } else if (warp == C::MMA) {
+    } else if (warp == MMA) {
         if (elect_one()) {
             const uint32_t q = smem_u32(f.big), kv = smem_u32(f.ring);
             Poll poll{bar, a.status};
@@ -559,21 +555,23 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 while (pv < end && poll.go_on(moved)) {
                     moved = false;
                     if (!big) big = moved = ready(&bar->big_full, k & 1);
-                    if (big && sc < end && sc < pv + G && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
-                        (sc < G || ready(&bar->done[sc % G], (sc / G - 1) & 1))) {
+                    if (big && sc < end && sc < pv + 2 && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
+                        (sc < 2 || ready(&bar->done[sc & 1], ((sc >> 1) - 1) & 1))) {
                         tc_fence_after();
-                        mma_rows<T>(f.tmem + sc % G * 64, q, kv + 2 * (sc % STAGES) * SMALL);
-                        tc_commit(&bar->s_full[sc % G]);
+                        mma_rows<T>(f.tmem + (sc & 1) * 64, q, kv + 2 * (sc % STAGES) * SMALL);
+                        tc_commit(&bar->s_full[sc & 1]);
                         if (++sc == end) tc_commit(&bar->big_empty);
                         moved = true;
                     }
-                    if (pv < sc && ready(&bar->p_full[pv % G], (pv / G) & 1) &&
+                    if (pv < sc && ready(&bar->p_full[pv & 1], (pv >> 1) & 1) &&
                         (k == 0 || pv > c || ready(&bar->acc_free[0], (k - 1) & 1))) {
-                        const int s = pv % STAGES, g = pv % G;
+                        const int s = pv % STAGES;
+                        const uint32_t p = f.tmem + (pv & 1) * 64, v = kv + (2 * s + 1) * SMALL;
                         tc_fence_after();
-                        mma_sum<T>(f.tmem + (G + g) * 64, f.tmem + g * 64, 8, kv + (2 * s + 1) * SMALL, pv >= c + G);
+                        mma_sum<T, 2>(f.tmem + 128, p, 8, v, pv > c);
+                        mma_sum<T, 2>(f.tmem + 192, p + 32, 8, v + 2 * 2048, pv > c);
                         tc_commit(&bar->empty[s]);
-                        tc_commit(&bar->done[g]);
+                        tc_commit(&bar->done[pv & 1]);
                         if (++pv == end) tc_commit(&bar->acc_full[0]);
                         moved = true;
                     }
@@ -587,54 +585,53 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
         __syncwarp();
     } else {
         const int g = warp >> 2, r = threadIdx.x & (ROWS - 1);
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = f.tmem + lanes + g * 64, t_o = t_s + G * 64;
+        const uint32_t lanes = f.tmem + ((uint32_t)((warp & 3) * 32) << 16), t_o = lanes + 128 + g * 64;
         const float sl2 = a.scale * LOG2E;
         constexpr float RESCALE = 8.0f;  // exponent growth that moves the reference point
         // halves of the rows of O that the groups exchange, 32 columns a warp's 32 rows
         float* give = reinterpret_cast<float*>(f.stage + (g ? -4 : 4) * C::STAGE_BYTES) + lane;
         const float* take = reinterpret_cast<const float*>(f.stage) + lane;
-        Turn<C> turn(g);
-        int ahead = g;  // the group's next tile, counted from the item's first
+        Turn turn;
         bool ok = true;
         for (int k = 0; ok; k++) {
             if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
             const Item& it = f.slots->item[k & 1];
-            if (G == 2) mbar_arrive(&bar->sync[0]);  // through with the last item's exchange
-            const int n = it.n, row0 = it.row0, t0 = it.t0;
-            const bool mine = ahead < n;  // the item has a tile for this group
+            mbar_arrive(&bar->sync[0]);  // through with the last item's exchange
+            const int n = it.n, row0 = it.row0, len = it.len;
+            int col0 = it.t0 * STEP + g * 32;
             float m = -INFINITY, l = 0.f;
-            bool first = true;
-            for (; ahead < n; ahead += C::G, turn.next(), first = false) {
-                const int col0 = (t0 + ahead) * STEP;
-                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) && wait_all(&bar->s_full[g], turn.own, a, bar);
+            for (int j = 0; j < n; j++, col0 += STEP, turn.next()) {
+                const uint32_t t_s = lanes + turn.buffer * 64 + g * 32;
+                uint32_t bits;
+                ok = wait_all(&bar->s_full[turn.buffer], turn.own, a, bar) &&
+                     column_bits(f, a, turn, g, col0, len, &bits);
                 if (!ok) break;
                 tc_fence_after();
-                float v[64];
-                load64(t_s, v);
-                const uint32_t bits[2] = {f.slots->bits[turn.stage][0], f.slots->bits[turn.stage][1]};
-                if ((bits[0] & bits[1]) != ~0u || edge(a.window, row0, ROWS, col0, STEP))
-                    mask_row(v, bits, a.window, row0 + r, col0, -INFINITY);
+                float v[32];
+                load32(t_s, v);
+                if (bits != ~0u || edge(a.window, row0, ROWS, col0, 32)) mask_row(v, bits, a.window, row0 + r, col0);
                 float mx[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) mx[e] = v[e];
 #pragma unroll
-                for (int e = 4; e < 60; e += 8)
+                for (int e = 4; e < 28; e += 8)
 #pragma unroll
                     for (int x = 0; x < 4; x++) mx[x] = max3(mx[x], v[e + x], v[e + 4 + x]);
-                const float top = fmaxf(max3(max3(mx[0], v[60], v[61]), mx[1], mx[2]), max3(mx[3], v[62], v[63]));
+                const float top = fmaxf(max3(max3(mx[0], v[28], v[29]), mx[1], mx[2]), max3(mx[3], v[30], v[31]));
                 // The reference point moves when the maximum has grown by more
                 // than 2^8 (p stays below 2^8 otherwise): then O and l shrink.
-                // S was asked for when P V of the group's tile before was
-                // complete, so O is at rest here.
                 float alpha = 1.f;
-                const bool move = first || (top - m) * sl2 > RESCALE;
+                const bool move = j == 0 || (top - m) * sl2 > RESCALE;
                 if (move) {
                     alpha = m == -INFINITY ? 0.f : ex2_approx((m - top) * sl2);
                     m = top;
                     l *= alpha;
                 }
-                if (!first && __any_sync(0xffffffffu, move)) {
+                if (j > 0 && __any_sync(0xffffffffu, move)) {
+                    // once P V of the tile before is complete, O is at rest
+                    ok = wait_all(&bar->done[turn.buffer ^ 1], turn.own ^ (turn.buffer ^ 1), a, bar);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll
                     for (int e = 0; e < 64; e += 16) {
                         uint32_t o[16];
@@ -647,73 +644,49 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 }
                 const float u = m == -INFINITY ? 0.f : m * sl2;
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                uint32_t p[16];
 #pragma unroll
-                for (int e = 0; e < 64; e += 16) {
-                    uint32_t p[8];
-#pragma unroll
-                    for (int x = 0; x < 8; x++) {
-                        const float2 y = fma2(make_float2(v[e + 2 * x], v[e + 2 * x + 1]), make_float2(sl2, sl2),
-                                              make_float2(-u, -u));
-                        const float2 q = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-                        sum[x & 1] = add2(sum[x & 1], q);
-                        p[x] = pack2<T>(q.x, q.y);
-                    }
-                    tmem_st8(t_s + e / 2, p);
+                for (int x = 0; x < 16; x++) {
+                    const float2 y = fma2(make_float2(v[2 * x], v[2 * x + 1]), make_float2(sl2, sl2), make_float2(-u, -u));
+                    const float2 q = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                    sum[x & 1] = add2(sum[x & 1], q);
+                    p[x] = pack2<T>(q.x, q.y);
                 }
+                tmem_st16(t_s, p);
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar->p_full[g]);
+                mbar_arrive(&bar->p_full[turn.buffer]);
             }
-            ahead -= n;
-            ok = ok && wait_all(&bar->acc_full[0], k & 1, a, bar);
+            // The groups' halves of the row are joined: each takes 32 columns of both.
+            ok = ok && wait_all(&bar->acc_full[0], k & 1, a, bar) && wait_all(&bar->sync[0], k & 1, a, bar);
             if (!ok) break;
             tc_fence_after();
+            float o[32];
+            load32(t_o + (1 - g) * 32, o);
+#pragma unroll
+            for (int e = 0; e < 32; e++) give[e * 32] = o[e];
+            load32(t_o + g * 32, o);
+            tc_fence_before();
+            mbar_arrive(&bar->acc_free[0]);
+            float2* ml = reinterpret_cast<float2*>(f.extra) + r;  // [group][row]
+            ml[g * ROWS] = make_float2(m, l);
+            mbar_arrive(&bar->sync[1]);
+            ok = wait_all(&bar->sync[1], k & 1, a, bar);
+            if (!ok) break;
+            const float2 other = ml[(1 - g) * ROWS];
+            const float top = fmaxf(m, other.x);
+            const float u = top == -INFINITY ? 0.f : top;
+            const float f0 = ex2_approx((m - u) * sl2), f1 = ex2_approx((other.x - u) * sl2);
+            const float sum = l * f0 + other.y * f1;
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = fmaf(o[e], f0, take[e * 32] * f1);
             const SeqTile t{it.start, it.len, row0};
             const bool there = present(a, t, row0 + r);
             const int row = row0 + (warp & 3) * 32;  // the warp's first
-            T* out = static_cast<T*>(a.io.out.p) + ((long long)t.start + row) * a.io.out.ld + it.head * 64;
-            float top = m, sum = l;
-            if constexpr (G == 1) {
-                float o[64];
-                load64(t_o, o);
-                tc_fence_before();
-                mbar_arrive(&bar->acc_free[0]);
-                const float by = there ? 1.f / l : 0.f;
-                store_rows<T>(f.stage, o, by, out, a.io.out.ld, t.len - row, lane);
-                store_rows<T>(f.stage, o + 32, by, out + 32, a.io.out.ld, t.len - row, lane);
-            } else {
-                // The groups' halves of the row are joined: each takes 32
-                // columns of both. A group without a tile (n is 1) takes the
-                // other's.
-                ok = wait_all(&bar->sync[0], k & 1, a, bar);
-                if (!ok) break;
-                const bool two = n > 1;
-                float o[32];
-                if (two) {
-                    load32(t_o + (1 - g) * 32, o);
-#pragma unroll
-                    for (int e = 0; e < 32; e++) give[e * 32] = o[e];
-                }
-                load32(f.tmem + lanes + 128 + (mine ? g : 1 - g) * 64 + g * 32, o);
-                tc_fence_before();
-                mbar_arrive(&bar->acc_free[0]);
-                float2* ml = reinterpret_cast<float2*>(f.extra) + r;  // [group][row]
-                ml[g * ROWS] = make_float2(m, l);
-                mbar_arrive(&bar->sync[1]);
-                ok = wait_all(&bar->sync[1], k & 1, a, bar);
-                if (!ok) break;
-                const float2 other = ml[(1 - g) * ROWS];
-                top = fmaxf(m, other.x);
-                const float u = top == -INFINITY ? 0.f : top;
-                const float f0 = ex2_approx((m - u) * sl2), f1 = ex2_approx((other.x - u) * sl2);
-                sum = l * f0 + other.y * f1;
-                if (two) {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = fmaf(o[e], f0, take[e * 32] * f1);
-                }
-                store_rows<T>(f.stage, o, there ? 1.f / sum : 0.f, out + g * 32, a.io.out.ld, t.len - row, lane);
-            }
+            store_rows<T>(f.stage, o, there ? 1.f / sum : 0.f,
+                          static_cast<T*>(a.io.out.p) + ((long long)t.start + row) * a.io.out.ld + it.head * 64 + g * 32,
+                          a.io.out.ld, t.len - row, lane);
             if (a.io.lse && g == 0 && row0 + r < t.len)
                 a.io.lse[(long long)it.head * a.n_tokens + t.start + row0 + r] =
                     there ? top * a.scale + logf(sum) : -INFINITY;
@@ -725,9 +698,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
 
 // The MMA lane of either backward kernel: S = A0 . R0^T, dP = A1 . R1^T (A:
 // 128-row tiles, R: the ring's), then the sums over the tile's rows.
-template <typename T, typename C, int ACCS, typename Sum>
+template <typename T, int ACCS, typename Sum>
 __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a, Sum sums) {
-    constexpr int G = C::G, STAGES = C::STAGES;
     Bars* bar = f.bar;
     const uint32_t big0 = smem_u32(f.big), big1 = big0 + BIG, ring = smem_u32(f.ring);
     Poll poll{bar, a.status};
@@ -740,28 +712,30 @@ __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a,
         while (sum < end && poll.go_on(moved)) {
             moved = false;
             if (!big) big = moved = ready(&bar->big_full, k & 1);
-            if (dp < sc && ready(&bar->s_read[dp % G], (dp / G) & 1)) {
+            if (dp < sc && ready(&bar->s_read[dp & 1], (dp >> 1) & 1)) {
                 tc_fence_after();
-                mma_rows<T>(f.tmem + dp % G * 64, big1, ring + (2 * (dp % STAGES) + 1) * SMALL);
-                tc_commit(&bar->dp_full[dp % G]);
+                mma_rows<T>(f.tmem + (dp & 1) * 64, big1, ring + (2 * (dp % STAGES) + 1) * SMALL);
+                tc_commit(&bar->dp_full[dp & 1]);
                 if (++dp == end) tc_commit(&bar->big_empty);
                 moved = true;
             }
-            if (sum < dp && ready(&bar->p_full[sum % G], (sum / G) & 1) &&
+            // The next tile's dP goes first: the softmax warps come to it right
+            // after this tile, and its sum can wait.
+            if ((sum + 1 < dp || (sum < dp && dp == end)) && ready(&bar->p_full[sum & 1], (sum >> 1) & 1) &&
                 (k < ACCS || sum > c || ready(&bar->acc_free[acc], (k / ACCS - 1) & 1))) {
-                const int s = sum % STAGES, g = sum % G;
+                const int s = sum % STAGES;
                 tc_fence_after();
-                sums(f.tmem + g * 64, ring + 2 * s * SMALL, acc, sum > c);
+                sums(f.tmem + (sum & 1) * 64, ring + 2 * s * SMALL, acc, sum > c);
                 tc_commit(&bar->empty[s]);
-                tc_commit(&bar->done[g]);
+                tc_commit(&bar->done[sum & 1]);
                 if (++sum == end) tc_commit(&bar->acc_full[acc]);
                 moved = true;
             }
-            if (big && sc < end && sc < sum + G && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
-                (sc < G || ready(&bar->done[sc % G], (sc / G - 1) & 1))) {
+            if (big && sc < end && sc < sum + 2 && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
+                (sc < 2 || ready(&bar->done[sc & 1], ((sc >> 1) - 1) & 1))) {
                 tc_fence_after();
-                mma_rows<T>(f.tmem + sc % G * 64, big0, ring + 2 * (sc % STAGES) * SMALL);
-                tc_commit(&bar->s_full[sc % G]);
+                mma_rows<T>(f.tmem + (sc & 1) * 64, big0, ring + 2 * (sc % STAGES) * SMALL);
+                tc_commit(&bar->s_full[sc & 1]);
                 sc++;
                 moved = true;
             }
@@ -802,13 +776,12 @@ __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const At
 }
 
 // ------------------------------------------------------------------ dQ
-// TMEM: S of group g at column 64 g (dP over it, dS over that); dQ at 64 G, with
-// two groups the next item's at 192
-template <int G>
-using Dq = Shape<G, 2, 2048, 128 * G, 0>;
+// TMEM: S at columns 0, 64 (dP over it, dS over that, 8 columns of every 16);
+// dQ at 128, the next item's at 192
+using Dq = Shape<2, 2048, 0>;
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(C::THREADS, C::CTAS)
+__global__ void __launch_bounds__(THREADS, CTAS)
     attention_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
                            const AttnArgs a, int heads, long long work) {
@@ -816,9 +789,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
-    constexpr int G = C::G, ACCS = G;  // accumulators in turn
 
-    if (warp == C::LOADER) {
+    if (warp == LOADER) {
         Loader<C> ld{f, a, lane};
         bool ok = true;
         for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
@@ -835,7 +807,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 if (j + 1 < kt1) row_bits(next, a, t, (j + 1) * STEP, lane);
                 ok = ld.room();
                 if (!ok) break;
-                if (lane < 2) f.slots->bits[ld.issued % C::STAGES][lane] = lane ? bits[1] : bits[0];
+                if (lane < 2) f.slots->bits[ld.issued % STAGES][lane] = lane ? bits[1] : bits[0];
                 ld.tile(&mk, &mv, h / a.group * 64, t.start + j * STEP, bits);
             }
             ld.fill();  // before the search for the next item
@@ -843,88 +815,78 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mq, &mdo);
         ld.finish(big);
-    } else if (warp == C::MMA) {
+    } else if (warp == MMA) {
         if (elect_one())
-            backward_mmas<T, C, ACCS>(f, a, [&](uint32_t p, uint32_t kv, int acc, bool more) {
-                mma_sum<T>(f.tmem + (G + acc) * 64, p, 8, kv, more);
+            backward_mmas<T, 2>(f, a, [&](uint32_t p, uint32_t kv, int acc, bool more) {
+                mma_sum<T, 4>(f.tmem + 128 + acc * 64, p, 16, kv, more);
             });
         __syncwarp();
     } else {
         const int g = warp >> 2, r = threadIdx.x & (ROWS - 1);
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = f.tmem + lanes + g * 64;
+        const uint32_t lanes = f.tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float sl2 = a.scale * LOG2E;
-        Turn<C> turn(g);
-        int ahead = g;  // the group's next tile, counted from the item's first
+        Turn turn;
         bool ok = true;
         for (int k = 0; ok; k++) {
             if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
             const Item& it = f.slots->item[k & 1];
-            const int n = it.n, t0 = it.t0, i = it.row0 + r;  // query
+            const int n = it.n, i = it.row0 + r;  // query
+            int col0 = it.t0 * STEP + g * 32;
             const SeqTile t{it.start, it.len, it.row0};
             const bool there = present(a, t, i);
             const long long at = (long long)it.head * a.n_tokens + t.start + i;
             // absent rows are not stored: any finite values will do
             const float e = there ? a.io.lse[at] * LOG2E : 0.f, delta = there ? a.io.delta[at] : 0.f;
-            for (; ahead < n; ahead += C::G, turn.next()) {
-                const int col0 = (t0 + ahead) * STEP;
-                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) && wait_all(&bar->s_full[g], turn.own, a, bar);
+            for (int j = 0; j < n; j++, col0 += STEP, turn.next()) {
+                const uint32_t t_s = lanes + turn.buffer * 64 + g * 32;
+                uint32_t bits;
+                ok = wait_all(&bar->s_full[turn.buffer], turn.own, a, bar) &&
+                     column_bits(f, a, turn, g, col0, t.len, &bits);
                 if (!ok) break;
                 tc_fence_after();
-                float v[64];
-                load64(t_s, v);
+                float v[32];
+                load32(t_s, v);
                 tc_fence_before();
-                mbar_arrive(&bar->s_read[g]);
-                const uint32_t bits[2] = {f.slots->bits[turn.stage][0], f.slots->bits[turn.stage][1]};
-                if ((bits[0] & bits[1]) != ~0u || edge(a.window, i - r, ROWS, col0, STEP))
-                    mask_row(v, bits, a.window, i, col0, -INFINITY);
-                // P as 16-bit pairs, which is how it waits for dP: in 32 bits
-                // the row would not fit the thread's 96 registers
-                uint32_t p[32];
+                mbar_arrive(&bar->s_read[turn.buffer]);
+                if (bits != ~0u || edge(a.window, i - r, ROWS, col0, 32)) mask_row(v, bits, a.window, i, col0);
 #pragma unroll
-                for (int x = 0; x < 32; x++) {
-                    const float2 y = fma2(make_float2(v[2 * x], v[2 * x + 1]), make_float2(sl2, sl2), make_float2(-e, -e));
-                    p[x] = pack2<T>(ex2_approx(y.x), ex2_approx(y.y));
+                for (int x = 0; x < 32; x += 2) {
+                    const float2 y = fma2(make_float2(v[x], v[x + 1]), make_float2(sl2, sl2), make_float2(-e, -e));
+                    v[x] = ex2_approx(y.x);
+                    v[x + 1] = ex2_approx(y.y);
                 }
-                ok = wait_all(&bar->dp_full[g], turn.own, a, bar);
+                ok = wait_all(&bar->dp_full[turn.buffer], turn.own, a, bar);
                 if (!ok) break;
                 tc_fence_after();
+                float d[32];
+                load32(t_s, d);
 #pragma unroll
-                for (int x = 0; x < 64; x += 16) {
-                    uint32_t d[16], ds[8];
-                    tmem_ld16(t_s + x, d);
-                    tc_wait_ld();
+                for (int x = 0; x < 32; x += 16) {
+                    uint32_t ds[8];
 #pragma unroll
                     for (int z = 0; z < 8; z++) {
-                        const float2 y = mul2(unpack2<T>(p[x / 2 + z]),
-                                              add2(make_float2(__uint_as_float(d[2 * z]), __uint_as_float(d[2 * z + 1])),
-                                                   make_float2(-delta, -delta)));
+                        const int c = x + 2 * z;
+                        const float2 y = mul2(make_float2(v[c], v[c + 1]),
+                                              add2(make_float2(d[c], d[c + 1]), make_float2(-delta, -delta)));
                         ds[z] = pack2<T>(y.x, y.y);
                     }
-                    tmem_st8(t_s + x / 2, ds);
+                    tmem_st8(t_s + x, ds);
                 }
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar->p_full[g]);
+                mbar_arrive(&bar->p_full[turn.buffer]);
             }
-            ahead -= n;
-            if (ok) ok = wait_all(&bar->acc_full[k % ACCS], (k / ACCS) & 1, a, bar);
+            if (ok) ok = wait_all(&bar->acc_full[k & 1], (k >> 1) & 1, a, bar);
             if (!ok) break;
             tc_fence_after();
-            // each group stores 64 / G columns
-            float d[64 / G];
-            const uint32_t t_acc = f.tmem + lanes + (G + k % ACCS) * 64 + g * 32;
-            if constexpr (G == 1)
-                load64(t_acc, d);
-            else
-                load32(t_acc, d);
+            float d[32];
+            load32(lanes + 128 + (k & 1) * 64 + g * 32, d);
             tc_fence_before();
-            mbar_arrive(&bar->acc_free[k % ACCS]);
+            mbar_arrive(&bar->acc_free[k & 1]);
             const int row = it.row0 + (warp & 3) * 32;  // the warp's first
-            const float by = there ? a.scale : 0.f;
-            T* dq = static_cast<T*>(a.io.dq.p) + ((long long)it.start + row) * a.io.dq.ld + it.head * 64 + g * 32;
-            store_rows<T>(f.stage, d, by, dq, a.io.dq.ld, it.len - row, lane);
-            if constexpr (G == 1) store_rows<T>(f.stage, d + 32, by, dq + 32, a.io.dq.ld, it.len - row, lane);
+            store_rows<T>(f.stage, d, there ? a.scale : 0.f,
+                          static_cast<T*>(a.io.dq.p) + ((long long)it.start + row) * a.io.dq.ld + it.head * 64 + g * 32,
+                          a.io.dq.ld, it.len - row, lane);
             mbar_arrive(&bar->item_empty[k & 1]);
         }
     }
@@ -932,13 +894,13 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
 }
 
 // ------------------------------------------------------------------ dK, dV
-// TMEM: S^T of group 0, 1 at columns 0, 64 (dP^T over it, P^T and dS^T over
+// TMEM: S^T at columns 0, 64 (dP^T over it, P^T and dS^T over
 // that, 8 columns of each in turn); dV at 128; dK at 192. extra: -lse * log2 e
 // and -delta of each stage's queries.
-using Dkv = Shape<2, 2, 2048, 256, 2 * MAX_STAGES * STEP>;
+using Dkv = Shape<2, 2048, 2 * STAGES * STEP>;
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(C::THREADS, C::CTAS)
+__global__ void __launch_bounds__(THREADS, CTAS)
     attention_dkv_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                             const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
                             const AttnArgs a, int heads, long long work) {
@@ -947,7 +909,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
 
-    if (warp == C::LOADER) {
+    if (warp == LOADER) {
         Loader<C> ld{f, a, lane};
         bool ok = true;
         for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
@@ -978,7 +940,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 if (j + 1 < n) row_bits(next, a, t, q * STEP, lane);
                 ok = ld.room();
                 if (!ok) break;
-                const int s = ld.issued % C::STAGES;
+                const int s = ld.issued % STAGES;
                 float* stat = f.extra + s * 2 * STEP + lane;
                 stat[0] = -LOG2E * l0;
                 stat[32] = -LOG2E * l1;
@@ -991,70 +953,70 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mk, &mv);
         ld.finish(big);
-    } else if (warp == C::MMA) {
+    } else if (warp == MMA) {
         if (elect_one())
-            backward_mmas<T, C, 1>(f, a, [&](uint32_t p, uint32_t qd, int, bool more) {
-                mma_sum<T>(f.tmem + 128, p, 16, qd + SMALL, more);
-                mma_sum<T>(f.tmem + 192, p + 8, 16, qd, more);
+            backward_mmas<T, 1>(f, a, [&](uint32_t p, uint32_t qd, int, bool more) {
+                mma_sum<T, 4>(f.tmem + 128, p, 16, qd + SMALL, more);
+                mma_sum<T, 4>(f.tmem + 192, p + 8, 16, qd, more);
             });
         __syncwarp();
     } else {
         const int g = warp >> 2, r = threadIdx.x & (ROWS - 1);
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = f.tmem + lanes + g * 64;
+        const uint32_t lanes = f.tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float sl2 = a.scale * LOG2E;
-        Turn<C> turn(g);
-        int ahead = g;  // the group's next tile, counted from the item's first
+        Turn turn;
         bool ok = true;
         for (int k = 0; ok; k++) {
             if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
             const Item& it = f.slots->item[k & 1];
             const int n = it.n, i = it.row0 + r;  // key
-            for (; ahead < n; ahead += C::G, turn.next()) {
-                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) && wait_all(&bar->s_full[g], turn.own, a, bar);
+            for (int j = 0; j < n; j++, turn.next()) {
+                const uint32_t t_s = lanes + turn.buffer * 64 + g * 32;
+                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) &&
+                     wait_all(&bar->s_full[turn.buffer], turn.own, a, bar);
                 if (!ok) break;
                 tc_fence_after();
-                float v[64];
-                load64(t_s, v);
+                float v[32];
+                load32(t_s, v);
                 tc_fence_before();
-                mbar_arrive(&bar->s_read[g]);
+                mbar_arrive(&bar->s_read[turn.buffer]);
                 if (a.window >= 0) {
-                    const int row0 = (it.t0 + ahead % (n / a.group)) * STEP;
-                    if (edge(a.window, row0, STEP, i - r, ROWS)) {
-                        const uint32_t all[2] = {~0u, ~0u};
-                        mask_row(v, all, a.window, i, row0, -INFINITY);
-                    }
+                    const int col0 = (it.t0 + j % (n / a.group)) * STEP + g * 32;
+                    if (edge(a.window, col0, 32, i - r, ROWS)) mask_row(v, ~0u, a.window, i, col0);
                 }
-                const float4* lse = reinterpret_cast<const float4*>(f.extra + turn.stage * 2 * STEP);
-                uint32_t p[32];  // P in 16-bit pairs, as dV's product takes it; dS uses the same values
+                const float4* lse = reinterpret_cast<const float4*>(f.extra + turn.stage * 2 * STEP + g * 32);
+                const float4* delta = lse + STEP / 4;
 #pragma unroll
-                for (int x = 0; x < 16; x++) {
+                for (int x = 0; x < 8; x++) {
                     const float4 e = lse[x];
                     const float2 y = fma2(make_float2(v[4 * x], v[4 * x + 1]), make_float2(sl2, sl2), make_float2(e.x, e.y));
                     const float2 z =
                         fma2(make_float2(v[4 * x + 2], v[4 * x + 3]), make_float2(sl2, sl2), make_float2(e.z, e.w));
-                    p[2 * x] = pack2<T>(ex2_approx(y.x), ex2_approx(y.y));
-                    p[2 * x + 1] = pack2<T>(ex2_approx(z.x), ex2_approx(z.y));
+                    v[4 * x] = ex2_approx(y.x);
+                    v[4 * x + 1] = ex2_approx(y.y);
+                    v[4 * x + 2] = ex2_approx(z.x);
+                    v[4 * x + 3] = ex2_approx(z.y);
                 }
-                ok = wait_all(&bar->dp_full[g], turn.own, a, bar);
+                ok = wait_all(&bar->dp_full[turn.buffer], turn.own, a, bar);
                 if (!ok) break;
                 tc_fence_after();
-                const float4* delta = lse + STEP / 4;
 #pragma unroll
-                for (int x = 0; x < 64; x += 16) {
+                for (int x = 0; x < 32; x += 16) {
                     uint32_t d[16], w[16];  // 16 of dP, then 16 of P and 16 of dS in pairs
                     tmem_ld16(t_s + x, d);
                     tc_wait_ld();
 #pragma unroll
                     for (int z = 0; z < 4; z++) {
                         const float4 e = delta[x / 4 + z];
-                        const float2 y0 = add2(make_float2(__uint_as_float(d[4 * z]), __uint_as_float(d[4 * z + 1])),
-                                               make_float2(e.x, e.y));
-                        const float2 y1 = add2(make_float2(__uint_as_float(d[4 * z + 2]), __uint_as_float(d[4 * z + 3])),
-                                               make_float2(e.z, e.w));
-                        w[2 * z] = p[x / 2 + 2 * z];
-                        w[2 * z + 1] = p[x / 2 + 2 * z + 1];
-                        const float2 s0 = mul2(unpack2<T>(w[2 * z]), y0), s1 = mul2(unpack2<T>(w[2 * z + 1]), y1);
+                        const float2 p0 = make_float2(v[x + 4 * z], v[x + 4 * z + 1]);
+                        const float2 p1 = make_float2(v[x + 4 * z + 2], v[x + 4 * z + 3]);
+                        const float2 s0 = mul2(p0, add2(make_float2(__uint_as_float(d[4 * z]), __uint_as_float(d[4 * z + 1])),
+                                                        make_float2(e.x, e.y)));
+                        const float2 s1 =
+                            mul2(p1, add2(make_float2(__uint_as_float(d[4 * z + 2]), __uint_as_float(d[4 * z + 3])),
+                                          make_float2(e.z, e.w)));
+                        w[2 * z] = pack2<T>(p0.x, p0.y);
+                        w[2 * z + 1] = pack2<T>(p1.x, p1.y);
                         w[8 + 2 * z] = pack2<T>(s0.x, s0.y);
                         w[9 + 2 * z] = pack2<T>(s1.x, s1.y);
                     }
@@ -1062,15 +1024,14 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS)
                 }
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar->p_full[g]);
+                mbar_arrive(&bar->p_full[turn.buffer]);
             }
-            ahead -= n;
             if (ok) ok = wait_all(&bar->acc_full[0], k & 1, a, bar);
             if (!ok) break;
             tc_fence_after();
             // group 0 stores dV, group 1 dK
             float d[64];
-            load64(f.tmem + lanes + 128 + g * 64, d);
+            load64(lanes + 128 + g * 64, d);
             tc_fence_before();
             mbar_arrive(&bar->acc_free[0]);
             const SeqTile t{it.start, it.len, it.row0};
@@ -1108,17 +1069,10 @@ template <typename C>
 cudaError_t launch(Kernel kernel, int heads, const Maps& m, const AttnArgs& a, int sms, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<C>());
     if (e != cudaSuccess) return e;
-    const long long work = seq_tiles(a.n_tokens, a.n_seqs, ROWS) * heads, most = (long long)C::CTAS * sms;
-    kernel<<<(unsigned)(work < most ? work : most), C::THREADS, smem_bytes<C>(), stream>>>(m.q, m.k, m.v, m.dout, a,
+    const long long work = seq_tiles(a.n_tokens, a.n_seqs, ROWS) * heads, most = (long long)CTAS * sms;
+    kernel<<<(unsigned)(work < most ? work : most), THREADS, smem_bytes<C>(), stream>>>(m.q, m.k, m.v, m.dout, a,
                                                                                           heads, work);
     return cudaGetLastError();
-}
-
-// One group a CTA or two?
-bool solo(int heads, const AttnArgs& a, int sms) {
-    const char* e = getenv("SOLO");
-    if (e) return e[0] == '1';
-    return a.max_len <= 1024;
 }
 
 }  // namespace
@@ -1130,12 +1084,8 @@ cudaError_t launch_attention_fwd_tc(bool bf16, int n_heads, const AttnArgs& a, c
         !map_rows(&m.v, a.io.v, kv, a, bf16))
         return cudaErrorInvalidValue;
     m.dout = m.q;  // not used
-    const int sms = sm_count();
-    if (solo(n_heads, a, sms))
-        return launch<Fwd<1>>(bf16 ? attention_fwd_tc_kernel<__nv_bfloat16, Fwd<1>> : attention_fwd_tc_kernel<__half, Fwd<1>>,
-                              n_heads, m, a, sms, stream);
-    return launch<Fwd<2>>(bf16 ? attention_fwd_tc_kernel<__nv_bfloat16, Fwd<2>> : attention_fwd_tc_kernel<__half, Fwd<2>>,
-                          n_heads, m, a, sms, stream);
+    return launch<Fwd>(bf16 ? attention_fwd_tc_kernel<__nv_bfloat16, Fwd> : attention_fwd_tc_kernel<__half, Fwd>, n_heads, m,
+                       a, sm_count(), stream);
 }
 
 cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, const AttnArgs& a, cudaStream_t stream) {
@@ -1152,11 +1102,8 @@ cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, cons
         attention_delta_kernel<__half><<<blocks, DELTA_THREADS, 0, stream>>>(a, n_heads);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    e = solo(n_heads, a, sms)
-            ? launch<Dq<1>>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq<1>> : attention_dq_tc_kernel<__half, Dq<1>>,
-                            n_heads, m, a, sms, stream)
-            : launch<Dq<2>>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq<2>> : attention_dq_tc_kernel<__half, Dq<2>>,
-                            n_heads, m, a, sms, stream);
+    e = launch<Dq>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq> : attention_dq_tc_kernel<__half, Dq>, n_heads, m, a, sms,
+                   stream);
     if (e == cudaSuccess)
         e = launch<Dkv>(bf16 ? attention_dkv_tc_kernel<__nv_bfloat16, Dkv> : attention_dkv_tc_kernel<__half, Dkv>,
                         n_kv_heads, m, a, sms, stream);
