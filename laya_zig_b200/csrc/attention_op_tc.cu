@@ -56,10 +56,12 @@ constexpr int LOADER = 8, MMA = 9, THREADS = SOFTMAX + 64;
 constexpr int CTAS = 2;  // on an SM
 constexpr uint32_t COLS = 256;
 
-// Of one kernel: 128-row tiles, staging bytes a softmax warp, floats besides.
-template <int BIGS_, int STAGE_BYTES_, int EXTRA_>
+constexpr int STAGE_BYTES = 2048;  // staging for a softmax warp's stores
+
+// Of one kernel: 128-row tiles, floats besides.
+template <int BIGS_, int EXTRA_>
 struct Shape {
-    static constexpr int BIGS = BIGS_, STAGE_BYTES = STAGE_BYTES_, EXTRA = EXTRA_;
+    static constexpr int BIGS = BIGS_, EXTRA = EXTRA_;
 };
 
 // What the loading warp found; n < 0: there is no further item.
@@ -79,7 +81,7 @@ struct Bars {
     uint64_t p_full[2];              // P (and dS) written: operands of the next products
     uint64_t done[2];                // which are complete: the columns may take S again
     uint64_t acc_full[2], acc_free[2];  // an item's accumulators
-    uint64_t sync[2];                // among the softmax threads
+    uint64_t sync;                   // among the softmax threads
     uint64_t drained;
     uint32_t tmem;
     int abort;
@@ -93,7 +95,7 @@ struct Slots {
 struct Frame {
     uint8_t* big;    // the 128-row tiles
     uint8_t* ring;   // STAGES pairs of 64-row tiles
-    uint8_t* stage;  // 2 KB (forward: 4 KB) a softmax warp
+    uint8_t* stage;  // the warp's STAGE_BYTES
     Bars* bar;
     Slots* slots;
     float* extra;  // 16-byte aligned
@@ -102,7 +104,7 @@ struct Frame {
 
 template <typename C>
 constexpr int smem_bytes() {
-    return C::BIGS * BIG + STAGES * 2 * SMALL + 8 * C::STAGE_BYTES + C::EXTRA * 4 + (int)sizeof(Bars) +
+    return C::BIGS * BIG + STAGES * 2 * SMALL + 8 * STAGE_BYTES + C::EXTRA * 4 + (int)sizeof(Bars) +
            (int)sizeof(Slots) + 1024;
 }
 
@@ -197,16 +199,16 @@ struct Loader {
         mbar_arrive(&bar->full[patch]);
         patch = -1;
     }
+    // Room for the next item (and what a kernel keeps beside it).
+    __device__ __forceinline__ bool slot() { return wait(&f.bar->item_empty[items & 1], ((items >> 1) & 1) ^ 1); }
     // The next item for everyone, and its 128-row tiles (columns `col`) once
     // the one before has no use for the old ones.
     __device__ __forceinline__ bool item(const Item& it, const CUtensorMap* b0, const CUtensorMap* b1) {
         Bars* bar = f.bar;
         const int s = items & 1;
-        if (!wait(&bar->item_empty[s], ((items >> 1) & 1) ^ 1)) return false;
-        if (lane == 0) {
-            f.slots->item[s] = it;
-            mbar_arrive(&bar->item_full[s]);
-        }
+        if (!slot()) return false;
+        if (lane == 0) f.slots->item[s] = it;
+        mbar_arrive(&bar->item_full[s]);
         if (it.n >= 0) {
             if (!wait(&bar->big_empty, (items & 1) ^ 1)) return false;
             if (lane == 0) {
@@ -254,13 +256,67 @@ struct Loader {
     }
 };
 
-// Item w of the call (heads first, then tiles of 128 rows): false if it names no rows.
-__device__ __forceinline__ bool find_item(const AttnArgs& a, long long w, int heads, int lane, SeqTile* t, int* head) {
-    const long long x = w / heads;
-    *head = (int)(w - x * heads);
-    if (lane == 0 && *head == 0) check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, x, a.status);
-    return find_tile(a.cu, a.n_seqs, a.n_tokens, a.max_len, ROWS, x, lane, t);
-}
+// The loading warp's walk over the call's items: tile slot x of the call (see
+// seq_tiles) for one head after the other, every gridDim.x-th to a CTA.
+struct Walk {
+    const AttnArgs& a;
+    int heads, lane;
+    long long x, slots;
+    int head, dx, dh;  // the next candidate, and the way to the one after
+    long long pivot;   // key of entry lane * step: the search's first round
+    int step;
+    SeqTile t;         // the item found
+    int found_head;
+    bool found;
+
+    // The first item is found here, before the frame is open: its look at the
+    // offsets passes while the other warps set the CTA up.
+    __device__ __forceinline__ Walk(const AttnArgs& a_, int heads_, int lane_, bool mine) : a(a_), heads(heads_), lane(lane_) {
+        found = false;
+        if (!mine) return;
+        slots = (long long)(a.n_tokens / ROWS) + a.n_seqs;
+        x = blockIdx.x / heads;
+        head = blockIdx.x % heads;
+        dx = gridDim.x / heads;
+        dh = gridDim.x % heads;
+        step = (a.n_seqs + 31) / 32;
+        pivot = lane * step < a.n_seqs ? key(a.cu[lane * step], lane * step) : 0;
+        next();
+    }
+    __device__ __forceinline__ static long long key(int start, int s) { return (long long)(max(start, 0) / ROWS) + s; }
+    __device__ __forceinline__ void next() {
+        for (found = false; x < slots && !found;) {
+            if (lane == 0 && head == 0) check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, x, a.status);
+            found = find();
+            found_head = head;
+            x += dx;
+            head += dh;
+            if (head >= heads) {
+                head -= heads;
+                x++;
+            }
+        }
+    }
+    // find_tile for slot x, with one look at the table for up to 1,024 sequences.
+    __device__ __forceinline__ bool find() {
+        const int n = a.n_seqs;
+        if (n > 1024) return find_tile(a.cu, n, a.n_tokens, a.max_len, ROWS, x, lane, &t);
+        const int c = __popc(__ballot_sync(0xffffffffu, lane * step < n && pivot <= x));
+        if (c == 0) return false;
+        const int lo = (c - 1) * step, m = min(step, n - lo);
+        const int at = a.cu[min(lo + lane, n)];
+        const int c1 = __popc(__ballot_sync(0xffffffffu, lane < m && key(at, lo + lane) <= x));
+        if (c1 == 0) return false;
+        const int s = lo + c1 - 1, start = __shfl_sync(0xffffffffu, at, c1 - 1);
+        const int end = c1 < 32 ? __shfl_sync(0xffffffffu, at, c1 & 31) : a.cu[s + 1];
+        if (!run_ok(start, end, a.n_tokens, a.max_len)) return false;
+        const long long tile = x - key(start, s);
+        t = SeqTile{start, end - start, 0};
+        if (tile < 0 || tile * ROWS >= t.len) return false;
+        t.row0 = (int)tile * ROWS;
+        return true;
+    }
+};
 
 // The k-th item, for every other warp: its slot, until it arrives on item_empty.
 __device__ __forceinline__ bool next_item(const Frame& f, const AttnArgs& a, int k) {
@@ -345,12 +401,13 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, const float* v, float
             make_uint4(u[0], u[1], u[2], u[3]);
     }
     __syncwarp();
-    const int c = lane & 3;
+    const int c = lane & 3, r0 = lane >> 2;  // r0 >> 1 & 3 is the same for r0 + 8 i
+    const uint8_t* from = stage + r0 * 64 + ((c ^ (r0 >> 1 & 3)) << 4);
+    T* to = g + r0 * ld + c * 8;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = i * 8 + (lane >> 2);
-        const uint4 u = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
-        if (r < rows) *reinterpret_cast<uint4*>(g + r * ld + c * 8) = u;
+    for (int i = 0; i < 4; i++, to += 8 * ld) {
+        const uint4 u = *reinterpret_cast<const uint4*>(from + i * 512);
+        if (r0 + i * 8 < rows) *reinterpret_cast<uint4*>(to) = u;
     }
 }
 
@@ -436,10 +493,10 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
     f.big = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     f.ring = f.big + C::BIGS * BIG;
     f.stage = f.ring + STAGES * 2 * SMALL;
-    f.extra = reinterpret_cast<float*>(f.stage + 8 * C::STAGE_BYTES);
+    f.extra = reinterpret_cast<float*>(f.stage + 8 * STAGE_BYTES);
     f.bar = reinterpret_cast<Bars*>(f.extra + C::EXTRA);
     f.slots = reinterpret_cast<Slots*>(f.bar + 1);
-    f.stage += (warp & 7) * C::STAGE_BYTES;
+    f.stage += (warp & 7) * STAGE_BYTES;
     if (threadIdx.x == 0) {
         Bars* b = f.bar;
         for (int s = 0; s < STAGES; s++) {
@@ -450,7 +507,7 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
         mbar_init(&b->big_full, 1);
         mbar_init(&b->big_empty, 1);
         for (int s = 0; s < 2; s++) {
-            mbar_init(&b->item_full[s], 1);
+            mbar_init(&b->item_full[s], 32);
             mbar_init(&b->item_empty[s], SOFTMAX + 1);
             mbar_init(&b->s_full[s], 1);
             mbar_init(&b->dp_full[s], 1);
@@ -459,8 +516,8 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
             mbar_init(&b->done[s], 1);
             mbar_init(&b->acc_full[s], 1);
             mbar_init(&b->acc_free[s], SOFTMAX);
-            mbar_init(&b->sync[s], SOFTMAX);
         }
+        mbar_init(&b->sync, SOFTMAX);
         mbar_init(&b->drained, 1);
         b->abort = 0;
         fence_barrier_init();
@@ -504,26 +561,32 @@ __device__ __forceinline__ bool column_bits(const Frame& f, const AttnArgs& a, c
 
 // ------------------------------------------------------------------ forward
 // TMEM: S at columns 0, 64 (P over it, a group's 16 columns at the start of its
-// 32); O of group 0, 1 at 128, 192. extra: either group's maximum and sum.
-using Fwd = Shape<1, 4096, 4 * ROWS>;
+// 32); O of group 0, 1 at 128, 192. extra: maximum and sum of the rows of either
+// group, of two items in turn.
+using Fwd = Shape<1, 8 * ROWS>;
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS, CTAS)
     attention_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                             const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap,
-                            const AttnArgs a, int heads, long long work) {
+                            const AttnArgs a, int heads) {
     extern __shared__ uint8_t raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == LOADER * 32) {
+        prefetch_tmap(&mq);
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+    }
+    Walk walk(a, heads, lane, warp == LOADER);
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
 
     if (warp == LOADER) {
         Loader<C> ld{f, a, lane};
         bool ok = true;
-        for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
-            SeqTile t;
-            int h;
-            if (!find_item(a, w, heads, lane, &t, &h)) continue;
+        while (walk.found && ok) {
+            const SeqTile t = walk.t;
+            const int h = walk.found_head;
             int kt0, kt1;
             visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
             uint32_t next[2];
@@ -537,7 +600,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 if (lane < 2) f.slots->bits[ld.issued % STAGES][lane] = lane ? bits[1] : bits[0];
                 ld.tile(&mk, &mv, h / a.group * 64, t.start + j * STEP, bits);
             }
-            ld.fill();  // before the search for the next item
+            walk.next();  // while the last boxes are on their way
+            ld.fill();
         }
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mq, nullptr);
@@ -588,15 +652,11 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         const uint32_t lanes = f.tmem + ((uint32_t)((warp & 3) * 32) << 16), t_o = lanes + 128 + g * 64;
         const float sl2 = a.scale * LOG2E;
         constexpr float RESCALE = 8.0f;  // exponent growth that moves the reference point
-        // halves of the rows of O that the groups exchange, 32 columns a warp's 32 rows
-        float* give = reinterpret_cast<float*>(f.stage + (g ? -4 : 4) * C::STAGE_BYTES) + lane;
-        const float* take = reinterpret_cast<const float*>(f.stage) + lane;
         Turn turn;
         bool ok = true;
         for (int k = 0; ok; k++) {
             if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
             const Item& it = f.slots->item[k & 1];
-            mbar_arrive(&bar->sync[0]);  // through with the last item's exchange
             const int n = it.n, row0 = it.row0, len = it.len;
             int col0 = it.t0 * STEP + g * 32;
             float m = -INFINITY, l = 0.f;
@@ -658,33 +718,38 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 tc_fence_before();
                 mbar_arrive(&bar->p_full[turn.buffer]);
             }
-            // The groups' halves of the row are joined: each takes 32 columns of both.
-            ok = ok && wait_all(&bar->acc_full[0], k & 1, a, bar) && wait_all(&bar->sync[0], k & 1, a, bar);
+            // The groups' halves of the row are joined: each takes 32 columns
+            // of both (the two threads of a row share its TMEM lane).
+            float2* ml = reinterpret_cast<float2*>(f.extra) + (k & 1) * 2 * ROWS + r;
+            if (ok) {
+                ml[g * ROWS] = make_float2(m, l);
+                mbar_arrive(&bar->sync);
+            }
+            ok = ok && wait_all(&bar->sync, k & 1, a, bar) && wait_all(&bar->acc_full[0], k & 1, a, bar);
             if (!ok) break;
             tc_fence_after();
-            float o[32];
-            load32(t_o + (1 - g) * 32, o);
-#pragma unroll
-            for (int e = 0; e < 32; e++) give[e * 32] = o[e];
-            load32(t_o + g * 32, o);
+            float o[32], o1[32];
+            tmem_ld32(lanes + 128 + g * 64 + g * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+            tmem_ld32(lanes + 128 + (1 - g) * 64 + g * 32, *reinterpret_cast<uint32_t(*)[32]>(&o1[0]));
+            tc_wait_ld();
             tc_fence_before();
             mbar_arrive(&bar->acc_free[0]);
-            float2* ml = reinterpret_cast<float2*>(f.extra) + r;  // [group][row]
-            ml[g * ROWS] = make_float2(m, l);
-            mbar_arrive(&bar->sync[1]);
-            ok = wait_all(&bar->sync[1], k & 1, a, bar);
-            if (!ok) break;
             const float2 other = ml[(1 - g) * ROWS];
             const float top = fmaxf(m, other.x);
             const float u = top == -INFINITY ? 0.f : top;
             const float f0 = ex2_approx((m - u) * sl2), f1 = ex2_approx((other.x - u) * sl2);
             const float sum = l * f0 + other.y * f1;
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = fmaf(o[e], f0, take[e * 32] * f1);
+            for (int e = 0; e < 32; e += 2) {
+                const float2 x = fma2(make_float2(o[e], o[e + 1]), make_float2(f0, f0),
+                                      mul2(make_float2(o1[e], o1[e + 1]), make_float2(f1, f1)));
+                o[e] = x.x;
+                o[e + 1] = x.y;
+            }
             const SeqTile t{it.start, it.len, row0};
             const bool there = present(a, t, row0 + r);
             const int row = row0 + (warp & 3) * 32;  // the warp's first
-            store_rows<T>(f.stage, o, there ? 1.f / sum : 0.f,
+            store_rows<T>(f.stage, o, there ? rcp_approx(sum) : 0.f,
                           static_cast<T*>(a.io.out.p) + ((long long)t.start + row) * a.io.out.ld + it.head * 64 + g * 32,
                           a.io.out.ld, t.len - row, lane);
             if (a.io.lse && g == 0 && row0 + r < t.len)
@@ -777,30 +842,55 @@ __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const At
 
 // ------------------------------------------------------------------ dQ
 // TMEM: S at columns 0, 64 (dP over it, dS over that, 8 columns of every 16);
-// dQ at 128, the next item's at 192
-using Dq = Shape<2, 2048, 0>;
+// dQ at 128, the next item's at 192. extra: -lse * log2 e and -delta of the rows
+// of two items in turn.
+using Dq = Shape<2, 4 * ROWS>;
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS, CTAS)
     attention_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
-                           const AttnArgs a, int heads, long long work) {
+                           const AttnArgs a, int heads) {
     extern __shared__ uint8_t raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == LOADER * 32) {
+        prefetch_tmap(&mq);
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+        prefetch_tmap(&mdo);
+    }
+    Walk walk(a, heads, lane, warp == LOADER);
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
 
     if (warp == LOADER) {
         Loader<C> ld{f, a, lane};
         bool ok = true;
-        for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
-            SeqTile t;
-            int h;
-            if (!find_item(a, w, heads, lane, &t, &h)) continue;
+        while (walk.found && ok) {
+            const SeqTile t = walk.t;
+            const int h = walk.found_head;
             int kt0, kt1;
             visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
             uint32_t next[2];
             row_bits(next, a, t, kt0 * STEP, lane);
+            // the rows' statistics (absent rows are not stored: 0 will do)
+            float* stat = f.extra + (ld.items & 1) * 2 * ROWS + lane;
+            float lse[4], delta[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int i = t.row0 + x * 32 + lane;
+                const bool there = present(a, t, i);
+                const long long at = (long long)h * a.n_tokens + t.start + i;
+                lse[x] = there ? a.io.lse[at] : 0.f;
+                delta[x] = there ? a.io.delta[at] : 0.f;
+            }
+            ok = ld.slot();
+            if (!ok) break;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                stat[x * 32] = -LOG2E * lse[x];
+                stat[ROWS + x * 32] = -delta[x];
+            }
             ok = ld.item(Item{t.start, t.len, t.row0, h, kt0, kt1 - kt0}, &mq, &mdo);
             for (int j = kt0; j < kt1 && ok; j++) {
                 const uint32_t bits[2] = {next[0], next[1]};
@@ -810,7 +900,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 if (lane < 2) f.slots->bits[ld.issued % STAGES][lane] = lane ? bits[1] : bits[0];
                 ld.tile(&mk, &mv, h / a.group * 64, t.start + j * STEP, bits);
             }
-            ld.fill();  // before the search for the next item
+            walk.next();  // while the last boxes are on their way
+            ld.fill();
         }
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mq, &mdo);
@@ -834,9 +925,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             int col0 = it.t0 * STEP + g * 32;
             const SeqTile t{it.start, it.len, it.row0};
             const bool there = present(a, t, i);
-            const long long at = (long long)it.head * a.n_tokens + t.start + i;
-            // absent rows are not stored: any finite values will do
-            const float e = there ? a.io.lse[at] * LOG2E : 0.f, delta = there ? a.io.delta[at] : 0.f;
+            const float* stat = f.extra + (k & 1) * 2 * ROWS + r;
+            const float e = stat[0], delta = stat[ROWS];
             for (int j = 0; j < n; j++, col0 += STEP, turn.next()) {
                 const uint32_t t_s = lanes + turn.buffer * 64 + g * 32;
                 uint32_t bits;
@@ -851,7 +941,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 if (bits != ~0u || edge(a.window, i - r, ROWS, col0, 32)) mask_row(v, bits, a.window, i, col0);
 #pragma unroll
                 for (int x = 0; x < 32; x += 2) {
-                    const float2 y = fma2(make_float2(v[x], v[x + 1]), make_float2(sl2, sl2), make_float2(-e, -e));
+                    const float2 y = fma2(make_float2(v[x], v[x + 1]), make_float2(sl2, sl2), make_float2(e, e));
                     v[x] = ex2_approx(y.x);
                     v[x + 1] = ex2_approx(y.y);
                 }
@@ -867,7 +957,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                     for (int z = 0; z < 8; z++) {
                         const int c = x + 2 * z;
                         const float2 y = mul2(make_float2(v[c], v[c + 1]),
-                                              add2(make_float2(d[c], d[c + 1]), make_float2(-delta, -delta)));
+                                              add2(make_float2(d[c], d[c + 1]), make_float2(delta, delta)));
                         ds[z] = pack2<T>(y.x, y.y);
                     }
                     tmem_st8(t_s + x, ds);
@@ -897,25 +987,31 @@ __global__ void __launch_bounds__(THREADS, CTAS)
 // TMEM: S^T at columns 0, 64 (dP^T over it, P^T and dS^T over
 // that, 8 columns of each in turn); dV at 128; dK at 192. extra: -lse * log2 e
 // and -delta of each stage's queries.
-using Dkv = Shape<2, 2048, 2 * STAGES * STEP>;
+using Dkv = Shape<2, 2 * STAGES * STEP>;
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS, CTAS)
     attention_dkv_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                             const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
-                            const AttnArgs a, int heads, long long work) {
+                            const AttnArgs a, int heads) {
     extern __shared__ uint8_t raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == LOADER * 32) {
+        prefetch_tmap(&mq);
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+        prefetch_tmap(&mdo);
+    }
+    Walk walk(a, heads, lane, warp == LOADER);
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
 
     if (warp == LOADER) {
         Loader<C> ld{f, a, lane};
         bool ok = true;
-        for (long long w = blockIdx.x; w < work && ok; w += gridDim.x) {
-            SeqTile t;
-            int hk;
-            if (!find_item(a, w, heads, lane, &t, &hk)) continue;
+        while (walk.found && ok) {
+            const SeqTile t = walk.t;
+            const int hk = walk.found_head;
             int qt0, qt1;
             visible_tiles(a, t, ROWS, STEP, &qt0, &qt1);
             // the query tiles of every head of the group
@@ -948,7 +1044,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 stat[STEP + 32] = -d1;
                 ld.tile(&mq, &mdo, head * 64, t.start + row0, bits);
             }
-            ld.fill();  // before the search for the next item
+            walk.next();  // while the last boxes are on their way
+            ld.fill();
         }
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mk, &mv);
@@ -1047,7 +1144,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     close_frame<C>(f, warp);
 }
 
-using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnArgs, int, long long);
+using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnArgs, int);
 
 struct Maps {
     CUtensorMap q, k, v, dout;
@@ -1071,7 +1168,7 @@ cudaError_t launch(Kernel kernel, int heads, const Maps& m, const AttnArgs& a, i
     if (e != cudaSuccess) return e;
     const long long work = seq_tiles(a.n_tokens, a.n_seqs, ROWS) * heads, most = (long long)CTAS * sms;
     kernel<<<(unsigned)(work < most ? work : most), THREADS, smem_bytes<C>(), stream>>>(m.q, m.k, m.v, m.dout, a,
-                                                                                          heads, work);
+                                                                                        heads);
     return cudaGetLastError();
 }
 
