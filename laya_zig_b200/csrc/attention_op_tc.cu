@@ -152,12 +152,24 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err) 
 
 // ------------------------------------------------------------------ items and loads
 
-// Presence bits of N * 32 rows of the sequence from row0.
-template <int N>
-__device__ __forceinline__ void row_bits(uint32_t (&bits)[N], const AttnArgs& a, const SeqTile& t, int row0, int lane) {
-#pragma unroll
-    for (int i = 0; i < N; i++) bits[i] = __ballot_sync(0xffffffffu, present(a, t, row0 + i * 32 + lane));
-}
+// Presence of 64 rows of the sequence, two a lane: read for a tile while the
+// one before is dealt with, made bits of when its turn comes.
+struct Presence {
+    uint32_t v0, v1;
+    __device__ __forceinline__ void read(const AttnArgs& a, const SeqTile& t, int row0, int lane) {
+        const int i0 = row0 + lane, i1 = i0 + 32;
+        v0 = i0 < t.len;
+        v1 = i1 < t.len;
+        if (a.mask) {
+            if (v0) v0 = a.mask[t.start + i0];
+            if (v1) v1 = a.mask[t.start + i1];
+        }
+    }
+    __device__ __forceinline__ void bits(uint32_t (&b)[2]) const {
+        b[0] = __ballot_sync(0xffffffffu, v0 != 0);
+        b[1] = __ballot_sync(0xffffffffu, v1 != 0);
+    }
+};
 
 // The loading warp: items in order, their tiles into the ring. A stage is full
 // when its boxes have landed, zeroed where they must be, and every lane has
@@ -257,44 +269,46 @@ struct Loader {
 };
 
 // The loading warp's walk over the call's items: tile slot x of the call (see
-// seq_tiles) for one head after the other, every gridDim.x-th to a CTA.
+// seq_tiles) for one head after the other. A CTA begins with item blockIdx.x
+// and then takes every gridDim.x-th or, with a counter in global memory, the
+// next that nobody has: sequences of different lengths make items of different
+// cost (128 sequences of 1-512 tokens: dK and dV 214 us by turns, 187 by tickets).
 struct Walk {
     const AttnArgs& a;
     int heads, lane;
-    long long x, slots;
-    int head, dx, dh;  // the next candidate, and the way to the one after
-    long long pivot;   // key of entry lane * step: the search's first round
+    unsigned long long* tickets;
+    unsigned long long ahead;  // the next candidate
+    long long x;               // the candidate's slot
+    int head;
+    long long pivot;  // key of entry lane * step: the search's first round
     int step;
-    SeqTile t;         // the item found
-    int found_head;
+    SeqTile t;  // the item found
     bool found;
 
     // The first item is found here, before the frame is open: its look at the
     // offsets passes while the other warps set the CTA up.
-    __device__ __forceinline__ Walk(const AttnArgs& a_, int heads_, int lane_, bool mine) : a(a_), heads(heads_), lane(lane_) {
+    __device__ __forceinline__ Walk(const AttnArgs& a_, int heads_, int lane_, bool mine, unsigned long long* tickets_)
+        : a(a_), heads(heads_), lane(lane_), tickets(tickets_) {
         found = false;
         if (!mine) return;
-        slots = (long long)(a.n_tokens / ROWS) + a.n_seqs;
-        x = blockIdx.x / heads;
-        head = blockIdx.x % heads;
-        dx = gridDim.x / heads;
-        dh = gridDim.x % heads;
+        ahead = blockIdx.x;
         step = (a.n_seqs + 31) / 32;
         pivot = lane * step < a.n_seqs ? key(a.cu[lane * step], lane * step) : 0;
         next();
     }
     __device__ __forceinline__ static long long key(int start, int s) { return (long long)(max(start, 0) / ROWS) + s; }
     __device__ __forceinline__ void next() {
-        for (found = false; x < slots && !found;) {
+        for (found = false; !found;) {
+            const unsigned long long item = __shfl_sync(0xffffffffu, ahead, 0);
+            x = (long long)(item / heads);
+            head = (int)(item - (unsigned long long)x * heads);
+            if (x >= (long long)(a.n_tokens / ROWS) + a.n_seqs) return;
+            if (!tickets)
+                ahead = item + gridDim.x;
+            else if (lane == 0)
+                ahead = atomicAdd(tickets, 1ull) + gridDim.x;  // not looked at before the item after this one
             if (lane == 0 && head == 0) check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, x, a.status);
             found = find();
-            found_head = head;
-            x += dx;
-            head += dh;
-            if (head >= heads) {
-                head -= heads;
-                x++;
-            }
         }
     }
     // find_tile for slot x, with one look at the table for up to 1,024 sequences.
@@ -577,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
     }
-    Walk walk(a, heads, lane, warp == LOADER);
+    Walk walk(a, heads, lane, warp == LOADER, nullptr);
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
 
@@ -586,15 +600,16 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         bool ok = true;
         while (walk.found && ok) {
             const SeqTile t = walk.t;
-            const int h = walk.found_head;
+            const int h = walk.head;
             int kt0, kt1;
             visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
-            uint32_t next[2];
-            row_bits(next, a, t, kt0 * STEP, lane);
+            Presence rows;
+            rows.read(a, t, kt0 * STEP, lane);
             ok = ld.item(Item{t.start, t.len, t.row0, h, kt0, kt1 - kt0}, &mq, nullptr);
             for (int j = kt0; j < kt1 && ok; j++) {
-                const uint32_t bits[2] = {next[0], next[1]};
-                if (j + 1 < kt1) row_bits(next, a, t, (j + 1) * STEP, lane);
+                uint32_t bits[2];
+                rows.bits(bits);
+                if (j + 1 < kt1) rows.read(a, t, (j + 1) * STEP, lane);
                 ok = ld.room();
                 if (!ok) break;
                 if (lane < 2) f.slots->bits[ld.issued % STAGES][lane] = lane ? bits[1] : bits[0];
@@ -820,6 +835,7 @@ constexpr int DELTA_THREADS = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const AttnArgs a, int heads) {
+    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the two kernels that follow
     const int n = a.n_seqs;
     const int first = max(a.cu[0], 0), last = min(a.cu[n], a.n_tokens);  // rows past either are not the call's
     const long long at = ((long long)blockIdx.x * DELTA_THREADS + threadIdx.x) / 8;
@@ -859,7 +875,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         prefetch_tmap(&mv);
         prefetch_tmap(&mdo);
     }
-    Walk walk(a, heads, lane, warp == LOADER);
+    Walk walk(a, heads, lane, warp == LOADER, a.io.tickets);
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
 
@@ -868,11 +884,11 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         bool ok = true;
         while (walk.found && ok) {
             const SeqTile t = walk.t;
-            const int h = walk.found_head;
+            const int h = walk.head;
             int kt0, kt1;
             visible_tiles(a, t, ROWS, STEP, &kt0, &kt1);
-            uint32_t next[2];
-            row_bits(next, a, t, kt0 * STEP, lane);
+            Presence rows;
+            rows.read(a, t, kt0 * STEP, lane);
             // the rows' statistics (absent rows are not stored: 0 will do)
             float* stat = f.extra + (ld.items & 1) * 2 * ROWS + lane;
             float lse[4], delta[4];
@@ -893,8 +909,9 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             }
             ok = ld.item(Item{t.start, t.len, t.row0, h, kt0, kt1 - kt0}, &mq, &mdo);
             for (int j = kt0; j < kt1 && ok; j++) {
-                const uint32_t bits[2] = {next[0], next[1]};
-                if (j + 1 < kt1) row_bits(next, a, t, (j + 1) * STEP, lane);
+                uint32_t bits[2];
+                rows.bits(bits);
+                if (j + 1 < kt1) rows.read(a, t, (j + 1) * STEP, lane);
                 ok = ld.room();
                 if (!ok) break;
                 if (lane < 2) f.slots->bits[ld.issued % STAGES][lane] = lane ? bits[1] : bits[0];
@@ -1002,7 +1019,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         prefetch_tmap(&mv);
         prefetch_tmap(&mdo);
     }
-    Walk walk(a, heads, lane, warp == LOADER);
+    Walk walk(a, heads, lane, warp == LOADER, a.io.tickets + 1);
     const Frame f = open_frame<C>(raw, warp);
     Bars* bar = f.bar;
 
@@ -1011,17 +1028,18 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         bool ok = true;
         while (walk.found && ok) {
             const SeqTile t = walk.t;
-            const int hk = walk.found_head;
+            const int hk = walk.head;
             int qt0, qt1;
             visible_tiles(a, t, ROWS, STEP, &qt0, &qt1);
             // the query tiles of every head of the group
             const int n = (qt1 - qt0) * a.group;
-            uint32_t next[2];
-            row_bits(next, a, t, qt0 * STEP, lane);
+            Presence rows;
+            rows.read(a, t, qt0 * STEP, lane);
             ok = ld.item(Item{t.start, t.len, t.row0, hk, qt0, n}, &mk, &mv);
             int h = hk * a.group, q = qt0;
             for (int j = 0; j < n && ok; j++) {
-                const uint32_t bits[2] = {next[0], next[1]};
+                uint32_t bits[2];
+                rows.bits(bits);
                 const int row0 = q * STEP;
                 // statistics of rows lane and lane + 32 (0 for rows that are not there: q = dO = 0)
                 const long long at = (long long)h * a.n_tokens + t.start + row0 + lane;
@@ -1033,7 +1051,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                     q = qt0;
                     h++;
                 }
-                if (j + 1 < n) row_bits(next, a, t, q * STEP, lane);
+                if (j + 1 < n) rows.read(a, t, q * STEP, lane);
                 ok = ld.room();
                 if (!ok) break;
                 const int s = ld.issued % STAGES;

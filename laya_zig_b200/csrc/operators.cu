@@ -113,6 +113,12 @@ int check_attention(const char* op, const laya_attention* a) {
     return LAYA_OK;
 }
 
+// Two counters, then delta.
+constexpr uint64_t WORKSPACE_HEAD = 16;
+uint64_t workspace_bytes_of(const laya_attention* a) {
+    return WORKSPACE_HEAD + (uint64_t)a->n_heads * a->n_tokens * sizeof(float);
+}
+
 struct Rows {
     const char* name;
     const void* p;
@@ -256,7 +262,7 @@ int laya_gpu_attention(const laya_attention* a, const void* q, int64_t q_stride,
 
 uint64_t laya_gpu_attention_backward_workspace(const laya_attention* a) {
     if (check_attention("attention_backward_workspace", a)) return 0;
-    return (uint64_t)a->n_heads * a->n_tokens * sizeof(float);  // delta
+    return a->n_tokens ? workspace_bytes_of(a) : 0;
 }
 
 int laya_gpu_attention_backward(const laya_attention* a, const void* q, int64_t q_stride, const void* k,
@@ -275,7 +281,7 @@ int laya_gpu_attention_backward(const laya_attention* a, const void* q, int64_t 
     for (const Rows& x : r)
         if (int rc = check_rows(op, x)) return rc;
     if (!lse) return fail(LAYA_ERR_ARG, "%s: lse is NULL", op);
-    const uint64_t need = (uint64_t)hq * a->n_tokens * sizeof(float);
+    const uint64_t need = workspace_bytes_of(a);
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
         return fail(LAYA_ERR_ARG, "%s: the workspace needs %llu bytes, 16-byte aligned", op,
                     (unsigned long long)need);
@@ -283,7 +289,7 @@ int laya_gpu_attention_backward(const laya_attention* a, const void* q, int64_t 
     const Span s[] = {span(r[0], T), span(r[1], T), span(r[2], T), span(r[3], T), span(r[4], T), span(r[5], T),
                       span(r[6], T), span(r[7], T),
                       {"lse", lse, (int64_t)T * 4, (int64_t)T * 4, hq, false},
-                      {"workspace", workspace, (int64_t)T * 4, (int64_t)T * 4, hq, true}};
+                      {"workspace", workspace, (int64_t)need, (int64_t)need, 1, true}};
     if (int rc = check_overlap(op, s)) return rc;
     const Ptr ptrs[] = {{"q", q}, {"k", k}, {"v", v}, {"out", out}, {"lse", lse}, {"dout", dout}, {"dq", dq},
                         {"dk", dk}, {"dv", dv}, {"workspace", workspace}, {"cu_seqlens", a->cu_seqlens},
@@ -299,7 +305,8 @@ int laya_gpu_attention_backward(const laya_attention* a, const void* q, int64_t 
     io.dk = {dk, dk_stride};
     io.dv = {dv, dv_stride};
     io.lse = const_cast<float*>(lse);
-    io.delta = static_cast<float*>(workspace);
+    io.tickets = static_cast<unsigned long long*>(workspace);
+    io.delta = static_cast<float*>(workspace) + WORKSPACE_HEAD / sizeof(float);
     const cudaError_t e = launch_attention_bwd(*a, io, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? LAYA_OK : cuda_fail(op, e);
 }

@@ -111,7 +111,8 @@ struct AttnRows {
 struct AttnIO {
     AttnRows q, k, v, out, dout, dq, dk, dv;
     float* lse;    // [n_heads][n_tokens]
-    float* delta;  // [n_heads][n_tokens], the backward pass's workspace
+    float* delta;  // [n_heads][n_tokens], of the backward pass's workspace
+    unsigned long long* tickets;  // two counters, of the workspace
 };
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream);
 cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream);
