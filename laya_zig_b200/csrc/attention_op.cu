@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const AttnArgs
     T* sv = sk + 2 * TILE;
     __shared__ uint32_t bits[2][2];
     __shared__ float sdelta[TB];
+    griddep_launch();
     SeqTile t;
     if (!block_tile(a, &t)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -378,6 +379,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const AttnArg
     T* sdo = sq + 2 * TILE;
     float* slse = reinterpret_cast<float*>(sdo + 2 * TILE);  // [2][64]
     float* sdelta = slse + 2 * TB;
+    griddep_wait();  // delta comes from the kernel before, which this one's launch overlaps
     SeqTile t;
     if (!block_tile(a, &t)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -470,43 +472,44 @@ AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
     return g;
 }
 
-cudaError_t launch(void (*kernel)(AttnArgs), unsigned heads, int smem, const AttnArgs& g, cudaStream_t stream) {
+cudaError_t launch(void (*kernel)(AttnArgs), unsigned heads, int smem, const AttnArgs& g, bool dependent,
+                   cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), heads);
+    if (dependent) return launch_k(kernel, grid, THREADS, smem, stream, g);
     kernel<<<grid, THREADS, smem, stream>>>(g);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-// Calls whose longest sequence has at least this many tokens go to tcgen05
-// (LAYA_ATTN_OP_TC_MIN_LEN in the environment overrides).
-static uint32_t tc_min_len() {
-    static const uint32_t v = [] {
-        const char* e = getenv("LAYA_ATTN_OP_TC_MIN_LEN");
-        return e && *e ? (uint32_t)strtoul(e, nullptr, 10) : 65u;
-    }();
-    return v;
+// Which kernels a call gets: 64-row mma.sync blocks while they all fit the GPU
+// at once and their sequences are short, tcgen05 otherwise. Forward and
+// backward, 12 heads, us by mma.sync / tcgen05: 1 x 64 tokens 13.8 / 20.7, 1 x
+// 256 25.5 / 28.9, 64 x 16 39.8 / 44.6; 1 x 512 40.7 / 38.5, 64 x 64 45.9 /
+// 48.3, 64 x 100 101 / 68, 512 x 64 331 / 250.
+static bool small_call(const laya_attention& a) {
+    return a.max_len <= 256 && (uint64_t)a.n_tokens * a.n_heads <= 32768;
 }
 
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
-    if (a.max_len >= tc_min_len())
-        return launch_attention_fwd_tc(a.elem_dtype == LAYA_DT_BF16, (int)a.n_heads, make_args(a, io), stream);
-    return launch(a.elem_dtype == LAYA_DT_BF16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>,
-                  a.n_heads, FWD_SMEM, make_args(a, io), stream);
+    const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
+    const AttnArgs g = make_args(a, io);
+    if (!small_call(a)) return launch_attention_fwd_tc(bf16, (int)a.n_heads, g, stream);
+    return launch(bf16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>, a.n_heads, FWD_SMEM, g, false,
+                  stream);
 }
 
 cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
     const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
     const AttnArgs g = make_args(a, io);
-    if (a.max_len >= tc_min_len())
-        return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
-    cudaError_t e = launch(bf16 ? attention_dq_kernel<__nv_bfloat16> : attention_dq_kernel<__half>, a.n_heads,
-                           DQ_SMEM, g, stream);
+    if (!small_call(a)) return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
+    cudaError_t e = launch(bf16 ? attention_dq_kernel<__nv_bfloat16> : attention_dq_kernel<__half>, a.n_heads, DQ_SMEM, g,
+                           false, stream);
     if (e == cudaSuccess)
-        e = launch(bf16 ? attention_dkv_kernel<__nv_bfloat16> : attention_dkv_kernel<__half>, a.n_kv_heads, DKV_SMEM,
-                   g, stream);
+        e = launch(bf16 ? attention_dkv_kernel<__nv_bfloat16> : attention_dkv_kernel<__half>, a.n_kv_heads, DKV_SMEM, g,
+                   true, stream);
     return e;
 }
 

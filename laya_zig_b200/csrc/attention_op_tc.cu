@@ -285,8 +285,8 @@ struct Walk {
     SeqTile t;  // the item found
     bool found;
 
-    // The first item is found here, before the frame is open: its look at the
-    // offsets passes while the other warps set the CTA up.
+    // Finds the first item (in the forward, before the frame is open: the look
+    // at the offsets passes while the other warps set the CTA up).
     __device__ __forceinline__ Walk(const AttnArgs& a_, int heads_, int lane_, bool mine, unsigned long long* tickets_)
         : a(a_), heads(heads_), lane(lane_), tickets(tickets_) {
         found = false;
@@ -835,6 +835,7 @@ constexpr int DELTA_THREADS = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const AttnArgs a, int heads) {
+    griddep_launch();
     if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the two kernels that follow
     const int n = a.n_seqs;
     const int first = max(a.cu[0], 0), last = min(a.cu[n], a.n_tokens);  // rows past either are not the call's
@@ -875,8 +876,10 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         prefetch_tmap(&mv);
         prefetch_tmap(&mdo);
     }
-    Walk walk(a, heads, lane, warp == LOADER, a.io.tickets);
+    griddep_launch();
     const Frame f = open_frame<C>(raw, warp);
+    griddep_wait();  // from here on, what earlier kernels wrote
+    Walk walk(a, heads, lane, warp == LOADER, a.io.tickets);
     Bars* bar = f.bar;
 
     if (warp == LOADER) {
@@ -1019,8 +1022,9 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         prefetch_tmap(&mv);
         prefetch_tmap(&mdo);
     }
-    Walk walk(a, heads, lane, warp == LOADER, a.io.tickets + 1);
     const Frame f = open_frame<C>(raw, warp);
+    griddep_wait();  // from here on, what earlier kernels wrote
+    Walk walk(a, heads, lane, warp == LOADER, a.io.tickets + 1);
     Bars* bar = f.bar;
 
     if (warp == LOADER) {
@@ -1181,12 +1185,16 @@ int sm_count() {
 }
 
 template <typename C>
-cudaError_t launch(Kernel kernel, int heads, const Maps& m, const AttnArgs& a, int sms, cudaStream_t stream) {
+cudaError_t launch(Kernel kernel, int heads, const Maps& m, const AttnArgs& a, int sms, bool dependent,
+                   cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<C>());
     if (e != cudaSuccess) return e;
     const long long work = seq_tiles(a.n_tokens, a.n_seqs, ROWS) * heads, most = (long long)CTAS * sms;
-    kernel<<<(unsigned)(work < most ? work : most), THREADS, smem_bytes<C>(), stream>>>(m.q, m.k, m.v, m.dout, a,
-                                                                                        heads);
+    const dim3 grid((unsigned)(work < most ? work : most));
+    // dependent: the kernel before belongs to the same call, and this one may
+    // set itself up while that one ends
+    if (dependent) return launch_k(kernel, grid, THREADS, smem_bytes<C>(), stream, m.q, m.k, m.v, m.dout, a, heads);
+    kernel<<<grid, THREADS, smem_bytes<C>(), stream>>>(m.q, m.k, m.v, m.dout, a, heads);
     return cudaGetLastError();
 }
 
@@ -1200,7 +1208,7 @@ cudaError_t launch_attention_fwd_tc(bool bf16, int n_heads, const AttnArgs& a, c
         return cudaErrorInvalidValue;
     m.dout = m.q;  // not used
     return launch<Fwd>(bf16 ? attention_fwd_tc_kernel<__nv_bfloat16, Fwd> : attention_fwd_tc_kernel<__half, Fwd>, n_heads, m,
-                       a, sm_count(), stream);
+                       a, sm_count(), false, stream);
 }
 
 cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, const AttnArgs& a, cudaStream_t stream) {
@@ -1218,10 +1226,10 @@ cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, cons
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     e = launch<Dq>(bf16 ? attention_dq_tc_kernel<__nv_bfloat16, Dq> : attention_dq_tc_kernel<__half, Dq>, n_heads, m, a, sms,
-                   stream);
+                   true, stream);
     if (e == cudaSuccess)
         e = launch<Dkv>(bf16 ? attention_dkv_tc_kernel<__nv_bfloat16, Dkv> : attention_dkv_tc_kernel<__half, Dkv>,
-                        n_kv_heads, m, a, sms, stream);
+                        n_kv_heads, m, a, sms, true, stream);
     return e;
 }
 

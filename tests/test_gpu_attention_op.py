@@ -12,6 +12,11 @@ pytestmark = pytest.mark.gpu
 
 POISON = 4  # rows of NaN before the first and behind the last sequence
 
+# Short sequences and few tokens go to one set of kernels, the rest to another;
+# a longest length that no sequence reaches asks for the second.
+LONG = 5000
+kernels = pytest.mark.parametrize("max_len", [None, LONG], ids=["small", "large"])
+
 
 class Problem:
     """Packed rows with columns to spare, NaN wherever no present token is."""
@@ -124,16 +129,18 @@ LENGTHS = {"one": [1], "tile": [64], "tile+1": [65], "edges": [1, 63, 64, 65, 0,
 @pytest.mark.parametrize("dtype", ["BF16", "F16"])
 @pytest.mark.parametrize("window", [-1, 0, 1, 64, 1000])
 @pytest.mark.parametrize("lens", list(LENGTHS))
-def test_lengths_and_windows(lens, window, dtype):
-    p = Problem(LENGTHS[lens], window=window, dtype=dtype)
+@kernels
+def test_lengths_and_windows(lens, window, dtype, max_len):
+    p = Problem(LENGTHS[lens], window=window, dtype=dtype, max_len=max_len)
     p.run()
     p.check()
 
 
 @pytest.mark.parametrize("hq,hk", [(1, 1), (3, 1), (6, 2), (12, 12), (12, 4)])
 @pytest.mark.parametrize("window", [-1, 17])
-def test_head_groups(hq, hk, window):
-    p = Problem([70, 129], hq=hq, hk=hk, window=window, seed=hq)
+@kernels
+def test_head_groups(hq, hk, window, max_len):
+    p = Problem([70, 129], hq=hq, hk=hk, window=window, seed=hq, max_len=max_len)
     p.run()
     p.check()
 
@@ -154,36 +161,43 @@ def _only(*kept):
 @pytest.mark.parametrize("mask", [_every(2), _every(3), _only(), _only(0), _only(130, 131), _only(63, 64, 200)],
                          ids=["half", "third", "none", "first", "tile2", "across"])
 @pytest.mark.parametrize("window", [-1, 5])
-def test_absent_tokens(mask, window, dtype):
+@kernels
+def test_absent_tokens(mask, window, dtype, max_len):
     """NaN in every absent token's rows; sequences with no token left."""
-    p = Problem([66, 1, 190, 64], window=window, mask=mask, dtype=dtype, hq=2, hk=1)
+    p = Problem([66, 1, 190, 64], window=window, mask=mask, dtype=dtype, hq=2, hk=1, max_len=max_len)
     p.run()
     p.check()
 
 
-def test_large_scores():
+@kernels
+def test_large_scores(max_len):
     """Scores of some hundreds: rows that put all weight on one key, and keys
     no query gives any."""
-    p = Problem([200, 31], spread=8.0, dtype="BF16", scale=0.5)
+    p = Problem([200, 31], spread=8.0, dtype="BF16", scale=0.5, max_len=max_len)
     p.run()
     p.check()
 
 
-def test_scale_and_padded_rows():
-    p = Problem([130], scale=0.7, pad=64, dtype="F16", hq=4, hk=2)
+@kernels
+def test_scale_and_padded_rows(max_len):
+    p = Problem([130], scale=0.7, pad=64, dtype="F16", hq=4, hk=2, max_len=max_len)
     p.run()
     p.check()
 
 
-def test_many_short_sequences():
+@kernels
+@pytest.mark.parametrize("n", [700, 1500])
+def test_many_short_sequences(n, max_len):
+    """More than 1,024 of them: the search for a tile takes another round."""
     rng = np.random.default_rng(5)
-    p = Problem(rng.integers(0, 9, 700).tolist() + [1], hq=2, hk=1, window=3)
+    p = Problem(rng.integers(0, 9, n).tolist() + [1], hq=2, hk=1, window=3, max_len=max_len)
     p.run()
     p.check()
 
 
-def test_same_bits_every_time():
-    a = Problem([300, 77, 180], hq=6, hk=2, mask=_every(5))
+@pytest.mark.parametrize("lens", [[200, 77, 180], [300, 77, 180], [1200, 700]])
+def test_same_bits_every_time(lens):
+    a = Problem(lens, hq=6, hk=2, mask=_every(5))
     a.run()
     first = (a.out.clone(), a.lse.clone(), a.dqkv.clone())
     import torch
@@ -194,12 +208,13 @@ def test_same_bits_every_time():
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
-def test_gradient_against_differences():
+@kernels
+def test_gradient_against_differences(max_len):
     """sum(out * dout) of the definition, moved both ways along random
     directions, against the kernel's gradients: they agree within the
     gradients' own bounds plus the differences' h^2 term."""
     import torch
-    p = Problem([90], hq=2, hk=1, window=40, dtype="F16", seed=3)
+    p = Problem([90], hq=2, hk=1, window=40, dtype="F16", seed=3, max_len=max_len)
     p.run()
     rows = torch.arange(POISON, POISON + 90, device="cuda")
     x = p.qkv[rows][:, :256].double().reshape(90, 4, 64)
@@ -222,10 +237,11 @@ def test_gradient_against_differences():
         assert abs((g * d).sum() - d1) <= (bound * d.abs()).sum() + 2 * (d2 - d1).abs()
 
 
-def test_forward_without_statistics():
+@kernels
+def test_forward_without_statistics(max_len):
     import torch
     from laya_zig_b200 import gpu
-    p = Problem([100, 3])
+    p = Problem([100, 3], max_len=max_len)
     p.forward()
     want = p.out.clone()
     p.out.fill_(7.0)
@@ -233,13 +249,15 @@ def test_forward_without_statistics():
     assert torch.equal(want, p.out)
 
 
-@pytest.mark.parametrize("table", [[0, 50, 40, 100], [-3, 20, 60, 100], [0, 30, 60, 5000], [90, 60, 30, 0],
-                                   [0, 10, 20, 100]])
-def test_broken_offsets_are_recorded(table):
-    """Decreasing, negative, too far and (the last) a run longer than max_len."""
+@pytest.mark.parametrize("table,max_len", [([0, 50, 40, 100], 60), ([-3, 20, 60, 100], 60), ([0, 30, 60, 5000], 60),
+                                           ([90, 60, 30, 0], 60), ([0, 10, 20, 100], 60), ([0, 50, 40, 100], LONG),
+                                           ([-3, 20, 60, 100], LONG), ([0, 30, 60, 5000], LONG),
+                                           ([90, 60, 30, 0], LONG), ([-70, -60, 30, 0], LONG)])
+def test_broken_offsets_are_recorded(table, max_len):
+    """Decreasing, negative, too far, and a run longer than max_len."""
     import torch
     from laya_zig_b200 import gpu
-    p = Problem([30, 30, 40], max_len=60)
+    p = Problem([30, 30, 40], max_len=max_len)
     p.forward()  # sets the pointers
     gpu.op_status(p.status.data_ptr())
     p.cu.copy_(torch.tensor(table, dtype=torch.int32))
@@ -261,12 +279,13 @@ def test_host_memory_is_refused():
     assert e.value.code == gpu.ERR_ARG and "device memory" in str(e.value)
 
 
-def test_captured_and_replayed_on_new_inputs():
+@pytest.mark.parametrize("max_len", [200, LONG])
+def test_captured_and_replayed_on_new_inputs(max_len):
     """Forward and backward in one CUDA graph, replayed after the inputs and
     the offsets changed, give what eager calls give."""
     import torch
-    a = Problem([100, 60, 30], hq=4, hk=2, seed=1, max_len=200)
-    b = Problem([20, 160, 10], hq=4, hk=2, seed=2, max_len=200)
+    a = Problem([100, 60, 30], hq=4, hk=2, seed=1, max_len=max_len)
+    b = Problem([20, 160, 10], hq=4, hk=2, seed=2, max_len=max_len)
     s = torch.cuda.Stream()
     with torch.cuda.stream(s):
         a.run(s.cuda_stream)
@@ -285,9 +304,10 @@ def test_captured_and_replayed_on_new_inputs():
     assert torch.equal(a.dqkv, b.dqkv) and torch.equal(a.out, b.out)
 
 
-def test_two_streams_at_once():
+@pytest.mark.parametrize("lens", [[100, 30], [400, 300]])
+def test_two_streams_at_once(lens):
     import torch
-    ps = [Problem([400, 300], seed=i) for i in range(2)]
+    ps = [Problem(lens, seed=i) for i in range(2)]
     for p in ps:
         p.run()
     want = [p.dqkv.clone() for p in ps]

@@ -204,24 +204,54 @@ def find_tile(cu, n_seqs, n_tokens, max_len, rows, x):
     return s, start, end - start, tile * rows
 
 
+def walk_find(cu, n_seqs, n_tokens, max_len, rows, x):
+    """The search of csrc/attention_op_tc.cu's Walk: the first round's keys
+    kept, the second round's entries handed among the lanes."""
+    if n_seqs > 1024:
+        return find_tile(cu, n_seqs, n_tokens, max_len, rows, x)
+
+    def key(start, s):
+        return max(start, 0) // rows + s
+    step = (n_seqs + 31) // 32
+    c = sum(lane * step < n_seqs and key(cu[lane * step], lane * step) <= x for lane in range(32))
+    if c == 0:
+        return None
+    lo = (c - 1) * step
+    m = min(step, n_seqs - lo)
+    at = [cu[min(lo + lane, n_seqs)] for lane in range(32)]
+    c1 = sum(lane < m and key(at[lane], lo + lane) <= x for lane in range(32))
+    if c1 == 0:
+        return None
+    s = lo + c1 - 1
+    start, end = at[c1 - 1], at[c1] if c1 < 32 else cu[s + 1]
+    if not (start >= 0 and end >= start and end <= n_tokens and end - start <= max_len):
+        return None
+    tile = x - key(start, s)
+    if tile < 0 or tile * rows >= end - start:
+        return None
+    return s, start, end - start, tile * rows
+
+
+@pytest.mark.parametrize("find", [find_tile, walk_find])
 @pytest.mark.parametrize("rows", [64, 128, 256])
 @pytest.mark.parametrize("seed", range(12))
-def test_every_tile_has_one_block(rows, seed):
+def test_every_tile_has_one_block(rows, seed, find):
     r = random.Random(seed * 7 + rows)
-    n = r.choice([1, 2, 31, 32, 33, 64, 200, 1025])
+    n = r.choice([1, 2, 31, 32, 33, 64, 200, 1023, 1024, 1025])
     lens = [r.choice([0, 1, rows - 1, rows, rows + 1, r.randint(0, 700)]) for _ in range(n)]
     cu = [r.choice([0, 5, 300])]
     for v in lens:
         cu.append(cu[-1] + v)
     T = cu[-1] + r.choice([0, 17])
     want = {(s, row0) for s, v in enumerate(lens) for row0 in range(0, v, rows)}
-    got = [find_tile(cu, n, T, max(lens), rows, x) for x in range(T // rows + n)]
+    got = [find(cu, n, T, max(lens), rows, x) for x in range(T // rows + n)]
     got = [(g[0], g[3]) for g in got if g]
     assert len(got) == len(set(got)) and set(got) == want
 
 
+@pytest.mark.parametrize("find,rows", [(find_tile, 64), (walk_find, 128)])
 @pytest.mark.parametrize("seed", range(30))
-def test_broken_tables_name_no_row_outside(seed):
+def test_broken_tables_name_no_row_outside(seed, find, rows):
     """Unsorted, negative and overlong entries: an accepted tile's rows stay
     inside [0, n_tokens)."""
     r = random.Random(seed)
@@ -229,8 +259,8 @@ def test_broken_tables_name_no_row_outside(seed):
     cu = [r.randint(-50, 1100) for _ in range(n + 1)]
     if r.random() < 0.5:
         cu.sort()
-    for x in range(T // 64 + n):
-        g = find_tile(cu, n, T, 400, 64, x)
+    for x in range(T // rows + n):
+        g = find(cu, n, T, 400, rows, x)
         if g:
             s, start, L, row0 = g
             assert 0 <= s < n and 0 <= start and start + L <= T and 0 <= row0 < L <= 400
