@@ -22,7 +22,7 @@ namespace laya {
 namespace {
 
 constexpr int THREADS = 128;
-constexpr float LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Scalars {
     const int* cu;
@@ -87,6 +87,13 @@ __device__ __forceinline__ Decision load_decision(const Scalars& s, const Policy
     return d;
 }
 
+// log2 on the SFU: absolute error about 2^-22
+__device__ __forceinline__ float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 struct Result {
     float loss, logp, kl, ent;
     float g;  // d loss / d logp through the clipped ratio
@@ -97,7 +104,7 @@ __device__ __forceinline__ Result finish(const Scalars& s, const Decision& d, fl
     r.logp = logp;
     r.kl = kl;
     r.ent = ent;
-    const float ratio = expf(logp - d.old_logp);
+    const float ratio = ex2_approx((logp - d.old_logp) * LOG2E);
     const float free_ = ratio * d.adv;
     const float held = fminf(fmaxf(ratio, s.lo), s.hi) * d.adv;
     const bool active = !(free_ > held);  // NaN stays NaN
@@ -145,7 +152,8 @@ __device__ __forceinline__ Slope slope(const Scalars& s, const Decision& d, cons
     return c;
 }
 
-template <typename T, int G, int V>
+// REF: there are reference logits.
+template <typename T, int G, int V, bool REF>
 __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io) {
     static_assert(G <= 32 || G == THREADS, "a decision is part of a warp, a warp or a block");
     __shared__ float2 buf[3][THREADS / 32];  // one row for each block-wide reduction
@@ -156,7 +164,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
     Decision d = load_decision<T>(s, io, i);
     if (live && !d.ok && l == 0) atomicOr(s.status, ERR_BAD_INDEX);
     const T* x = static_cast<const T*>(io.logits) + d.start;
-    const T* xr = static_cast<const T*>(io.ref) + d.start;
+    const T* xr = REF ? static_cast<const T*>(io.ref) + d.start : x;
     const int k = d.k;
     // thread l holds options l, l + G, ..; all loads are under way before the
     // first is used
@@ -166,7 +174,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
 #pragma unroll
         for (int v = 0; v < V; v++)
             if (l + v * G < k) raw[v] = x[l + v * G];
-        if (io.ref) {
+        if (REF) {
 #pragma unroll
             for (int v = 0; v < V; v++)
                 if (l + v * G < k) rawr[v] = xr[l + v * G];
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
 #pragma unroll
         for (int v = 0; v < V; v++) {
             z[v] = l + v * G < k ? to_float(raw[v]) * d.scale : -INFINITY;
-            zr[v] = io.ref && l + v * G < k ? to_float(rawr[v]) * d.scale : -INFINITY;
+            zr[v] = REF && l + v * G < k ? to_float(rawr[v]) * d.scale : -INFINITY;
         }
     }
     float m = -INFINITY, mr = -INFINITY;
@@ -192,11 +200,11 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
     for (int v = 0; v < V; v++) {
         if (v * G >= k) break;  // of the whole group
         sum += ex2_approx(z[v] - mz);
-        if (io.ref) sumr += ex2_approx(zr[v] - mrz);
+        if (REF) sumr += ex2_approx(zr[v] - mrz);
     }
     group_reduce<G, false>(sum, sumr, buf[1]);
     const bool some = d.ok && !(sum == 0.f);  // an option that is not ruled out
-    const float lse = mz + log2f(sum), lser = mrz + log2f(sumr);
+    const float lse = mz + lg2_approx(sum), lser = mrz + lg2_approx(sumr);
     float ent = 0.f, kl = 0.f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
         z[v] -= lse;  // log2 p
         p[v] = ex2_approx(z[v]);
         if (!(p[v] == 0.f)) ent = fmaf(-p[v], z[v], ent);
-        if (io.ref && l + v * G < k) {
+        if (REF && l + v * G < k) {
             zr[v] -= lser;
             const float dv = z[v] - zr[v];
             kl += kl_term(dv, p[v], zr[v]);
@@ -223,7 +231,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
             if (v * G >= k) break;
             const int j = l + v * G;
             float g = fmaf(c.c2, z[v], c.c0);
-            if (io.ref) g = fmaf(c.c1, zr[v], g);
+            if (REF) g = fmaf(c.c1, zr[v], g);
             g = p[v] == 0.f ? 0.f : p[v] * g;  // an option that is ruled out has log p = -inf
             if (j == d.action) g += c.own;
             if (j < k) dx[j] = from_float<T>(some ? g : 0.f);
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyI
         }
         group_reduce<THREADS, false>(sum, sumr, buf[1]);
         const bool some = d.ok && !(sum == 0.f);
-        const float lse = mz + log2f(sum), lser = mrz + log2f(sumr);
+        const float lse = mz + lg2_approx(sum), lser = mrz + lg2_approx(sumr);
         float ent = 0.f, kl = 0.f;
         for (int j = threadIdx.x; j < k; j += THREADS) {
             const float lp = to_float(x[j]) * d.scale - lse, p = ex2_approx(lp);
@@ -288,7 +296,11 @@ __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyI
 template <typename T, int G, int V>
 cudaError_t launch_g(const Scalars& s, const PolicyIO& io, cudaStream_t stream) {
     constexpr int per = THREADS / G;
-    policy_kernel<T, G, V><<<(unsigned)(((long long)s.n + per - 1) / per), THREADS, 0, stream>>>(s, io);
+    const unsigned grid = (unsigned)(((long long)s.n + per - 1) / per);
+    if (io.ref)
+        policy_kernel<T, G, V, true><<<grid, THREADS, 0, stream>>>(s, io);
+    else
+        policy_kernel<T, G, V, false><<<grid, THREADS, 0, stream>>>(s, io);
     return cudaGetLastError();
 }
 
