@@ -306,8 +306,16 @@ cudaError_t launch_g(const Scalars& s, const PolicyIO& io, cudaStream_t stream) 
 
 template <typename T>
 cudaError_t launch_t(const Scalars& s, const PolicyIO& io, cudaStream_t stream) {
-    if (s.max_k <= 16) return launch_g<T, 8, 2>(s, io, stream);
-    if (s.max_k <= 128) return launch_g<T, 32, 4>(s, io, stream);
+    // The fewest threads to a decision that hold its options in registers:
+    // what a group does once (its scalars, three reductions) is half the work.
+    // 4 M options (f32) in decisions of up to 16 / 64 / 256: 17 / 14 / 13 us;
+    // with the next larger group 26 / 19 / 19 us.
+    if (s.max_k <= 16) return launch_g<T, 4, 4>(s, io, stream);
+    if (s.max_k <= 32) return launch_g<T, 8, 4>(s, io, stream);
+    if (s.max_k <= 64) return launch_g<T, 8, 8>(s, io, stream);
+    if (s.max_k <= 128) return launch_g<T, 16, 8>(s, io, stream);
+    if (s.max_k <= 256) return launch_g<T, 32, 8>(s, io, stream);
+    if (s.max_k <= 512) return launch_g<T, 32, 16>(s, io, stream);
     if (s.max_k <= 1024) return launch_g<T, THREADS, 8>(s, io, stream);
     policy_wide_kernel<T><<<(unsigned)(s.n < 148 * 8 ? s.n : 148 * 8), THREADS, 0, stream>>>(s, io);
     return cudaGetLastError();

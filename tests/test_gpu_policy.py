@@ -130,8 +130,9 @@ def _check(lens, dtype="F32", klc=0.1, entc=0.03, use_ref=True, use_q=True, use_
     return got
 
 
-SHAPES = {"one": [1], "four": [4] * 9, "mixed": [4, 16, 1, 0, 7, 9, 16, 2], "to32": [17, 32, 5, 31, 128, 1, 0],
-          "wide": [129, 1000, 1024, 3], "wider": [1025, 3, 4000, 0]}
+SHAPES = {"one": [1], "four": [4] * 9, "mixed": [4, 16, 1, 0, 7, 9, 16, 2], "to32": [17, 32, 5, 31, 1, 0],
+          "to64": [33, 64, 2, 0, 63, 8], "to128": [17, 65, 5, 31, 128, 1, 0], "to256": [129, 256, 1, 32, 33],
+          "to512": [257, 512, 31, 0, 4], "wide": [129, 1000, 1024, 3], "wider": [1025, 3, 4000, 0]}
 
 
 @pytest.mark.parametrize("dtype", ["F32", "BF16", "F16"])
@@ -140,7 +141,7 @@ def test_shapes(lens, dtype):
     _check(SHAPES[lens], dtype)
 
 
-@pytest.mark.parametrize("lens", ["mixed", "to32", "wide", "wider"])
+@pytest.mark.parametrize("lens", ["mixed", "to32", "to64", "to128", "to256", "to512", "wide", "wider"])
 @pytest.mark.parametrize("kw", [dict(ruled_out=0.4), dict(use_ref=False), dict(use_q=False), dict(use_grad=False),
                                 dict(klc=0.0, entc=0.0), dict(spread=30.0), dict(klc=3.0, entc=-1.0, seed=9)])
 def test_forms(lens, kw):
@@ -208,7 +209,7 @@ def test_outputs_are_optional():
             assert torch.equal(part[k], full[k]) if k == name else (part[k] == 7).all()
 
 
-@pytest.mark.parametrize("max_options", [16, 128, 1024, 5000])
+@pytest.mark.parametrize("max_options", [16, 32, 64, 128, 256, 512, 1024, 5000])
 def test_bad_indices_are_recorded(max_options):
     """An action outside its decision, a question type above 2: the decision's
     outputs are 0, the others' untouched by it."""
