@@ -464,7 +464,7 @@ AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
     g.status = a.status;
     g.n_seqs = (int)a.n_seqs;
     g.n_tokens = (int)a.n_tokens;
-    g.max_len = (int)a.max_len;
+    g.max_len = (int)(a.max_len < a.n_tokens ? a.max_len : a.n_tokens);
     g.group = (int)(a.n_heads / a.n_kv_heads);
     g.window = a.window;
     g.scale = a.scale;

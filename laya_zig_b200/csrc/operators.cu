@@ -29,15 +29,19 @@ int cuda_fail(const char* op, cudaError_t e) {
 
 constexpr uint32_t MAX_ROWS = 1u << 30;  // row indexes and their sums with a tile stay inside 32 bits
 
-// Is every pointer (nullptr entries skipped) memory that a kernel on the
-// current device may use? Host memory and another device's are refused here
-// instead of faulting there.
+// Is every pointer (nullptr entries skipped) aligned, and memory that a kernel
+// on the current device may use? Host memory and another device's are refused
+// here instead of faulting there.
 struct Ptr {
     const char* name;
     const void* p;
+    unsigned align = 4;  // bytes
 };
 template <int N>
-int check_device(const char* op, const Ptr (&ptrs)[N]) {
+int check_pointers(const char* op, const Ptr (&ptrs)[N]) {
+    for (const Ptr& x : ptrs)
+        if ((uintptr_t)x.p % x.align)
+            return fail(LAYA_ERR_ARG, "%s: %s must be %u-byte aligned", op, x.name, x.align);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) {
@@ -106,7 +110,7 @@ int check_attention(const char* op, const laya_attention* a) {
         return fail(LAYA_ERR_ARG, "%s: %u tokens, %u sequences (2^30 at most)", op, a->n_tokens, a->n_seqs);
     if (!a->n_heads || !a->n_kv_heads || a->n_heads % a->n_kv_heads || a->n_heads > 65535)
         return fail(LAYA_ERR_ARG, "%s: %u heads over %u key heads", op, a->n_heads, a->n_kv_heads);
-    if (!(a->scale > 0.f) || !std::isfinite(a->scale))
+    if (!(a->scale > 0.f) || !std::isfinite(2.f * a->scale))  // it is multiplied by log2 e
         return fail(LAYA_ERR_ARG, "%s: scale must be positive and finite", op);
     if (a->n_tokens && a->n_seqs && (!a->cu_seqlens || !a->status))
         return fail(LAYA_ERR_ARG, "%s: NULL cu_seqlens or status", op);
@@ -147,7 +151,7 @@ extern "C" {
 int laya_gpu_op_status(int32_t* status, void* stream) {
     if (!status) return fail(LAYA_ERR_ARG, "op_status: status is NULL");
     const Ptr ptrs[] = {{"status", status}};
-    if (int rc = check_device("op_status", ptrs)) return rc;
+    if (int rc = check_pointers("op_status", ptrs)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     int32_t v = 0;
     cudaError_t e = cudaMemcpyAsync(&v, status, 4, cudaMemcpyDeviceToHost, s);
@@ -216,14 +220,13 @@ int laya_gpu_rope(const laya_rope_plan* plan, const void* x, int64_t x_stride, v
     if (width > (int64_t)1 << 30) return fail(LAYA_ERR_ARG, "rope: %u heads of %u", heads, plan->head_dim);
     if (x_stride < width || y_stride < width || x_stride > (int64_t)1 << 31 || y_stride > (int64_t)1 << 31)
         return fail(LAYA_ERR_ARG, "rope: a stride is less than %u heads x %u", heads, plan->head_dim);
-    if (((uintptr_t)x | (uintptr_t)y) % e) return fail(LAYA_ERR_ARG, "rope: x or y is not aligned to its elements");
     if (x != y || x_stride != y_stride) {
         const Span s[] = {{"x", x, x_stride * e, width * e, n_tokens, false},
                           {"y", y, y_stride * e, width * e, n_tokens, true}};
         if (int rc = check_overlap("rope", s)) return rc;
     }
-    const Ptr ptrs[] = {{"x", x}, {"y", y}, {"cu_seqlens", cu_seqlens}, {"positions", positions}, {"status", status}};
-    if (int rc = check_device("rope", ptrs)) return rc;
+    const Ptr ptrs[] = {{"x", x, (unsigned)e}, {"y", y, (unsigned)e}, {"cu_seqlens", cu_seqlens}, {"positions", positions}, {"status", status}};
+    if (int rc = check_pointers("rope", ptrs)) return rc;
     const bool vec = !(((uintptr_t)x | (uintptr_t)y | (uint64_t)(x_stride * e) | (uint64_t)(y_stride * e)) & 15);
     const cudaError_t err = launch_rope(*plan, x, x_stride, y, y_stride, (int)n_tokens, (int)heads, cu_seqlens,
                                         (int)n_seqs, positions, inverse != 0, elem_dtype, vec, status,
@@ -248,8 +251,8 @@ int laya_gpu_attention(const laya_attention* a, const void* q, int64_t q_stride,
                       {"lse", lse, (int64_t)T * 4, (int64_t)T * 4, hq, true}};
     if (int rc = check_overlap(op, s)) return rc;
     const Ptr ptrs[] = {{"q", q}, {"k", k}, {"v", v}, {"out", out}, {"lse", lse}, {"cu_seqlens", a->cu_seqlens},
-                        {"token_mask", a->token_mask}, {"status", a->status}};
-    if (int rc = check_device(op, ptrs)) return rc;
+                        {"token_mask", a->token_mask, 1}, {"status", a->status}};
+    if (int rc = check_pointers(op, ptrs)) return rc;
     AttnIO io{};
     io.q = {const_cast<void*>(q), q_stride};
     io.k = {const_cast<void*>(k), k_stride};
@@ -293,8 +296,8 @@ int laya_gpu_attention_backward(const laya_attention* a, const void* q, int64_t 
     if (int rc = check_overlap(op, s)) return rc;
     const Ptr ptrs[] = {{"q", q}, {"k", k}, {"v", v}, {"out", out}, {"lse", lse}, {"dout", dout}, {"dq", dq},
                         {"dk", dk}, {"dv", dv}, {"workspace", workspace}, {"cu_seqlens", a->cu_seqlens},
-                        {"token_mask", a->token_mask}, {"status", a->status}};
-    if (int rc = check_device(op, ptrs)) return rc;
+                        {"token_mask", a->token_mask, 1}, {"status", a->status}};
+    if (int rc = check_pointers(op, ptrs)) return rc;
     AttnIO io{};
     io.q = {const_cast<void*>(q), q_stride};
     io.k = {const_cast<void*>(k), k_stride};
@@ -330,8 +333,6 @@ int laya_gpu_policy_loss(const laya_policy* p, const void* logits, const void* r
     if (!p->cu_options || !p->status || !actions || !advantages || !old_logp || (p->n_options && !logits))
         return fail(LAYA_ERR_ARG, "%s: NULL input or status", op);
     const int e = elem_size(p->elem_dtype);
-    if (((uintptr_t)logits | (uintptr_t)ref_logits | (uintptr_t)dlogits) % e)
-        return fail(LAYA_ERR_ARG, "%s: logits, ref_logits or dlogits is not aligned to its elements", op);
     const int64_t G = (int64_t)p->n_options * e, n = (int64_t)p->n_decisions * 4;
     const Span s[] = {{"logits", logits, G, G, G != 0, false}, {"ref_logits", ref_logits, G, G, G != 0, false},
                       {"actions", actions, n, n, 1, false},    {"advantages", advantages, n, n, 1, false},
@@ -340,11 +341,12 @@ int laya_gpu_policy_loss(const laya_policy* p, const void* logits, const void* r
                       {"kl", kl, n, n, 1, true},               {"entropy", entropy, n, n, 1, true},
                       {"dlogits", dlogits, G, G, G != 0, true}};
     if (int rc = check_overlap(op, s)) return rc;
-    const Ptr ptrs[] = {{"logits", logits}, {"ref_logits", ref_logits}, {"actions", actions},
+    const unsigned el = (unsigned)e;
+    const Ptr ptrs[] = {{"logits", logits, el}, {"ref_logits", ref_logits, el}, {"actions", actions},
                         {"advantages", advantages}, {"old_logp", old_logp}, {"grad", grad}, {"loss", loss},
-                        {"logp", logp}, {"kl", kl}, {"entropy", entropy}, {"dlogits", dlogits},
+                        {"logp", logp}, {"kl", kl}, {"entropy", entropy}, {"dlogits", dlogits, el},
                         {"cu_options", p->cu_options}, {"qtypes", p->qtypes}, {"status", p->status}};
-    if (int rc = check_device(op, ptrs)) return rc;
+    if (int rc = check_pointers(op, ptrs)) return rc;
     const PolicyIO io{logits, ref_logits, actions, advantages, old_logp, grad, loss, logp, kl, entropy, dlogits};
     const cudaError_t err = launch_policy(*p, io, static_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? LAYA_OK : cuda_fail(op, err);

@@ -329,7 +329,7 @@ cudaError_t launch_policy(const laya_policy& p, const PolicyIO& io, cudaStream_t
     s.qtypes = p.qtypes;
     s.n = (int)p.n_decisions;
     s.G = (int)p.n_options;
-    s.max_k = (int)p.max_options;
+    s.max_k = (int)(p.max_options < p.n_options ? p.max_options : p.n_options);
     for (int i = 0; i < 3; i++) {
         s.inv_t[i] = 1.f / fmaxf(1e-3f, p.temperature[i]);
         s.scale[i] = (float)(1.4426950408889634 / fmaxf(1e-3f, p.temperature[i]));

@@ -45,7 +45,8 @@ def _code(f, *a, **kw):
 
 @pytest.mark.parametrize("kw", [dict(n_heads=0), dict(n_kv_heads=0), dict(n_heads=12, n_kv_heads=5),
                                 dict(n_heads=70000, n_kv_heads=1), dict(scale=0.0), dict(scale=-1.0),
-                                dict(scale=math.inf), dict(scale=math.nan), dict(n_tokens=(1 << 30) + 1),
+                                dict(scale=math.inf), dict(scale=math.nan), dict(scale=3e38),
+                                dict(cu_seqlens_ptr=A + 2), dict(status_ptr=A + 1), dict(n_tokens=(1 << 30) + 1),
                                 dict(cu_seqlens_ptr=0), dict(status_ptr=0)])
 def test_attention_refuses_shapes(kw):
     assert _code(_fwd, _shape(**kw)) == gpu.ERR_ARG
@@ -60,7 +61,7 @@ def test_attention_refuses_f32():
 @pytest.mark.parametrize("kw", [dict(q_ptr=0), dict(k_ptr=0), dict(v_ptr=0), dict(out_ptr=0), dict(q_ptr=A + 8),
                                 dict(q_stride=760), dict(k_stride=2300), dict(out_stride=769),
                                 dict(out_ptr=A), dict(out_ptr=A + 3072, out_stride=2304), dict(lse_ptr=A + 4096),
-                                dict(out_ptr=A + 3072 + 16, out_stride=2304)])
+                                dict(out_ptr=A + 3072 + 16, out_stride=2304), dict(lse_ptr=A + (1 << 25) + 2)])
 def test_attention_refuses_rows(kw):
     assert _code(_fwd, _shape(), **kw) == gpu.ERR_ARG
 
@@ -119,7 +120,8 @@ def test_rope_refuses(kw):
                                      ({}, dict(logits_ptr=0)), ({}, dict(actions_ptr=0)), ({}, dict(advantages_ptr=0)),
                                      ({}, dict(old_logp_ptr=0)), ({}, dict(dlogits_ptr=A)),
                                      ({}, dict(dlogits_ptr=A + 4)), ({}, dict(logits_ptr=A + 2)),
-                                     ({}, dict(loss_ptr=A + 8192)), ({}, dict(kl_ptr=A + (1 << 16)))])
+                                     ({}, dict(loss_ptr=A + 8192)), ({}, dict(actions_ptr=A + 8194)), ({}, dict(kl_ptr=A + (1 << 18) + 1)),
+                                     (dict(cu_options_ptr=A + 1), {}), (dict(qtypes_ptr=A + 2), {}), ({}, dict(kl_ptr=A + (1 << 16)))])
 def test_policy_refuses(kw, args):
     b = dict(cu_options_ptr=A, n_decisions=8, n_options=64, max_options=8, status_ptr=A)
     b.update(kw)
