@@ -839,9 +839,9 @@ __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const At
     if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the two kernels that follow
     const int n = a.n_seqs;
     const int first = max(a.cu[0], 0), last = min(a.cu[n], a.n_tokens);  // rows past either are not the call's
-    const long long at = ((long long)blockIdx.x * DELTA_THREADS + threadIdx.x) / 8;
+    const unsigned at = blockIdx.x * (DELTA_THREADS / 8) + threadIdx.x / 8;  // tokens times heads: below 2^32
     const int c = threadIdx.x & 7;
-    const int t = (int)(at / heads), h = (int)(at - (long long)t * heads);
+    const int t = (int)(at / (unsigned)heads), h = (int)(at - (unsigned)t * heads);
     const bool ok = t >= first && t < last && (!a.mask || a.mask[t] != 0);
     float sum = 0.f;
     if (ok) {
@@ -1217,8 +1217,7 @@ cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, cons
         !map_rows(&m.v, a.io.v, n_kv_heads, a, bf16) || !map_rows(&m.dout, a.io.dout, n_heads, a, bf16))
         return cudaErrorInvalidValue;
     const int sms = sm_count();
-    const long long threads = (long long)a.n_tokens * n_heads * 8;
-    const unsigned blocks = (unsigned)((threads + DELTA_THREADS - 1) / DELTA_THREADS);
+    const unsigned blocks = (unsigned)(((unsigned long long)a.n_tokens * n_heads * 8 + DELTA_THREADS - 1) / DELTA_THREADS);
     if (bf16)
         attention_delta_kernel<__nv_bfloat16><<<blocks, DELTA_THREADS, 0, stream>>>(a, n_heads);
     else

@@ -110,6 +110,8 @@ int check_attention(const char* op, const laya_attention* a) {
         return fail(LAYA_ERR_ARG, "%s: %u tokens, %u sequences (2^30 at most)", op, a->n_tokens, a->n_seqs);
     if (!a->n_heads || !a->n_kv_heads || a->n_heads % a->n_kv_heads || a->n_heads > 65535)
         return fail(LAYA_ERR_ARG, "%s: %u heads over %u key heads", op, a->n_heads, a->n_kv_heads);
+    if ((uint64_t)a->n_tokens * a->n_heads > 0xffff0000u)
+        return fail(LAYA_ERR_ARG, "%s: %u tokens of %u heads (2^32 in all)", op, a->n_tokens, a->n_heads);
     if (!(a->scale > 0.f) || !std::isfinite(2.f * a->scale))  // it is multiplied by log2 e
         return fail(LAYA_ERR_ARG, "%s: scale must be positive and finite", op);
     if (a->n_tokens && a->n_seqs && (!a->cu_seqlens || !a->status))

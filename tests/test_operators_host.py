@@ -46,7 +46,7 @@ def _code(f, *a, **kw):
 @pytest.mark.parametrize("kw", [dict(n_heads=0), dict(n_kv_heads=0), dict(n_heads=12, n_kv_heads=5),
                                 dict(n_heads=70000, n_kv_heads=1), dict(scale=0.0), dict(scale=-1.0),
                                 dict(scale=math.inf), dict(scale=math.nan), dict(scale=3e38),
-                                dict(cu_seqlens_ptr=A + 2), dict(status_ptr=A + 1), dict(n_tokens=(1 << 30) + 1),
+                                dict(cu_seqlens_ptr=A + 2), dict(status_ptr=A + 1), dict(n_tokens=(1 << 30) + 1), dict(n_tokens=1 << 30),
                                 dict(cu_seqlens_ptr=0), dict(status_ptr=0)])
 def test_attention_refuses_shapes(kw):
     assert _code(_fwd, _shape(**kw)) == gpu.ERR_ARG
