@@ -338,19 +338,14 @@ __device__ __forceinline__ bool next_item(const Frame& f, const AttnArgs& a, int
     return wait_one(&b->item_full[k & 1], (k >> 1) & 1, a.status, &b->abort) && f.slots->item[k & 1].n >= 0;
 }
 
-// The softmax warps' place in the ring and in the score buffers: both go on
-// from item to item.
+// The softmax warps' place in the score buffers and in the ring, from the
+// number of tiles they have gone through, of all items.
 struct Turn {
-    int stage = 0, buffer = 0;
-    uint32_t full = 0, own = 0;  // parities
-    __device__ __forceinline__ void next() {
-        own ^= buffer;
-        buffer ^= 1;
-        if (++stage == STAGES) {
-            stage = 0;
-            full ^= 1;
-        }
-    }
+    unsigned tile = 0;
+    __device__ __forceinline__ int buffer() const { return tile & 1; }
+    __device__ __forceinline__ uint32_t own() const { return (tile >> 1) & 1; }  // parity of the buffer's barriers
+    __device__ __forceinline__ int stage() const { return tile % STAGES; }
+    __device__ __forceinline__ uint32_t full() const { return (tile / STAGES) & 1; }
 };
 
 // ------------------------------------------------------------------ TMEM rows
@@ -568,8 +563,8 @@ __device__ __forceinline__ bool column_bits(const Frame& f, const AttnArgs& a, c
                                             uint32_t* bits) {
     *bits = ~0u;
     if (!a.mask && col0 + 32 <= len) return true;
-    if (!wait_all(&f.bar->full[turn.stage], turn.full, a, f.bar)) return false;
-    *bits = f.slots->bits[turn.stage][g];
+    if (!wait_all(&f.bar->full[turn.stage()], turn.full(), a, f.bar)) return false;
+    *bits = f.slots->bits[turn.stage()][g];
     return true;
 }
 
@@ -675,10 +670,10 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             const int n = it.n, row0 = it.row0, len = it.len;
             int col0 = it.t0 * STEP + g * 32;
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < n; j++, col0 += STEP, turn.next()) {
-                const uint32_t t_s = lanes + turn.buffer * 64 + g * 32;
+            for (int j = 0; j < n; j++, col0 += STEP, turn.tile++) {
+                const uint32_t t_s = lanes + turn.buffer() * 64 + g * 32;
                 uint32_t bits;
-                ok = wait_all(&bar->s_full[turn.buffer], turn.own, a, bar) &&
+                ok = wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar) &&
                      column_bits(f, a, turn, g, col0, len, &bits);
                 if (!ok) break;
                 tc_fence_after();
@@ -704,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 }
                 if (j > 0 && __any_sync(0xffffffffu, move)) {
                     // once P V of the tile before is complete, O is at rest
-                    ok = wait_all(&bar->done[turn.buffer ^ 1], turn.own ^ (turn.buffer ^ 1), a, bar);
+                    ok = wait_all(&bar->done[turn.buffer() ^ 1], ((turn.tile - 1) >> 1) & 1, a, bar);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
@@ -731,7 +726,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar->p_full[turn.buffer]);
+                mbar_arrive(&bar->p_full[turn.buffer()]);
             }
             // The groups' halves of the row are joined: each takes 32 columns
             // of both (the two threads of a row share its TMEM lane).
@@ -947,17 +942,17 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             const bool there = present(a, t, i);
             const float* stat = f.extra + (k & 1) * 2 * ROWS + r;
             const float e = stat[0], delta = stat[ROWS];
-            for (int j = 0; j < n; j++, col0 += STEP, turn.next()) {
-                const uint32_t t_s = lanes + turn.buffer * 64 + g * 32;
+            for (int j = 0; j < n; j++, col0 += STEP, turn.tile++) {
+                const uint32_t t_s = lanes + turn.buffer() * 64 + g * 32;
                 uint32_t bits;
-                ok = wait_all(&bar->s_full[turn.buffer], turn.own, a, bar) &&
+                ok = wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar) &&
                      column_bits(f, a, turn, g, col0, t.len, &bits);
                 if (!ok) break;
                 tc_fence_after();
                 float v[32];
                 load32(t_s, v);
                 tc_fence_before();
-                mbar_arrive(&bar->s_read[turn.buffer]);
+                mbar_arrive(&bar->s_read[turn.buffer()]);
                 if (bits != ~0u || edge(a.window, i - r, ROWS, col0, 32)) mask_row(v, bits, a.window, i, col0);
 #pragma unroll
                 for (int x = 0; x < 32; x += 2) {
@@ -965,7 +960,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                     v[x] = ex2_approx(y.x);
                     v[x + 1] = ex2_approx(y.y);
                 }
-                ok = wait_all(&bar->dp_full[turn.buffer], turn.own, a, bar);
+                ok = wait_all(&bar->dp_full[turn.buffer()], turn.own(), a, bar);
                 if (!ok) break;
                 tc_fence_after();
                 float d[32];
@@ -984,7 +979,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 }
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar->p_full[turn.buffer]);
+                mbar_arrive(&bar->p_full[turn.buffer()]);
             }
             if (ok) ok = wait_all(&bar->acc_full[k & 1], (k >> 1) & 1, a, bar);
             if (!ok) break;
@@ -1089,21 +1084,21 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
             const Item& it = f.slots->item[k & 1];
             const int n = it.n, i = it.row0 + r;  // key
-            for (int j = 0; j < n; j++, turn.next()) {
-                const uint32_t t_s = lanes + turn.buffer * 64 + g * 32;
-                ok = wait_all(&bar->full[turn.stage], turn.full, a, bar) &&
-                     wait_all(&bar->s_full[turn.buffer], turn.own, a, bar);
+            for (int j = 0; j < n; j++, turn.tile++) {
+                const uint32_t t_s = lanes + turn.buffer() * 64 + g * 32;
+                ok = wait_all(&bar->full[turn.stage()], turn.full(), a, bar) &&
+                     wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar);
                 if (!ok) break;
                 tc_fence_after();
                 float v[32];
                 load32(t_s, v);
                 tc_fence_before();
-                mbar_arrive(&bar->s_read[turn.buffer]);
+                mbar_arrive(&bar->s_read[turn.buffer()]);
                 if (a.window >= 0) {
                     const int col0 = (it.t0 + j % (n / a.group)) * STEP + g * 32;
                     if (edge(a.window, col0, 32, i - r, ROWS)) mask_row(v, ~0u, a.window, i, col0);
                 }
-                const float4* lse = reinterpret_cast<const float4*>(f.extra + turn.stage * 2 * STEP + g * 32);
+                const float4* lse = reinterpret_cast<const float4*>(f.extra + turn.stage() * 2 * STEP + g * 32);
                 const float4* delta = lse + STEP / 4;
 #pragma unroll
                 for (int x = 0; x < 8; x++) {
@@ -1116,7 +1111,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                     v[4 * x + 2] = ex2_approx(z.x);
                     v[4 * x + 3] = ex2_approx(z.y);
                 }
-                ok = wait_all(&bar->dp_full[turn.buffer], turn.own, a, bar);
+                ok = wait_all(&bar->dp_full[turn.buffer()], turn.own(), a, bar);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
@@ -1143,7 +1138,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 }
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar->p_full[turn.buffer]);
+                mbar_arrive(&bar->p_full[turn.buffer()]);
             }
             if (ok) ok = wait_all(&bar->acc_full[0], k & 1, a, bar);
             if (!ok) break;
