@@ -345,7 +345,6 @@ struct Turn {
     __device__ __forceinline__ int buffer() const { return tile & 1; }
     __device__ __forceinline__ uint32_t own() const { return (tile >> 1) & 1; }  // parity of the buffer's barriers
     __device__ __forceinline__ int stage() const { return tile % STAGES; }
-    __device__ __forceinline__ uint32_t full() const { return (tile / STAGES) & 1; }
 };
 
 // ------------------------------------------------------------------ TMEM rows
@@ -469,31 +468,6 @@ __device__ __forceinline__ void mma_sum(uint32_t d, uint32_t p, int step, uint32
         tc_mma_f16_ts(d, p + step * ks, sw128_desc(b + ks * 2048), IDESC<T> | B_MN, accumulate || ks != 0);
 }
 
-// The MMA lane takes whatever is ready next, S, dP or a sum, each kind in the
-// order of the tiles (so an accumulator's order does not depend on timing).
-struct Poll {
-    Bars* bar;
-    int* err;
-    unsigned idle = 0;  // polls since something was ready
-    unsigned long long t0 = 0;
-
-    // False once nothing has been ready for WAIT_LIMIT_NS, or a warp gave up.
-    __device__ __forceinline__ bool go_on(bool moved) {
-        if (moved) {
-            idle = 0;
-            return true;
-        }
-        if ((++idle & 255) != 0) return true;
-        if (*(volatile int*)&bar->abort) return false;
-        const unsigned long long now = globaltimer();
-        if (idle == 256) t0 = now;
-        if (now - t0 <= WAIT_LIMIT_NS) return true;
-        atomicOr(err, ERR_WAIT_TIMEOUT);
-        *(volatile int*)&bar->abort = 1;
-        return false;
-    }
-};
-
 // ------------------------------------------------------------------ CTA frame
 
 template <typename C>
@@ -518,7 +492,7 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
         for (int s = 0; s < 2; s++) {
             mbar_init(&b->item_full[s], 32);
             mbar_init(&b->item_empty[s], SOFTMAX + 1);
-            mbar_init(&b->s_full[s], 1);
+            mbar_init(&b->s_full[s], 2);  // the product, and the MMA lane on what the stage holds besides
             mbar_init(&b->dp_full[s], 1);
             mbar_init(&b->s_read[s], SOFTMAX);
             mbar_init(&b->p_full[s], SOFTMAX);
@@ -551,21 +525,20 @@ __device__ __forceinline__ void close_frame(const Frame& f, int warp) {
     if (warp == MMA) tmem_dealloc(f.tmem, COLS);
 }
 
+// The MMA lane's waits.
+struct Waits {
+    int* err;
+    int* abort;
+    __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+        const bool ok = wait_one(bar, parity, err, abort);
+        tc_fence_after();
+        return ok;
+    }
+};
+
 // Warp-wide wait of the softmax warps.
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, const AttnArgs& a, Bars* b) {
     return __all_sync(0xffffffffu, wait_one(bar, parity, a.status, &b->abort));
-}
-
-// Presence bits of group g's 32 columns, col0 and on, of the present tile; the
-// ring is only asked about a tile that may lack some (its barrier is complete:
-// the tile's scores have been computed).
-__device__ __forceinline__ bool column_bits(const Frame& f, const AttnArgs& a, const Turn& turn, int g, int col0, int len,
-                                            uint32_t* bits) {
-    *bits = ~0u;
-    if (!a.mask && col0 + 32 <= len) return true;
-    if (!wait_all(&f.bar->full[turn.stage()], turn.full(), a, f.bar)) return false;
-    *bits = f.slots->bits[turn.stage()][g];
-    return true;
 }
 
 // ------------------------------------------------------------------ forward
@@ -619,39 +592,40 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     } else if (warp == MMA) {
         if (elect_one()) {
             const uint32_t q = smem_u32(f.big), kv = smem_u32(f.ring);
-            Poll poll{bar, a.status};
+            const Waits wait{a.status, &bar->abort};
             int c = 0;  // tiles of the items before
+            auto scores = [&](int j) {
+                if (!wait(&bar->full[j % STAGES], (j / STAGES) & 1) || (j > 1 && !wait(&bar->done[j & 1], ((j >> 1) - 1) & 1)))
+                    return false;
+                mma_rows<T>(f.tmem + (j & 1) * 64, q, kv + 2 * (j % STAGES) * SMALL);
+                tc_commit(&bar->s_full[j & 1]);
+                mbar_arrive(&bar->s_full[j & 1]);
+                return true;
+            };
+            // S runs two tiles ahead of P V: of the tile before P V's buffer is free
             for (int k = 0; next_item(f, a, k); k++) {
-                const int end = c + f.slots->item[k & 1].n;
+                const int n = f.slots->item[k & 1].n;
                 mbar_arrive(&bar->item_empty[k & 1]);
-                int sc = c, pv = c;  // the next tile of each product
-                bool big = false, moved = true;
-                while (pv < end && poll.go_on(moved)) {
-                    moved = false;
-                    if (!big) big = moved = ready(&bar->big_full, k & 1);
-                    if (big && sc < end && sc < pv + 2 && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
-                        (sc < 2 || ready(&bar->done[sc & 1], ((sc >> 1) - 1) & 1))) {
-                        tc_fence_after();
-                        mma_rows<T>(f.tmem + (sc & 1) * 64, q, kv + 2 * (sc % STAGES) * SMALL);
-                        tc_commit(&bar->s_full[sc & 1]);
-                        if (++sc == end) tc_commit(&bar->big_empty);
-                        moved = true;
-                    }
-                    if (pv < sc && ready(&bar->p_full[pv & 1], (pv >> 1) & 1) &&
-                        (k == 0 || pv > c || ready(&bar->acc_free[0], (k - 1) & 1))) {
-                        const int s = pv % STAGES;
-                        const uint32_t p = f.tmem + (pv & 1) * 64, v = kv + (2 * s + 1) * SMALL;
-                        tc_fence_after();
-                        mma_sum<T, 2>(f.tmem + 128, p, 8, v, pv > c);
-                        mma_sum<T, 2>(f.tmem + 192, p + 32, 8, v + 2 * 2048, pv > c);
-                        tc_commit(&bar->empty[s]);
-                        tc_commit(&bar->done[pv & 1]);
-                        if (++pv == end) tc_commit(&bar->acc_full[0]);
-                        moved = true;
+                if (!wait(&bar->big_full, k & 1) || !scores(c) || (n > 1 && !scores(c + 1))) break;
+                if (n <= 2) tc_commit(&bar->big_empty);
+                int i = 0;
+                for (; i < n; i++) {
+                    const int j = c + i, s = j % STAGES;
+                    const uint32_t p = f.tmem + (j & 1) * 64, v = kv + (2 * s + 1) * SMALL;
+                    if (!wait(&bar->p_full[j & 1], (j >> 1) & 1)) break;
+                    if (i == 0 && k > 0 && !wait(&bar->acc_free[0], (k - 1) & 1)) break;
+                    mma_sum<T, 2>(f.tmem + 128, p, 8, v, i > 0);
+                    mma_sum<T, 2>(f.tmem + 192, p + 32, 8, v + 2 * 2048, i > 0);
+                    tc_commit(&bar->empty[s]);
+                    tc_commit(&bar->done[j & 1]);
+                    if (i + 2 < n) {
+                        if (!scores(j + 2)) break;
+                        if (i + 3 == n) tc_commit(&bar->big_empty);
                     }
                 }
-                if (pv < end) break;
-                c = end;
+                if (i < n) break;
+                tc_commit(&bar->acc_full[0]);
+                c += n;
             }
             tc_commit(&bar->drained);
             drain(&bar->drained, 0, a.status);
@@ -667,18 +641,17 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         for (int k = 0; ok; k++) {
             if (!__all_sync(0xffffffffu, next_item(f, a, k))) break;
             const Item& it = f.slots->item[k & 1];
-            const int n = it.n, row0 = it.row0, len = it.len;
+            const int n = it.n, row0 = it.row0;
             int col0 = it.t0 * STEP + g * 32;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < n; j++, col0 += STEP, turn.tile++) {
                 const uint32_t t_s = lanes + turn.buffer() * 64 + g * 32;
-                uint32_t bits;
-                ok = wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar) &&
-                     column_bits(f, a, turn, g, col0, len, &bits);
+                ok = wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar);
                 if (!ok) break;
                 tc_fence_after();
                 float v[32];
                 load32(t_s, v);
+                const uint32_t bits = f.slots->bits[turn.stage()][g];
                 if (bits != ~0u || edge(a.window, row0, ROWS, col0, 32)) mask_row(v, bits, a.window, row0 + r, col0);
                 float mx[4];
 #pragma unroll
@@ -777,46 +750,47 @@ template <typename T, int ACCS, typename Sum>
 __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a, Sum sums) {
     Bars* bar = f.bar;
     const uint32_t big0 = smem_u32(f.big), big1 = big0 + BIG, ring = smem_u32(f.ring);
-    Poll poll{bar, a.status};
+    const Waits wait{a.status, &bar->abort};
     int c = 0;  // tiles of the items before
+    auto scores = [&](int j) {
+        if (!wait(&bar->full[j % STAGES], (j / STAGES) & 1) || (j > 1 && !wait(&bar->done[j & 1], ((j >> 1) - 1) & 1)))
+            return false;
+        mma_rows<T>(f.tmem + (j & 1) * 64, big0, ring + 2 * (j % STAGES) * SMALL);
+        tc_commit(&bar->s_full[j & 1]);
+        mbar_arrive(&bar->s_full[j & 1]);
+        return true;
+    };
+    auto dp = [&](int j) {
+        if (!wait(&bar->s_read[j & 1], (j >> 1) & 1)) return false;
+        mma_rows<T>(f.tmem + (j & 1) * 64, big1, ring + (2 * (j % STAGES) + 1) * SMALL);
+        tc_commit(&bar->dp_full[j & 1]);
+        return true;
+    };
+    // In the order in which the softmax warps come to them: the sums of a
+    // tile, the next one's dP (its scores are read right after), the scores of
+    // the tile after that. An accumulator gets its tiles in their order.
     for (int k = 0; next_item(f, a, k); k++) {
-        const int end = c + f.slots->item[k & 1].n, acc = k % ACCS;
+        const int n = f.slots->item[k & 1].n, acc = k % ACCS;
         mbar_arrive(&bar->item_empty[k & 1]);
-        int sc = c, dp = c, sum = c;  // the next tile of each product
-        bool big = false, moved = true;
-        while (sum < end && poll.go_on(moved)) {
-            moved = false;
-            if (!big) big = moved = ready(&bar->big_full, k & 1);
-            if (dp < sc && ready(&bar->s_read[dp & 1], (dp >> 1) & 1)) {
-                tc_fence_after();
-                mma_rows<T>(f.tmem + (dp & 1) * 64, big1, ring + (2 * (dp % STAGES) + 1) * SMALL);
-                tc_commit(&bar->dp_full[dp & 1]);
-                if (++dp == end) tc_commit(&bar->big_empty);
-                moved = true;
+        if (!wait(&bar->big_full, k & 1) || !scores(c) || (n > 1 && !scores(c + 1)) || !dp(c)) break;
+        if (n == 1) tc_commit(&bar->big_empty);
+        int i = 0;
+        for (; i < n; i++) {
+            const int j = c + i;
+            if (!wait(&bar->p_full[j & 1], (j >> 1) & 1)) break;
+            if (i == 0 && k >= ACCS && !wait(&bar->acc_free[acc], (k / ACCS - 1) & 1)) break;
+            sums(f.tmem + (j & 1) * 64, ring + 2 * (j % STAGES) * SMALL, acc, i > 0);
+            tc_commit(&bar->empty[j % STAGES]);
+            tc_commit(&bar->done[j & 1]);
+            if (i + 1 < n) {
+                if (!dp(j + 1)) break;
+                if (i + 2 == n) tc_commit(&bar->big_empty);
             }
-            // The next tile's dP goes first: the softmax warps come to it right
-            // after this tile, and its sum can wait.
-            if ((sum + 1 < dp || (sum < dp && dp == end)) && ready(&bar->p_full[sum & 1], (sum >> 1) & 1) &&
-                (k < ACCS || sum > c || ready(&bar->acc_free[acc], (k / ACCS - 1) & 1))) {
-                const int s = sum % STAGES;
-                tc_fence_after();
-                sums(f.tmem + (sum & 1) * 64, ring + 2 * s * SMALL, acc, sum > c);
-                tc_commit(&bar->empty[s]);
-                tc_commit(&bar->done[sum & 1]);
-                if (++sum == end) tc_commit(&bar->acc_full[acc]);
-                moved = true;
-            }
-            if (big && sc < end && sc < sum + 2 && ready(&bar->full[sc % STAGES], (sc / STAGES) & 1) &&
-                (sc < 2 || ready(&bar->done[sc & 1], ((sc >> 1) - 1) & 1))) {
-                tc_fence_after();
-                mma_rows<T>(f.tmem + (sc & 1) * 64, big0, ring + 2 * (sc % STAGES) * SMALL);
-                tc_commit(&bar->s_full[sc & 1]);
-                sc++;
-                moved = true;
-            }
+            if (i + 2 < n && !scores(j + 2)) break;
         }
-        if (sum < end) break;
-        c = end;
+        if (i < n) break;
+        tc_commit(&bar->acc_full[acc]);
+        c += n;
     }
     tc_commit(&bar->drained);
     drain(&bar->drained, 0, a.status);
@@ -944,15 +918,14 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             const float e = stat[0], delta = stat[ROWS];
             for (int j = 0; j < n; j++, col0 += STEP, turn.tile++) {
                 const uint32_t t_s = lanes + turn.buffer() * 64 + g * 32;
-                uint32_t bits;
-                ok = wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar) &&
-                     column_bits(f, a, turn, g, col0, t.len, &bits);
+                ok = wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar);
                 if (!ok) break;
                 tc_fence_after();
                 float v[32];
                 load32(t_s, v);
                 tc_fence_before();
                 mbar_arrive(&bar->s_read[turn.buffer()]);
+                const uint32_t bits = f.slots->bits[turn.stage()][g];
                 if (bits != ~0u || edge(a.window, i - r, ROWS, col0, 32)) mask_row(v, bits, a.window, i, col0);
 #pragma unroll
                 for (int x = 0; x < 32; x += 2) {
@@ -1086,8 +1059,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             const int n = it.n, i = it.row0 + r;  // key
             for (int j = 0; j < n; j++, turn.tile++) {
                 const uint32_t t_s = lanes + turn.buffer() * 64 + g * 32;
-                ok = wait_all(&bar->full[turn.stage()], turn.full(), a, bar) &&
-                     wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar);
+                ok = wait_all(&bar->s_full[turn.buffer()], turn.own(), a, bar);
                 if (!ok) break;
                 tc_fence_after();
                 float v[32];
