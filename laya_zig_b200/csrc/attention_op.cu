@@ -8,12 +8,20 @@
 //   delta_i = sum_d dO_id O_id            (= sum_j P_ij dP_ij)
 //   dP = dO V^T,  dS = P (dP - delta)
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
-// Two kernels, without atomics: one block per query tile walks the keys for
-// dQ (and leaves delta for the other), one per key tile walks the queries of
-// every head of its group for dK and dV. S and dP are computed in both, seven
-// products instead of five, which is what fixed summation order costs here.
+// One launch, without atomics: a block per query tile walks the keys for dQ, a
+// block per key tile walks the queries of every head of its group for dK and
+// dV. S, dP and delta are computed in both, seven products instead of five,
+// which is what a fixed order of the sums costs here.
 // P and dS are rounded to 16 bits as operands of the products that follow;
 // statistics, sums and accumulators are f32.
+//
+// These kernels serve calls that a few waves of blocks finish, where what
+// counts is the chain of dependent steps in one block (find the sequence, load,
+// two to five products of 16 x 8 x 16 instructions, exponentials, store), not
+// a rate. One sequence of 64 tokens, 12 heads, bf16: forward 4.1 us, backward
+// 5.1 us (a short kernel on its own takes 2.1 there). Backward in one launch
+// instead of a dQ launch followed by a dK/dV launch that reads its delta: 9.3
+// -> 5.1 us there; delta is recomputed from O, which a row's tile costs little.
 //
 // Rows outside their sequence and absent tokens are filled with zeros on
 // their way into shared memory (cp.async with a source size of 0), so nothing
@@ -261,60 +269,50 @@ __global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const AttnArg
     }
 }
 
-// ------------------------------------------------------------------ dQ (and delta)
-constexpr int DQ_SMEM = 6 * TILE * 2;
+// ------------------------------------------------------------------ backward
+
+// delta of 64 rows from their tiles of O and dO: two threads to a row.
+template <typename T>
+__device__ __forceinline__ void tile_delta(float* sdelta, const T* so, const T* sdo) {
+    const int r = threadIdx.x >> 1, c0 = (threadIdx.x & 1) * 32;
+    float acc = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint4 o = *reinterpret_cast<const uint4*>(so + swz(r, c0 + 8 * c));
+        const uint4 d = *reinterpret_cast<const uint4*>(sdo + swz(r, c0 + 8 * c));
+        const T* x = reinterpret_cast<const T*>(&o);
+        const T* y = reinterpret_cast<const T*>(&d);
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc = fmaf(to_float(x[e]), to_float(y[e]), acc);
+    }
+    acc += __shfl_xor_sync(0xffffffffu, acc, 1);
+    if ((threadIdx.x & 1) == 0) sdelta[r] = acc;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const AttnArgs a) {
-    extern __shared__ __align__(128) uint8_t smem[];
+__device__ __forceinline__ void dq_block(const AttnArgs& a, const SeqTile& t, int h, uint8_t* smem) {
     T* sq = reinterpret_cast<T*>(smem);
     T* sdo = sq + TILE;
     T* sk = sdo + TILE;
     T* sv = sk + 2 * TILE;
+    T* so = sv + 2 * TILE;
+    float* sdelta = reinterpret_cast<float*>(so + TILE);
     __shared__ uint32_t bits[2][2];
-    __shared__ float sdelta[TB];
-    griddep_launch();
-    SeqTile t;
-    if (!block_tile(a, &t)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.y, hk = h / a.group;
+    const int hk = h / a.group;
     int kt0, kt1;
     visible_tiles(a, t, TB, TB, &kt0, &kt1);
     load_tile(sq, a.io.q, h, a, t, t.row0);
     load_tile(sdo, a.io.dout, h, a, t, t.row0);
+    load_tile(so, a.io.out, h, a, t, t.row0);
     load_tile(sk, a.io.k, hk, a, t, kt0 * TB);
     load_tile(sv, a.io.v, hk, a, t, kt0 * TB);
     key_bits(bits[0], a, t, kt0 * TB);
     copy_commit();
-    {  // delta: two threads to a row, 32 elements each
-        const int r = threadIdx.x >> 1, i = t.row0 + r, c0 = (threadIdx.x & 1) * 32;
-        const bool ok = present(a, t, i);
-        float acc = 0.f;
-        uint4 ov[4];
-        if (ok) {
-            const T* g = static_cast<const T*>(a.io.out.p) + (t.start + i) * a.io.out.ld + h * 64 + c0;
-#pragma unroll
-            for (int c = 0; c < 4; c++) ov[c] = *reinterpret_cast<const uint4*>(g + 8 * c);
-        }
-        copy_wait<0>();
-        __syncthreads();
-        if (ok) {
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const T* x = reinterpret_cast<const T*>(&ov[c]);
-                const uint4 dv = *reinterpret_cast<const uint4*>(sdo + swz(r, c0 + 8 * c));
-                const T* y = reinterpret_cast<const T*>(&dv);
-#pragma unroll
-                for (int e = 0; e < 8; e++) acc = fmaf(to_float(x[e]), to_float(y[e]), acc);
-            }
-        }
-        acc += __shfl_xor_sync(0xffffffffu, acc, 1);
-        if ((threadIdx.x & 1) == 0) {
-            sdelta[r] = acc;
-            if (i < t.len) a.io.delta[(long long)h * a.n_tokens + t.start + i] = acc;
-        }
-        __syncthreads();
-    }
+    copy_wait<0>();
+    __syncthreads();
+    tile_delta(sdelta, so, sdo);
+    __syncthreads();
     const float sl2 = a.scale * LOG2E;
     const int i0 = t.row0 + warp * 16 + (lane >> 2), i1 = i0 + 8;
     const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
@@ -367,23 +365,16 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_kernel(const AttnArgs
     store_rows<T>(a.io.dq, h, t, t.row0 + warp * 16, lane, dq, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
 }
 
-// ------------------------------------------------------------------ dK, dV
-constexpr int DKV_SMEM = 6 * TILE * 2 + 2 * 2 * TB * 4;
-
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const AttnArgs a) {
-    extern __shared__ __align__(128) uint8_t smem[];
+__device__ __forceinline__ void dkv_block(const AttnArgs& a, const SeqTile& t, int hk, uint8_t* smem) {
     T* sk = reinterpret_cast<T*>(smem);
     T* sv = sk + TILE;
     T* sq = sv + TILE;
     T* sdo = sq + 2 * TILE;
-    float* slse = reinterpret_cast<float*>(sdo + 2 * TILE);  // [2][64]
-    float* sdelta = slse + 2 * TB;
-    griddep_wait();  // delta comes from the kernel before, which this one's launch overlaps
-    SeqTile t;
-    if (!block_tile(a, &t)) return;
+    T* so = sdo + 2 * TILE;
+    float* sdelta = reinterpret_cast<float*>(so + 2 * TILE);
+    float* slse = sdelta + TB;  // [2][64]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int hk = blockIdx.y;
     int qt0, qt1;
     visible_tiles(a, t, TB, TB, &qt0, &qt1);
     const int nqt = qt1 - qt0, total = nqt * a.group;
@@ -391,10 +382,13 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const AttnArg
         const int h = hk * a.group + it / nqt, row0 = (qt0 + it % nqt) * TB;
         load_tile(sq + b * TILE, a.io.q, h, a, t, row0);
         load_tile(sdo + b * TILE, a.io.dout, h, a, t, row0);
-        const int r = threadIdx.x & 63;
-        const bool ok = present(a, t, row0 + r);
-        const long long at = (long long)h * a.n_tokens + t.start + (ok ? row0 + r : 0);
-        copy4((threadIdx.x < 64 ? slse : sdelta) + b * TB + r, (threadIdx.x < 64 ? a.io.lse : a.io.delta) + at, ok);
+        load_tile(so + b * TILE, a.io.out, h, a, t, row0);
+        if (threadIdx.x < TB) {
+            const int r = threadIdx.x;
+            const bool ok = present(a, t, row0 + r);
+            const long long at = (long long)h * a.n_tokens + t.start + (ok ? row0 + r : 0);
+            copy4(slse + b * TB + r, a.io.lse + at, ok);
+        }
     };
     load_tile(sk, a.io.k, hk, a, t, t.row0);
     load_tile(sv, a.io.v, hk, a, t, t.row0);
@@ -416,6 +410,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const AttnArg
             load_a(ka, sk, warp, lane);
             load_a(va, sv, warp, lane);
         }
+        tile_delta(sdelta, so + b * TILE, sdo + b * TILE);  // read behind the barrier below
         const int row0 = (qt0 + it % nqt) * TB;
         // transposed: rows are keys, columns queries
         float s[8][4], dp[8][4];
@@ -441,9 +436,10 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const AttnArg
         }
         mma_nn<T>(dv, s, sdo + b * TILE, lane);
         mma_nt<T>(dp, va, sdo + b * TILE, lane);
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float2 d = *reinterpret_cast<const float2*>(sdelta + b * TB + 8 * j + c0);
+            const float2 d = *reinterpret_cast<const float2*>(sdelta + 8 * j + c0);
             s[j][0] *= dp[j][0] - d.x;
             s[j][1] *= dp[j][1] - d.y;
             s[j][2] *= dp[j][2] - d.x;
@@ -455,6 +451,20 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dkv_kernel(const AttnArg
     const bool p0 = present(a, t, j0), p1 = present(a, t, j1);
     store_rows<T>(a.io.dk, hk, t, t.row0 + warp * 16, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
     store_rows<T>(a.io.dv, hk, t, t.row0 + warp * 16, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
+}
+
+constexpr int BWD_SMEM = 8 * TILE * 2 + 3 * TB * 4;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 2) attention_bwd_kernel(const AttnArgs a, int n_heads) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    SeqTile t;
+    if (!block_tile(a, &t)) return;
+    const int y = blockIdx.y;
+    if (y < n_heads)
+        dq_block<T>(a, t, y, smem);
+    else
+        dkv_block<T>(a, t, y - n_heads, smem);
 }
 
 AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
@@ -472,45 +482,39 @@ AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
     return g;
 }
 
-cudaError_t launch(void (*kernel)(AttnArgs), unsigned heads, int smem, const AttnArgs& g, bool dependent,
-                   cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), heads);
-    if (dependent) return launch_k(kernel, grid, THREADS, smem, stream, g);
-    kernel<<<grid, THREADS, smem, stream>>>(g);
-    return cudaGetLastError();
-}
-
 }  // namespace
 
-// Which kernels a call gets: 64-row mma.sync blocks while they all fit the GPU
-// at once and their sequences are short, tcgen05 otherwise. Forward and
-// backward, 12 heads, us by mma.sync / tcgen05: 1 x 64 tokens 13.8 / 20.7, 1 x
-// 256 25.5 / 28.9, 64 x 16 39.8 / 44.6; 1 x 512 40.7 / 38.5, 64 x 64 45.9 /
-// 48.3, 64 x 100 101 / 68, 512 x 64 331 / 250.
+// Which kernels a call gets: 64-row mma.sync blocks for a little work (rows of
+// all heads times keys, at most 2^20 x 3, in sequences of 512 at most), tcgen05
+// otherwise. Forward and backward of bf16, 12 heads, us by mma.sync / tcgen05:
+// 1 x 64 tokens 9.1 / 19.7, 1 x 256 18.1 / 27.0, 64 x 16 38.1 / 41.8, 16 x 128
+// 31.3 / 35.9; at the limit 1 x 512 36.3 / 36.1, 64 x 64 43.4 / 44.5; beyond it
+// 8 x 256 47.1 / 34.2, 64 x 100 99.8 / 66.1, 512 x 32 295 / 230. (A short
+// sequence takes a whole tile in both.)
 static bool small_call(const laya_attention& a) {
-    return a.max_len <= 256 && (uint64_t)a.n_tokens * a.n_heads <= 32768;
+    return a.max_len <= 512 && a.n_heads <= 1024 && (uint64_t)a.n_tokens * a.n_heads * a.max_len <= 3u << 20;
 }
 
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
     const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
     const AttnArgs g = make_args(a, io);
     if (!small_call(a)) return launch_attention_fwd_tc(bf16, (int)a.n_heads, g, stream);
-    return launch(bf16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>, a.n_heads, FWD_SMEM, g, false,
-                  stream);
+    auto kernel = bf16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>;
+    const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), a.n_heads);
+    kernel<<<grid, THREADS, FWD_SMEM, stream>>>(g);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
     const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
     const AttnArgs g = make_args(a, io);
     if (!small_call(a)) return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
-    cudaError_t e = launch(bf16 ? attention_dq_kernel<__nv_bfloat16> : attention_dq_kernel<__half>, a.n_heads, DQ_SMEM, g,
-                           false, stream);
-    if (e == cudaSuccess)
-        e = launch(bf16 ? attention_dkv_kernel<__nv_bfloat16> : attention_dkv_kernel<__half>, a.n_kv_heads, DKV_SMEM, g,
-                   true, stream);
-    return e;
+    auto kernel = bf16 ? attention_bwd_kernel<__nv_bfloat16> : attention_bwd_kernel<__half>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), a.n_heads + a.n_kv_heads);
+    kernel<<<grid, THREADS, BWD_SMEM, stream>>>(g, (int)a.n_heads);
+    return cudaGetLastError();
 }
 
 }  // namespace laya
