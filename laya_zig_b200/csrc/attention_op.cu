@@ -161,7 +161,7 @@ __device__ __forceinline__ void store_rows(const AttnRows& rows, int head, const
 }
 
 __device__ __forceinline__ bool block_tile(const AttnArgs& a, SeqTile* t) {
-    if (threadIdx.x == 0 && blockIdx.y == 0)
+    if (threadIdx.x == 0 && blockIdx.y == 0)  // the grid has a block for every entry
         check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, blockIdx.x, a.status);
     return find_tile(a.cu, a.n_seqs, a.n_tokens, a.max_len, TB, blockIdx.x, threadIdx.x & 31, t);
 }
@@ -485,14 +485,15 @@ AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
 }  // namespace
 
 // Which kernels a call gets: 64-row mma.sync blocks for a little work (rows of
-// all heads times keys, at most 2^20 x 3, in sequences of 512 at most), tcgen05
-// otherwise. Forward and backward of bf16, 12 heads, us by mma.sync / tcgen05:
+// all heads times keys, at most 2^20 x 3, in at most 64 sequences, of at most
+// 512 tokens, because every entry of the table costs blocks), tcgen05 otherwise. Forward and backward of bf16, 12 heads, us by mma.sync / tcgen05:
 // 1 x 64 tokens 9.1 / 19.7, 1 x 256 18.1 / 27.0, 64 x 16 38.1 / 41.8, 16 x 128
 // 31.3 / 35.9; at the limit 1 x 512 36.3 / 36.1, 64 x 64 43.4 / 44.5; beyond it
 // 8 x 256 47.1 / 34.2, 64 x 100 99.8 / 66.1, 512 x 32 295 / 230. (A short
 // sequence takes a whole tile in both.)
 static bool small_call(const laya_attention& a) {
-    return a.max_len <= 512 && a.n_heads <= 1024 && (uint64_t)a.n_tokens * a.n_heads * a.max_len <= 3u << 20;
+    return a.max_len <= 512 && a.n_seqs <= 64 && a.n_heads <= 1024 &&
+           (uint64_t)a.n_tokens * a.n_heads * a.max_len <= 3u << 20;
 }
 
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {

@@ -278,11 +278,12 @@ struct Walk {
     int heads, lane;
     unsigned long long* tickets;
     unsigned long long ahead;  // the next candidate
-    long long x;               // the candidate's slot
+    int x;                     // the candidate's slot
     int head;
-    long long pivot;  // key of entry lane * step: the search's first round
+    int pivot;  // key of entry lane * step: the search's first round
     int step;
-    SeqTile t;  // the item found
+    int end = -1;  // no slot from here on has a tile (-1: not looked up yet)
+    SeqTile t;     // the item found
     bool found;
 
     // Finds the first item (in the forward, before the frame is open: the look
@@ -296,20 +297,36 @@ struct Walk {
         pivot = lane * step < a.n_seqs ? key(a.cu[lane * step], lane * step) : 0;
         next();
     }
-    __device__ __forceinline__ static long long key(int start, int s) { return (long long)(max(start, 0) / ROWS) + s; }
+    __device__ __forceinline__ static int key(int start, int s) { return max(start, 0) / ROWS + s; }
     __device__ __forceinline__ void next() {
         for (found = false; !found;) {
             const unsigned long long item = __shfl_sync(0xffffffffu, ahead, 0);
-            x = (long long)(item / heads);
+            x = (int)(item / heads);
             head = (int)(item - (unsigned long long)x * heads);
-            if (x >= (long long)(a.n_tokens / ROWS) + a.n_seqs) return;
+            if (x >= (end < 0 ? a.n_tokens / ROWS + a.n_seqs : end)) return;
             if (!tickets)
                 ahead = item + gridDim.x;
             else if (lane == 0)
                 ahead = atomicAdd(tickets, 1ull) + gridDim.x;  // not looked at before the item after this one
-            if (lane == 0 && head == 0) check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, x, a.status);
+            t.len = 0;
             found = find();
+            if (!found && t.len == 0 && end < 0) end = slots();
         }
+    }
+    // A table with room for more sequences than it holds ends in many that
+    // start where the last one ends: the slots before those. (3 sequences of
+    // 180 tokens in a table of 1,024, forward and backward: 107 us without it,
+    // 29 with it; 26 in a table of 3.)
+    __device__ __forceinline__ int slots() const {
+        const int* cu = a.cu;
+        const int last = min(max(cu[a.n_seqs], 0), a.n_tokens);
+        const int used = warp_search(a.n_seqs, lane, [&](int i) { return (long long)cu[i]; }, (long long)last - 1) + 1;
+        return last / ROWS + used;
+    }
+    // The whole table, by the loading warps of all CTAs of one kernel of a call.
+    __device__ __forceinline__ void check() const {
+        for (long long s = (long long)blockIdx.x * 32 + lane; s < a.n_seqs; s += (long long)gridDim.x * 32)
+            check_table(a.cu, a.n_seqs, a.n_tokens, a.max_len, s, a.status);
     }
     // find_tile for slot x, with one look at the table for up to 1,024 sequences.
     __device__ __forceinline__ bool find() {
@@ -324,10 +341,10 @@ struct Walk {
         const int s = lo + c1 - 1, start = __shfl_sync(0xffffffffu, at, c1 - 1);
         const int end = c1 < 32 ? __shfl_sync(0xffffffffu, at, c1 & 31) : a.cu[s + 1];
         if (!run_ok(start, end, a.n_tokens, a.max_len)) return false;
-        const long long tile = x - key(start, s);
+        const int tile = x - key(start, s);
         t = SeqTile{start, end - start, 0};
-        if (tile < 0 || tile * ROWS >= t.len) return false;
-        t.row0 = (int)tile * ROWS;
+        if (tile < 0 || (long long)tile * ROWS >= t.len) return false;
+        t.row0 = tile * ROWS;
         return true;
     }
 };
@@ -589,6 +606,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mq, nullptr);
         ld.finish(big);
+        walk.check();
     } else if (warp == MMA) {
         if (elect_one()) {
             const uint32_t q = smem_u32(f.big), kv = smem_u32(f.ring);
@@ -799,7 +817,8 @@ __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a,
 // ------------------------------------------------------------------ delta
 // delta[h][t] = sum_d dO O, a thread to 8 elements, 8 lanes to a row of a head.
 // Bound by memory (both arrays once). Inside the dQ kernel, whose warps are
-// few, it took a third of an item's time at 175-180 tokens.
+// few, it took a third of an item's time at 175-180 tokens (dQ 80 -> 47 us
+// there, delta 8.6).
 constexpr int DELTA_THREADS = 256;
 
 template <typename T>
@@ -1040,6 +1059,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         const int big = ld.items;
         if (ok) ld.item(Item{0, 0, 0, 0, 0, -1}, &mk, &mv);
         ld.finish(big);
+        walk.check();
     } else if (warp == MMA) {
         if (elect_one())
             backward_mmas<T, 1>(f, a, [&](uint32_t p, uint32_t qd, int, bool more) {

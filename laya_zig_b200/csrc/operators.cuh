@@ -61,8 +61,7 @@ inline long long seq_tiles(long long n_tokens, long long n_seqs, int tile_rows) 
     return n_tokens / tile_rows + n_seqs;
 }
 
-// Thread 0 of block x checks entry x (every such grid has at least n_seqs
-// blocks): together the blocks check the whole table.
+// Entry x of the table: the threads of a launch check all of them together.
 __device__ __forceinline__ void check_table(const int* __restrict__ cu, int n_seqs, int n_tokens, int max_len,
                                             long long x, int* status) {
     if (x < n_seqs && !run_ok(cu[x], cu[x + 1], n_tokens, max_len)) atomicOr(status, ERR_BAD_INDEX);

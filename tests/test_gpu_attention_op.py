@@ -249,6 +249,24 @@ def test_forward_without_statistics(max_len):
     assert torch.equal(want, p.out)
 
 
+@kernels
+@pytest.mark.parametrize("lens", [[180, 33] + [0] * 900, [0, 70, 0, 300] + [0] * 1500, [0] * 40 + [130] + [0] * 5])
+def test_tables_with_unused_entries(lens, max_len):
+    """Entries behind the last sequence are passed over, and still checked."""
+    from laya_zig_b200 import gpu
+    p = Problem(lens, max_len=max_len)
+    p.run()
+    p.check()
+    p.cu[len(lens) - 2] += 1
+    p.forward()
+    with pytest.raises(gpu.LayaError) as e:
+        gpu.op_status(p.status.data_ptr())
+    assert e.value.code == gpu.ERR_ARG
+    p.run()
+    with pytest.raises(gpu.LayaError):
+        gpu.op_status(p.status.data_ptr())
+
+
 @pytest.mark.parametrize("table,max_len", [([0, 50, 40, 100], 60), ([-3, 20, 60, 100], 60), ([0, 30, 60, 5000], 60),
                                            ([90, 60, 30, 0], 60), ([0, 10, 20, 100], 60), ([0, 50, 40, 100], LONG),
                                            ([-3, 20, 60, 100], LONG), ([0, 30, 60, 5000], LONG),

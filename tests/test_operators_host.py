@@ -21,7 +21,7 @@ def _shape(**kw):
 
 
 def _fwd(shape, **kw):
-    d = dict(q_ptr=A, q_stride=2304, k_ptr=A + 1536, k_stride=2304, v_ptr=A + 3072, v_stride=2304,
+    d = dict(q_ptr=A, q_stride=2304, k_ptr=A + 1536, k_stride=2304, v_ptr=A + 2 * 1536, v_stride=2304,
              out_ptr=A + (1 << 24), out_stride=768, lse_ptr=A + (1 << 25))
     d.update(kw)
     gpu.attention(shape, **d)
@@ -29,9 +29,9 @@ def _fwd(shape, **kw):
 
 def _bwd(shape, **kw):
     far = A + (1 << 26)
-    d = dict(q_ptr=A, q_stride=2304, k_ptr=A + 1536, k_stride=2304, v_ptr=A + 3072, v_stride=2304,
+    d = dict(q_ptr=A, q_stride=2304, k_ptr=A + 1536, k_stride=2304, v_ptr=A + 2 * 1536, v_stride=2304,
              out_ptr=A + (1 << 24), out_stride=768, lse_ptr=A + (1 << 25), dout_ptr=A + (1 << 23), dout_stride=768,
-             dq_ptr=far, dq_stride=2304, dk_ptr=far + 1536, dk_stride=2304, dv_ptr=far + 3072, dv_stride=2304,
+             dq_ptr=far, dq_stride=2304, dk_ptr=far + 1536, dk_stride=2304, dv_ptr=far + 2 * 1536, dv_stride=2304,
              workspace_ptr=A + (1 << 27), workspace_bytes=1 << 20)
     d.update(kw)
     gpu.attention_backward(shape, **d)
@@ -60,8 +60,8 @@ def test_attention_refuses_f32():
 
 @pytest.mark.parametrize("kw", [dict(q_ptr=0), dict(k_ptr=0), dict(v_ptr=0), dict(out_ptr=0), dict(q_ptr=A + 8),
                                 dict(q_stride=760), dict(k_stride=2300), dict(out_stride=769),
-                                dict(out_ptr=A), dict(out_ptr=A + 3072, out_stride=2304), dict(lse_ptr=A + 4096),
-                                dict(out_ptr=A + 3072 + 16, out_stride=2304), dict(lse_ptr=A + (1 << 25) + 2)])
+                                dict(out_ptr=A), dict(out_ptr=A + 2 * 1536, out_stride=2304), dict(lse_ptr=A + 4096),
+                                dict(out_ptr=A + 2 * 1536 + 16, out_stride=2304), dict(lse_ptr=A + (1 << 25) + 2)])
 def test_attention_refuses_rows(kw):
     assert _code(_fwd, _shape(), **kw) == gpu.ERR_ARG
 
@@ -78,8 +78,8 @@ def test_attention_backward_refuses(kw):
 def test_columns_of_one_packed_array_do_not_overlap():
     """q, k, v and, behind them, out in one row array: accepted as far as the
     host can tell (this host has no GPU, or the address is no device memory)."""
-    code = _code(_fwd, _shape(), q_stride=3072 + 8, k_stride=3072 + 8, v_stride=3072 + 8, out_ptr=A + 4608,
-                 out_stride=3072 + 8)
+    code = _code(_fwd, _shape(), q_stride=3080, k_stride=3080, v_stride=3080, out_ptr=A + 4608,
+                 out_stride=3080)
     import torch
     assert code == (gpu.ERR_ARG if torch.cuda.is_available() else gpu.ERR_NODEV)
 
@@ -249,6 +249,23 @@ def test_every_tile_has_one_block(rows, seed, find):
     got = [find(cu, n, T, max(lens), rows, x) for x in range(T // rows + n)]
     got = [(g[0], g[3]) for g in got if g]
     assert len(got) == len(set(got)) and set(got) == want
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_no_tile_lies_past_the_slots_in_use(seed):
+    """Walk::slots: a table that ends in unused entries is not walked to its
+    end, and nothing before them is left out."""
+    r, rows = random.Random(seed), 128
+    n = r.choice([0, 1, 2, 31, 33, 200, 1024])
+    cu = [r.choice([0, 5, 300])]
+    for _ in range(n):
+        cu.append(cu[-1] + r.choice([0, 1, rows - 1, rows, rows + 1, r.randint(0, 700)]))
+    used, T = max([s + 1 for s in range(n) if cu[s] < cu[n]], default=0), cu[-1] + r.choice([0, 17, 5000])
+    cu += [cu[-1]] * r.choice([1, 3, 900])
+    n = len(cu) - 1
+    end = cu[n] // rows + warp_search(n, lambda i: cu[i], cu[n] - 1) + 1
+    assert end == cu[n] // rows + used
+    assert not any(walk_find(cu, n, T, 700, rows, x) for x in range(end, T // rows + n))
 
 
 @pytest.mark.parametrize("find,rows", [(find_tile, 64), (walk_find, 128)])
