@@ -29,9 +29,24 @@
 // first loads took a third of a CTA's time when every item had its own.
 //
 // TMEM holds 256 columns a CTA: two buffers for scores, so that a tile's are
-// there when the tile before has been dealt with, and the accumulators. What
-// bounds the kernels then is the SFU, 512 cycles of ex2 an SM sub-partition
-// for a 128 x 64 tile (its products take 320 to 640).
+// there when the tile before has been dealt with, and the accumulators. With
+// the registers (20 warps of 96) that allows two CTAs, four softmax warps to a
+// sub-partition, and what bounds the kernels is the latency of these warps'
+// dependent steps (TMEM load, ex2, pack, TMEM store, barrier) more than any
+// unit: on one sequence of 8,192 tokens, 12 heads, the SFU is busy 64 % of the
+// forward's time (512 cycles of ex2 for a 128 x 64 tile), 53 % of dQ's and 46 %
+// of dK/dV's, the tensor cores 32, 39 and 46 %, and issue slots 54 % at most.
+// There the forward takes 336 us (614 TFLOP/s) and the backward 857 (600 in
+// the seven products that it does); 64 sequences of 175-180 tokens 31 and 79
+// us, where an item has three tiles: dK/dV takes 2.9 us a tile there against
+// 1.5, the rest being an item's beginning and end; 2 of 16,000 with a window of
+// 64 (forward) 70 us. The mma.sync kernels took 3,619 us for both passes of the
+// first and 197 of the second.
+//
+// Measured and not kept: the groups on tiles of their own, three CTAs of one
+// group, four ring stages, 1 KB of staging (no faster); an
+// item's last sums followed at once by the next item's scores (batch 111 -> 119
+// us: every tile then pays for keeping track of both items).
 //
 // TMEM is only overwritten by a product after the barrier that says its last
 // reader is done: MMAs to different accumulators are not taken to be ordered.

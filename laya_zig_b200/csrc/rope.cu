@@ -10,7 +10,11 @@
 // Reads and writes each element once and computes one sine and cosine per
 // (token, pair), which all heads of the token share: a warp owns a token,
 // its lanes take a pair each for the table (in shared memory) and then 16
-// bytes each of the row. Bound by memory.
+// bytes each of the row. Bound by memory: 64 sequences of 175-180 tokens, 24
+// heads of 64, bf16 (70 MB) 14.6 us, 4.8 TB/s; 32,768 tokens with 32 of 64
+// elements rotated, f16 (201 MB) 33.7 us, 6.0 TB/s; one sequence of 64 tokens
+// 2.7 us. The first pieces are loaded before the search of the position and
+// the table, which leave the memory idle at a call's beginning and end.
 #include <cmath>
 
 #include "operators.cuh"
