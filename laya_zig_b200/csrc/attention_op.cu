@@ -18,10 +18,16 @@
 // These kernels serve calls that a few waves of blocks finish, where what
 // counts is the chain of dependent steps in one block (find the sequence, load,
 // two to five products of 16 x 8 x 16 instructions, exponentials, store), not
-// a rate. One sequence of 64 tokens, 12 heads, bf16: forward 4.1 us, backward
-// 5.1 us (a short kernel on its own takes 2.1 there). Backward in one launch
+// a rate. One sequence of 64 tokens, 12 heads, bf16: forward 4.2 us, backward
+// 4.5 us (a short kernel on its own takes 2.1 there). Backward in one launch
 // instead of a dQ launch followed by a dK/dV launch that reads its delta: 9.3
 // -> 5.1 us there; delta is recomputed from O, which a row's tile costs little.
+//
+// Sequences of 64 tokens at most have kernels of their own below, whatever
+// their number, because a 128-row tcgen05 item or a search for each of them
+// costs more than its work: forward and backward of 512 sequences of 16 / 32 /
+// 64 tokens, 12 heads, 265 / 230 / 235 us on tcgen05, 72 / 102 / 154 here (139 /
+// 277 / 553 MB: 3.6 TB/s for the last).
 //
 // Rows outside their sequence and absent tokens are filled with zeros on
 // their way into shared memory (cp.async with a source size of 0), so nothing
@@ -71,13 +77,16 @@ __device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Rows row0 .. row0 + 63 of the sequence, 64 elements each, into a tile.
+// Rows row0 .. row0 + 63 of the sequence (the first n times 16 of them), 64
+// elements each, into a tile.
 template <typename T>
 __device__ __forceinline__ void load_tile(T* s, const AttnRows& rows, int head, const AttnArgs& a, const SeqTile& t,
-                                          int row0) {
+                                          int row0, int n = TB / 16) {
     const T* g = static_cast<const T*>(rows.p) + head * 64;
+    static_assert(THREADS / 8 == 16, "a round of the loop takes 16 rows");
 #pragma unroll
     for (int i = 0; i < TILE / 8 / THREADS; i++) {
+        if (i >= n) break;
         const int idx = threadIdx.x + i * THREADS, r = idx >> 3, c = (idx & 7) * 8;
         const bool ok = present(a, t, row0 + r);
         const long long row = t.start + (ok ? row0 + r : 0);
@@ -107,14 +116,17 @@ __device__ __forceinline__ void clear(float (&c)[N][4]) {
     for (int j = 0; j < N; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
 }
 
-// c[16 x 64 tile rows] = a (16 x 64) . tile^T
+// c[16 x 64 tile rows] = a (16 x 64) . tile^T, of the tile's first n times 16
+// rows (0 for the others)
 template <typename T>
-__device__ __forceinline__ void mma_nt(float (&c)[8][4], const uint32_t (&a)[4][4], const T* tile, int lane) {
+__device__ __forceinline__ void mma_nt(float (&c)[8][4], const uint32_t (&a)[4][4], const T* tile, int lane,
+                                       int n = 4) {
     clear(c);
 #pragma unroll
     for (int ks = 0; ks < 4; ks++)
 #pragma unroll
         for (int np = 0; np < 4; np++) {
+            if (np >= n) break;
             uint32_t b[4];
             ldsm4(b, tile + swz(np * 16 + (lane & 7) + (lane >> 4) * 8, ks * 16 + ((lane >> 3) & 1) * 8));
             mma<T>(c[2 * np], a[ks], b[0], b[1]);
@@ -122,41 +134,74 @@ __device__ __forceinline__ void mma_nt(float (&c)[8][4], const uint32_t (&a)[4][
         }
 }
 
-// c[16 x 64] += p (16 x 64 tile rows, as accumulators) . tile
+// c[16 x 64] += a (16 x 16) . rows 16 kk .. 16 kk + 15 of the tile
 template <typename T>
-__device__ __forceinline__ void mma_nn(float (&c)[8][4], const float (&p)[8][4], const T* tile, int lane) {
+__device__ __forceinline__ void mma_step(float (&c)[8][4], const uint32_t (&a)[4], const T* tile, int kk, int lane) {
+#pragma unroll
+    for (int dp = 0; dp < 4; dp++) {
+        uint32_t b[4];
+        ldsm4_t(b, tile + swz(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, dp * 16 + (lane >> 4) * 8));
+        mma<T>(c[2 * dp], a, b[0], b[1]);
+        mma<T>(c[2 * dp + 1], a, b[2], b[3]);
+    }
+}
+
+// c[16 x 64] += p (16 x the tile's first n times 16 rows, as accumulators) . tile
+template <typename T>
+__device__ __forceinline__ void mma_nn(float (&c)[8][4], const float (&p)[8][4], const T* tile, int lane, int n = 4) {
 #pragma unroll
     for (int kk = 0; kk < 4; kk++) {
+        if (kk >= n) break;
         uint32_t a[4];
         a[0] = pack2<T>(p[2 * kk][0], p[2 * kk][1]);
         a[1] = pack2<T>(p[2 * kk][2], p[2 * kk][3]);
         a[2] = pack2<T>(p[2 * kk + 1][0], p[2 * kk + 1][1]);
         a[3] = pack2<T>(p[2 * kk + 1][2], p[2 * kk + 1][3]);
-#pragma unroll
-        for (int dp = 0; dp < 4; dp++) {
-            uint32_t b[4];
-            ldsm4_t(b, tile + swz(kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, dp * 16 + (lane >> 4) * 8));
-            mma<T>(c[2 * dp], a, b[0], b[1]);
-            mma<T>(c[2 * dp + 1], a, b[2], b[3]);
-        }
+        mma_step<T>(c, a, tile, kk, lane);
     }
 }
 
-// A warp's 16 x 64 accumulators, times two row factors, to rows of the
-// sequence; rows past its end are not written.
+// c[16 x 64] += the transpose of x's columns 16 warp .. 16 warp + 15, over the
+// first n times 16 rows of x and of the tile
 template <typename T>
-__device__ __forceinline__ void store_rows(const AttnRows& rows, int head, const SeqTile& t, int r0, int lane,
-                                           const float (&c)[8][4], float f0, float f1) {
-    const int i0 = r0 + (lane >> 2), i1 = i0 + 8;
-    T* g = static_cast<T*>(rows.p) + head * 64 + 2 * (lane & 3);
+__device__ __forceinline__ void mma_tn(float (&c)[8][4], const T* x, const T* tile, int warp, int lane, int n) {
+#pragma unroll
+    for (int kk = 0; kk < 4; kk++) {
+        if (kk >= n) break;
+        uint32_t a[4];
+        ldsm4_t(a, x + swz(kk * 16 + (lane & 7) + (lane >> 4) * 8, warp * 16 + ((lane >> 3) & 1) * 8));
+        mma_step<T>(c, a, tile, kk, lane);
+    }
+}
+
+// A warp's 16 x 64 accumulators, times two row factors, into its rows of a
+// tile as 16-bit values; 0 for the factor 0, whatever the accumulator holds.
+template <typename T>
+__device__ __forceinline__ void put_rows(T* s, const float (&c)[8][4], int warp, int lane, float f0 = 1.f,
+                                         float f1 = 1.f) {
+    const int r = warp * 16 + (lane >> 2), k = 2 * (lane & 3);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        if (i0 < t.len)
-            *reinterpret_cast<uint32_t*>(g + (t.start + i0) * rows.ld + j * 8) =
-                f0 == 0.f ? 0u : pack2<T>(c[j][0] * f0, c[j][1] * f0);
-        if (i1 < t.len)
-            *reinterpret_cast<uint32_t*>(g + (t.start + i1) * rows.ld + j * 8) =
-                f1 == 0.f ? 0u : pack2<T>(c[j][2] * f1, c[j][3] * f1);
+        *reinterpret_cast<uint32_t*>(s + swz(r, 8 * j + k)) = f0 == 0.f ? 0u : pack2<T>(c[j][0] * f0, c[j][1] * f0);
+        *reinterpret_cast<uint32_t*>(s + swz(r + 8, 8 * j + k)) = f1 == 0.f ? 0u : pack2<T>(c[j][2] * f1, c[j][3] * f1);
+    }
+}
+
+// The same to the sequence's rows r0 + 16 warp .. in global memory, those past
+// its end left alone; by way of the warp's rows of tile s, which nobody needs
+// any more: whole rows of 128 bytes an instruction instead of 16 bytes each.
+template <typename T>
+__device__ __forceinline__ void store_rows(T* s, const AttnRows& rows, int head, const SeqTile& t, int r0, int warp,
+                                           int lane, const float (&c)[8][4], float f0, float f1) {
+    __syncwarp();
+    put_rows<T>(s, c, warp, lane, f0, f1);
+    __syncwarp();
+    T* g = static_cast<T*>(rows.p) + head * 64 + (lane & 7) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = warp * 16 + i * 4 + (lane >> 3);
+        const uint4 u = *reinterpret_cast<const uint4*>(s + swz(r, (lane & 7) * 8));
+        if (r0 + r < t.len) *reinterpret_cast<uint4*>(g + (t.start + r0 + r) * rows.ld) = u;
     }
 }
 
@@ -261,7 +306,7 @@ __global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const AttnArg
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
-    store_rows<T>(a.io.out, h, t, t.row0 + warp * 16, lane, o, p0 ? 1.f / l0 : 0.f, p1 ? 1.f / l1 : 0.f);
+    store_rows<T>(sq, a.io.out, h, t, t.row0, warp, lane, o, p0 ? 1.f / l0 : 0.f, p1 ? 1.f / l1 : 0.f);
     if (a.io.lse && (lane & 3) == 0) {
         float* g = a.io.lse + (long long)h * a.n_tokens + t.start;
         if (i0 < t.len) g[i0] = p0 ? m0 * a.scale + logf(l0) : -INFINITY;
@@ -362,7 +407,7 @@ __device__ __forceinline__ void dq_block(const AttnArgs& a, const SeqTile& t, in
         mma_nn<T>(dq, s, sk + b * TILE, lane);
         __syncthreads();
     }
-    store_rows<T>(a.io.dq, h, t, t.row0 + warp * 16, lane, dq, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+    store_rows<T>(sq, a.io.dq, h, t, t.row0, warp, lane, dq, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
 }
 
 template <typename T>
@@ -449,8 +494,8 @@ __device__ __forceinline__ void dkv_block(const AttnArgs& a, const SeqTile& t, i
         __syncthreads();
     }
     const bool p0 = present(a, t, j0), p1 = present(a, t, j1);
-    store_rows<T>(a.io.dk, hk, t, t.row0 + warp * 16, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
-    store_rows<T>(a.io.dv, hk, t, t.row0 + warp * 16, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
+    store_rows<T>(sk, a.io.dk, hk, t, t.row0, warp, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+    store_rows<T>(sv, a.io.dv, hk, t, t.row0, warp, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
 }
 
 constexpr int BWD_SMEM = 8 * TILE * 2 + 3 * TB * 4;
@@ -465,6 +510,214 @@ __global__ void __launch_bounds__(THREADS, 2) attention_bwd_kernel(const AttnArg
         dq_block<T>(a, t, y, smem);
     else
         dkv_block<T>(a, t, y - n_heads, smem);
+}
+
+// ------------------------------------------------------------------ short sequences
+// Of 64 tokens at most: one tile, so no search, no running maximum, and no
+// second look at anything. Warps and steps of 16 rows that the sequence does
+// not reach are left out.
+
+// Sequence seq, if it has tokens.
+__device__ __forceinline__ bool one_sequence(const AttnArgs& a, long long seq, SeqTile* t) {
+    const int start = a.cu[seq], end = a.cu[seq + 1];
+    *t = SeqTile{start, end - start, 0};
+    if (run_ok(start, end, a.n_tokens, a.max_len)) return start < end;
+    if (blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.status, ERR_BAD_INDEX);
+    return false;
+}
+
+// What a thread holds of rows i0 and i1 becomes `gone` at keys (bits of
+// `there`) that its row does not see.
+__device__ __forceinline__ void hide(float (&s)[8][4], uint64_t there, int window, int i0, int i1, int lane, float gone) {
+    if (there == ~0ull && !edge(window, 0, TB, 0, TB)) return;
+    const int c0 = 2 * (lane & 3);
+    const uint64_t w = there >> c0;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const bool ok = (w >> (8 * j + e)) & 1;
+            const int key = c0 + 8 * j + e;
+            if (!ok || (window >= 0 && abs(i0 - key) > window)) s[j][e] = gone;
+            if (!ok || (window >= 0 && abs(i1 - key) > window)) s[j][2 + e] = gone;
+        }
+}
+
+constexpr int FWD_ONE_SMEM = 3 * TILE * 2;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 6) attention_fwd_one_kernel(const AttnArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    T* sq = reinterpret_cast<T*>(smem);
+    T* sk = sq + TILE;
+    T* sv = sk + TILE;
+    __shared__ uint32_t bits[2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, hk = h / a.group;
+    const float sl2 = a.scale * LOG2E;
+    for (long long seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
+        SeqTile t;
+        if (!one_sequence(a, seq, &t)) continue;
+        const int n = (t.len + 15) >> 4;
+        load_tile(sq, a.io.q, h, a, t, 0, n);
+        load_tile(sk, a.io.k, hk, a, t, 0, n);
+        load_tile(sv, a.io.v, hk, a, t, 0, n);
+        key_bits(bits, a, t, 0);
+        copy_commit();
+        const int i0 = warp * 16 + (lane >> 2), i1 = i0 + 8;
+        const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
+        copy_wait<0>();
+        __syncthreads();
+        if (warp < n) {
+            uint32_t f[4][4];
+            float s[8][4], o[8][4];
+            load_a(f, sq, warp, lane);
+            mma_nt<T>(s, f, sk, lane, n);
+            hide(s, bits[0] | (uint64_t)bits[1] << 32, a.window, i0, i1, lane, -INFINITY);
+            float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    m0 = fmaxf(m0, s[j][e]);
+                    m1 = fmaxf(m1, s[j][2 + e]);
+                }
+#pragma unroll
+            for (int x = 1; x < 4; x *= 2) {
+                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
+                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
+            }
+            const float u0 = m0 == -INFINITY ? 0.f : m0 * sl2, u1 = m1 == -INFINITY ? 0.f : m1 * sl2;
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    s[j][e] = ex2_approx(fmaf(s[j][e], sl2, -u0));
+                    s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -u1));
+                    l0 += s[j][e];
+                    l1 += s[j][2 + e];
+                }
+#pragma unroll
+            for (int x = 1; x < 4; x *= 2) {
+                l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+                l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+            }
+            clear(o);
+            mma_nn<T>(o, s, sv, lane, n);
+            store_rows<T>(sq, a.io.out, h, t, 0, warp, lane, o, p0 ? 1.f / l0 : 0.f, p1 ? 1.f / l1 : 0.f);
+            if (a.io.lse && (lane & 3) == 0) {
+                float* g = a.io.lse + (long long)h * a.n_tokens + t.start;
+                if (i0 < t.len) g[i0] = p0 ? m0 * a.scale + logf(l0) : -INFINITY;
+                if (i1 < t.len) g[i1] = p1 ? m1 * a.scale + logf(l1) : -INFINITY;
+            }
+        }
+        __syncthreads();  // the tiles are free for the next sequence
+    }
+}
+
+// The backward pass, all of a sequence and key head in one block.
+// S and dP are computed once, five products instead of seven; delta is the sum
+// over P dP, which is all there, in f32 (from O, rounded to 16 bits, it has an
+// error that a few keys do not average out).
+template <bool SHARED>
+constexpr int ONE_SMEM = (SHARED ? 7 : 6) * TILE * 2;
+
+// SHARED: several query heads to a key head, whose dK and dV are then held
+// while the next one's scores are computed: fewer blocks to an SM.
+template <typename T, bool SHARED>
+__global__ void __launch_bounds__(THREADS, SHARED ? 3 : 4) attention_bwd_one_kernel(const AttnArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    T* sk = reinterpret_cast<T*>(smem);
+    T* sv = sk + TILE;
+    T* sq = sv + TILE;
+    T* sdo = sq + TILE;
+    T* sp = sdo + TILE;
+    T* sds = sp + TILE;
+    T* sdq = SHARED ? sds + TILE : sv;  // V is not needed again when it has one query head
+    __shared__ uint32_t bits[2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y;
+    const float sl2 = a.scale * LOG2E;
+    for (long long seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
+        SeqTile t;
+        if (!one_sequence(a, seq, &t)) continue;
+        const int n = (t.len + 15) >> 4;
+        const int i0 = warp * 16 + (lane >> 2), i1 = i0 + 8;  // this thread's queries, then keys
+        const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
+        load_tile(sk, a.io.k, hk, a, t, 0, n);
+        load_tile(sv, a.io.v, hk, a, t, 0, n);
+        key_bits(bits, a, t, 0);
+        float dk[8][4], dv[8][4];
+        if (SHARED) {
+            clear(dk);
+            clear(dv);
+        }
+        int h = hk * a.group;
+        do {
+            load_tile(sq, a.io.q, h, a, t, 0, n);
+            load_tile(sdo, a.io.dout, h, a, t, 0, n);
+            copy_commit();
+            const float* lse = a.io.lse + (long long)h * a.n_tokens + t.start;
+            const float e0 = p0 ? lse[i0] * LOG2E : 0.f, e1 = p1 ? lse[i1] * LOG2E : 0.f;
+            copy_wait<0>();
+            __syncthreads();
+            float dp[8][4];  // later dQ
+            if (warp < n) {
+                uint32_t f[4][4];
+                float s[8][4];
+                load_a(f, sq, warp, lane);
+                mma_nt<T>(s, f, sk, lane, n);
+                load_a(f, sdo, warp, lane);
+                mma_nt<T>(dp, f, sv, lane, n);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        s[j][e] = ex2_approx(fmaf(s[j][e], sl2, -e0));
+                        s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -e1));
+                    }
+                hide(s, bits[0] | (uint64_t)bits[1] << 32, a.window, i0, i1, lane, 0.f);
+                float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        d0 = fmaf(s[j][e], dp[j][e], d0);
+                        d1 = fmaf(s[j][2 + e], dp[j][2 + e], d1);
+                    }
+                put_rows<T>(sp, s, warp, lane);
+#pragma unroll
+                for (int x = 1; x < 4; x *= 2) {
+                    d0 += __shfl_xor_sync(0xffffffffu, d0, x);
+                    d1 += __shfl_xor_sync(0xffffffffu, d1, x);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        s[j][e] *= dp[j][e] - d0;
+                        s[j][2 + e] *= dp[j][2 + e] - d1;
+                    }
+                put_rows<T>(sds, s, warp, lane);
+                clear(dp);
+                mma_nn<T>(dp, s, sk, lane, n);
+            }
+            __syncthreads();
+            if (warp < n) store_rows<T>(sdq, a.io.dq, h, t, 0, warp, lane, dp, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+            if (!SHARED) {
+                clear(dk);
+                clear(dv);
+            }
+            if (warp < n) {
+                mma_tn<T>(dv, sp, sdo, warp, lane, n);
+                mma_tn<T>(dk, sds, sq, warp, lane, n);
+            }
+            __syncthreads();
+        } while (SHARED && ++h < (hk + 1) * a.group);
+        if (warp < n) {
+            store_rows<T>(sds, a.io.dk, hk, t, 0, warp, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+            store_rows<T>(sp, a.io.dv, hk, t, 0, warp, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
+        }
+    }
 }
 
 AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
@@ -484,21 +737,43 @@ AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
 
 }  // namespace
 
-// Which kernels a call gets: 64-row mma.sync blocks for a little work (rows of
-// all heads times keys, at most 2^20 x 3, in at most 64 sequences, of at most
-// 512 tokens, because every entry of the table costs blocks), tcgen05 otherwise. Forward and backward of bf16, 12 heads, us by mma.sync / tcgen05:
-// 1 x 64 tokens 9.1 / 19.7, 1 x 256 18.1 / 27.0, 64 x 16 38.1 / 41.8, 16 x 128
-// 31.3 / 35.9; at the limit 1 x 512 36.3 / 36.1, 64 x 64 43.4 / 44.5; beyond it
-// 8 x 256 47.1 / 34.2, 64 x 100 99.8 / 66.1, 512 x 32 295 / 230. (A short
-// sequence takes a whole tile in both.)
+// Which kernels a call gets. Sequences of 64 tokens at most: a block to a
+// sequence and head; otherwise 64-row mma.sync blocks for a little work (rows
+// of all heads times keys, at most 2^20 x 3, in at most 64 sequences, of at
+// most 512 tokens, because every entry of the table costs blocks), and tcgen05
+// for the rest. Forward and backward of bf16, 12 heads, us by mma.sync /
+// tcgen05: 1 x 256 tokens 17.1 / 27.0, 16 x 128 29.3 / 35.9; at the limit 1 x
+// 512 36.3 / 36.1; beyond it 8 x 256 47.1 / 34.2, 64 x 100 99.8 / 66.1.
 static bool small_call(const laya_attention& a) {
     return a.max_len <= 512 && a.n_seqs <= 64 && a.n_heads <= 1024 &&
            (uint64_t)a.n_tokens * a.n_heads * a.max_len <= 3u << 20;
 }
 
+// Does the backward pass of short sequences take a block to a sequence and key
+// head? With no more than 96 of these most SMs would idle, and blocks of
+// their own for dQ and for dK and dV end sooner, searching included: 1 x 64
+// tokens, 12 heads 4.6 us instead of 7.2, 8 x 64 6.7 instead of 7.7, but 32 x 64
+// 17.3 instead of 9.2.
+static bool one_block_each(const laya_attention& a) {
+    return a.max_len <= TB && (uint64_t)a.n_seqs * a.n_kv_heads > 96;
+}
+
+// A few times the blocks that the GPU holds at once: a block takes every
+// gridDim.x-th sequence.
+static cudaError_t launch_one(void (*kernel)(AttnArgs), int smem, unsigned heads, const AttnArgs& g, cudaStream_t stream) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const unsigned most = (148 * 16 + heads - 1) / heads;
+    kernel<<<dim3((unsigned)g.n_seqs < most ? g.n_seqs : most, heads), THREADS, smem, stream>>>(g);
+    return cudaGetLastError();
+}
+
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
     const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
     const AttnArgs g = make_args(a, io);
+    if (a.max_len <= TB)
+        return launch_one(bf16 ? attention_fwd_one_kernel<__nv_bfloat16> : attention_fwd_one_kernel<__half>, FWD_ONE_SMEM,
+                          a.n_heads, g, stream);
     if (!small_call(a)) return launch_attention_fwd_tc(bf16, (int)a.n_heads, g, stream);
     auto kernel = bf16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>;
     const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), a.n_heads);
@@ -509,6 +784,13 @@ cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cuda
 cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
     const bool bf16 = a.elem_dtype == LAYA_DT_BF16;
     const AttnArgs g = make_args(a, io);
+    if (one_block_each(a)) {
+        if (g.group > 1)
+            return launch_one(bf16 ? attention_bwd_one_kernel<__nv_bfloat16, true> : attention_bwd_one_kernel<__half, true>,
+                              ONE_SMEM<true>, a.n_kv_heads, g, stream);
+        return launch_one(bf16 ? attention_bwd_one_kernel<__nv_bfloat16, false> : attention_bwd_one_kernel<__half, false>,
+                          ONE_SMEM<false>, a.n_kv_heads, g, stream);
+    }
     if (!small_call(a)) return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
     auto kernel = bf16 ? attention_bwd_kernel<__nv_bfloat16> : attention_bwd_kernel<__half>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM);

@@ -249,6 +249,34 @@ def test_forward_without_statistics(max_len):
     assert torch.equal(want, p.out)
 
 
+@pytest.mark.parametrize("hq,hk", [(2, 2), (6, 2), (5, 1), (64, 64)])
+@pytest.mark.parametrize("window", [-1, 0, 2, 40])
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_short_sequences(hq, hk, window, masked):
+    """At most 64 tokens each, more of them than blocks; a third of the tokens
+    and every seventh sequence absent."""
+    lens = ([1, 16, 17, 33, 0, 64, 48, 2, 31, 63, 15] * (4 if hq > 8 else 60))[:-3]
+    owner = np.repeat(np.arange(len(lens)), lens)
+
+    def mask(n):
+        return (np.arange(n) % 3 != 1) & (owner % 7 != 3)
+    p = Problem(lens, hq=hq, hk=hk, window=window, mask=mask if masked else None, dtype="F16" if masked else "BF16")
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("dtype", ["BF16", "F16"])
+def test_one_key_has_no_gradient_through_its_score(dtype):
+    """A query that sees one key has P = 1 whatever the score: dQ and dK are 0
+    but for what exp(S - lse) is off 1. delta = P dP, so dS = P dP (1 - P);
+    |1 - P| <= 2^-18 (S and lse below 2^3 in f32, each off by a few 2^-21), and
+    |dP| <= 64 |dO| |V| < 64 * 25: |dQ| <= 0.125 * 1600 * 2^-18 * 5 < 2^-8."""
+    p = Problem([1] * 50 + [9, 64, 30], hq=3, hk=3, window=0, dtype=dtype)
+    p.run()
+    assert (p.dqkv[POISON:p.T - POISON, :2 * 3 * 64].abs() < 2.0 ** -8).all()
+    p.check()
+
+
 @kernels
 @pytest.mark.parametrize("lens", [[180, 33] + [0] * 900, [0, 70, 0, 300] + [0] * 1500, [0] * 40 + [130] + [0] * 5])
 def test_tables_with_unused_entries(lens, max_len):
