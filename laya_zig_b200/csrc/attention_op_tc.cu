@@ -879,9 +879,13 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         prefetch_tmap(&mv);
         prefetch_tmap(&mdo);
     }
-    griddep_launch();
     const Frame f = open_frame<C>(raw, warp);
     griddep_wait();  // from here on, what earlier kernels wrote
+    // dK/dV's CTAs may take the places of this kernel's as they come free: that
+    // kernel needs only what was complete here (delta and the counters), made
+    // visible to it by the fence.
+    __threadfence();
+    griddep_launch();
     Walk walk(a, heads, lane, warp == LOADER, a.io.tickets);
     Bars* bar = f.bar;
 
@@ -1025,7 +1029,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         prefetch_tmap(&mdo);
     }
     const Frame f = open_frame<C>(raw, warp);
-    griddep_wait();  // from here on, what earlier kernels wrote
+    // Starts when every CTA of dQ has seen delta complete, and does not use
+    // dQ: it waits for that kernel only before it ends (below).
     Walk walk(a, heads, lane, warp == LOADER, a.io.tickets + 1);
     Bars* bar = f.bar;
 
@@ -1166,6 +1171,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         }
     }
     close_frame<C>(f, warp);
+    griddep_wait();  // what follows this kernel follows dQ too
 }
 
 using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnArgs, int);
