@@ -252,7 +252,7 @@ def test_forward_without_statistics(max_len):
 @pytest.mark.parametrize("hq,hk", [(2, 2), (6, 2), (5, 1), (64, 64)])
 @pytest.mark.parametrize("window", [-1, 0, 2, 40])
 @pytest.mark.parametrize("masked", [False, True])
-def test_many_short_sequences(hq, hk, window, masked):
+def test_more_short_sequences_than_blocks(hq, hk, window, masked):
     """At most 64 tokens each, more of them than blocks; a third of the tokens
     and every seventh sequence absent."""
     lens = ([1, 16, 17, 33, 0, 64, 48, 2, 31, 63, 15] * (4 if hq > 8 else 60))[:-3]
@@ -365,3 +365,48 @@ def test_two_streams_at_once(lens):
     torch.cuda.synchronize()
     for p, w in zip(ps, want):
         assert torch.equal(p.dqkv, w)
+
+
+@pytest.mark.parametrize("hq,hk", [(4, 4), (6, 2)])
+def test_calls_in_a_row_share_a_workspace(hq, hk):
+    """Backward passes back to back on one stream with one workspace, each
+    followed at once by a kernel that overwrites its results: eager, and as two
+    graphs replayed in turn."""
+    import torch
+    ps = [Problem(lens, hq=hq, hk=hk, seed=i) for i, lens in enumerate([[700, 900, 33], [2000], [300] * 20])]
+    for p in ps:
+        p.run()
+    torch.cuda.synchronize()
+    want = [p.dqkv.clone() for p in ps]
+    ws = max((p.ws for p in ps), key=lambda w: w.numel())
+    s = torch.cuda.Stream()
+    kept = [torch.empty_like(w) for w in want]
+
+    def go(i):
+        p = ps[i]
+        p.ws = ws
+        p.backward(s.cuda_stream)
+        kept[i].copy_(p.dqkv)
+        p.dqkv.fill_(7.0)
+
+    def check():
+        torch.cuda.synchronize()
+        for i, p in enumerate(ps):
+            assert torch.equal(kept[i], want[i]) and (p.dqkv == 7).all()
+            kept[i].zero_()
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            for i in range(3):
+                go(i)
+    check()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g, order in zip(graphs, [(0, 2, 1), (1, 0, 2)]):
+        with torch.cuda.graph(g, stream=s):
+            for i in order:
+                go(i)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(4):
+            for g in graphs:
+                g.replay()
+    check()
