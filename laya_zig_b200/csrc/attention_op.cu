@@ -617,8 +617,9 @@ __global__ void __launch_bounds__(THREADS, 6) attention_fwd_one_kernel(const Att
 
 // The backward pass, all of a sequence and key head in one block.
 // S and dP are computed once, five products instead of seven; delta is the sum
-// over P dP, which is all there, in f32 (from O, rounded to 16 bits, it has an
-// error that a few keys do not average out).
+// over P dP, which is all there, in f32 (from O, rounded to 16 bits, it is off by
+// up to half a step of sum |dO O|, which dQ and dK of a few keys then show: 1.8
+// times the error of a 32-bit pass rounded once at 2 keys, 1.4 at 32 and more).
 template <bool SHARED>
 constexpr int ONE_SMEM = (SHARED ? 7 : 6) * TILE * 2;
 
@@ -750,12 +751,14 @@ static bool small_call(const laya_attention& a) {
 }
 
 // Does the backward pass of short sequences take a block to a sequence and key
-// head? With no more than 96 of these most SMs would idle, and blocks of
-// their own for dQ and for dK and dV end sooner, searching included: 1 x 64
-// tokens, 12 heads 4.6 us instead of 7.2, 8 x 64 6.7 instead of 7.7, but 32 x 64
-// 17.3 instead of 9.2.
+// head? Up to 32 tokens always: delta from P dP matters with few keys (see the
+// kernel), and costs nothing (1 x 16 tokens, 12 heads 5.3 us, 5.2 in blocks of
+// their own for dQ and for dK and dV). Up to 64 when there are more than 96 of
+// them: before that most SMs idle and the blocks of their own end sooner (1 x 64
+// 4.9 us instead of 6.8, 8 x 64 6.7 instead of 7.0, but 32 x 64 17.3 instead of
+// 9.2).
 static bool one_block_each(const laya_attention& a) {
-    return a.max_len <= TB && (uint64_t)a.n_seqs * a.n_kv_heads > 96;
+    return a.max_len <= 32 || (a.max_len <= TB && (uint64_t)a.n_seqs * a.n_kv_heads > 96);
 }
 
 // A few times the blocks that the GPU holds at once: a block takes every
