@@ -794,7 +794,7 @@ cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cuda
         return launch_one(bf16 ? attention_bwd_one_kernel<__nv_bfloat16, false> : attention_bwd_one_kernel<__half, false>,
                           ONE_SMEM<false>, a.n_kv_heads, g, stream);
     }
-    if (!small_call(a)) return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
+    if (!small_call(a) || attention_near(a.window)) return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
     auto kernel = bf16 ? attention_bwd_kernel<__nv_bfloat16> : attention_bwd_kernel<__half>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM);
     if (e != cudaSuccess) return e;

@@ -69,6 +69,10 @@ __device__ __forceinline__ bool edge(int window, int row0, int rows, int col0, i
     return window >= 0 && (row0 + rows - 1 - col0 > window || col0 + cols - 1 - row0 > window);
 }
 
+// Windows whose delta the backward pass takes from P dP instead of dO O
+// (attention_op_tc.cu).
+inline bool attention_near(int window) { return window >= 0 && window <= 4; }
+
 // attention_op_tc.cu
 cudaError_t launch_attention_fwd_tc(bool bf16, int n_heads, const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attention_bwd_tc(bool bf16, int n_heads, int n_kv_heads, const AttnArgs& a, cudaStream_t stream);

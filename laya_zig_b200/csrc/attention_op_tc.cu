@@ -36,17 +36,19 @@
 // unit: on one sequence of 8,192 tokens, 12 heads, the SFU is busy 64 % of the
 // forward's time (512 cycles of ex2 for a 128 x 64 tile), 53 % of dQ's and 46 %
 // of dK/dV's, the tensor cores 32, 39 and 46 %, and issue slots 54 % at most.
-// There the forward takes 336 us (614 TFLOP/s) and the backward 857 (600 in
-// the seven products that it does); 64 sequences of 175-180 tokens 31 and 79
-// us, where an item has three tiles: dK/dV takes 2.9 us a tile there against
-// 1.5, the rest being an item's beginning and end; 2 of 16,000 with a window of
-// 64 (forward) 70 us. The mma.sync kernels took 3,619 us for both passes of the
-// first and 197 of the second.
+// There the forward takes 340 us (606 TFLOP/s) and the backward 760 (678 over
+// the five products needed, 949 over the seven that it does); 64 sequences of
+// 175-180 tokens 31 and 76 us, where an item has three tiles: of an item's 10,500
+// cycles in dK/dV these take 6,000, waiting for the accumulators 800, storing them
+// 2,500 and the next item's beginning 600 (forward: 6,200, of them 3,500 in tiles);
+// 2 of 16,000 with a window of 64 (forward) 71 us. The mma.sync kernels took 3,619
+// us for both passes of the first and 197 of the second.
 //
 // Measured and not kept: the groups on tiles of their own, three CTAs of one
-// group, four ring stages, 1 KB of staging (no faster); an
-// item's last sums followed at once by the next item's scores (batch 111 -> 119
-// us: every tile then pays for keeping track of both items).
+// group, four ring stages, 1 KB of staging (no faster); an item's last sums
+// followed at once by the next item's scores (111 -> 119 us for 64 x 175-180: the
+// scores are there in time as it is, and every tile pays for keeping track of both
+// items).
 //
 // TMEM is only overwritten by a product after the barrier that says its last
 // reader is done: MMAs to different accumulators are not taken to be ordered.
@@ -859,6 +861,55 @@ __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const At
     if (ok && c == 0) a.io.delta[(long long)h * a.n_tokens + t] = sum;
 }
 
+// The same for narrow windows, as the sum over P dP of the few keys: O, rounded to
+// 16 bits, puts delta off by up to half a step of sum |dO O|, which gradients of
+// few keys show (1.7 times the error of a 32-bit pass rounded once at a window of
+// 1, 1.5 at 4; 1.4 this way, as at wider ones). A warp to a token, eight lanes to a
+// head. 64 x 180 tokens, 12 heads, window 4: forward and backward 144 us, 112 with
+// the kernel above; window 1: 125.
+template <typename T>
+__global__ void __launch_bounds__(DELTA_THREADS) attention_near_delta_kernel(const AttnArgs a, int heads) {
+    griddep_launch();
+    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the two kernels that follow
+    const int lane = threadIdx.x & 31, c = (lane & 7) * 8;
+    const long long t = (long long)blockIdx.x * (DELTA_THREADS / 32) + (threadIdx.x >> 5);
+    if (t >= a.n_tokens) return;
+    const int seq = warp_search(a.n_seqs, lane, [&](int i) { return (long long)a.cu[i]; }, t);
+    if (seq < 0) return;
+    const int start = a.cu[seq], end = a.cu[seq + 1];
+    if (!run_ok(start, end, a.n_tokens, a.max_len) || t < start || t >= end || (a.mask && !a.mask[t])) return;
+    const long long lo = max((long long)start, t - a.window), hi = min((long long)end - 1, t + a.window);
+    const float sl2 = a.scale * LOG2E;
+    auto dot = [](const uint4& x, const uint4& y) {
+        const T* p = reinterpret_cast<const T*>(&x);
+        const T* q = reinterpret_cast<const T*>(&y);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum = fmaf(to_float(p[e]), to_float(q[e]), sum);
+        return sum;
+    };
+    auto row = [&](const AttnRows& r, long long i, int head) {
+        return *reinterpret_cast<const uint4*>(static_cast<const T*>(r.p) + i * r.ld + head * 64 + c);
+    };
+    for (int h0 = 0; h0 < heads; h0 += 4) {
+        const int h = min(h0 + (lane >> 3), heads - 1), hk = h / a.group;  // a head too many: the last one again
+        const uint4 q = row(a.io.q, t, h), d = row(a.io.dout, t, h);
+        const float e = a.io.lse[(long long)h * a.n_tokens + t] * LOG2E;
+        float sum = 0.f;
+        for (long long j = lo; j <= hi; j++) {
+            if (a.mask && !a.mask[j]) continue;
+            float s = dot(q, row(a.io.k, j, hk)), dp = dot(d, row(a.io.v, j, hk));
+#pragma unroll
+            for (int x = 1; x < 8; x *= 2) {
+                s += __shfl_xor_sync(0xffffffffu, s, x);
+                dp += __shfl_xor_sync(0xffffffffu, dp, x);
+            }
+            sum = fmaf(ex2_approx(fmaf(s, sl2, -e)), dp, sum);
+        }
+        if (c == 0) a.io.delta[(long long)h * a.n_tokens + t] = sum;
+    }
+}
+
 // dQ and dK/dV use nothing of one another. The first of them waits for delta
 // and the counters; then the second one's CTAs may take the places of its CTAs
 // as these come free, with what was complete there made visible by the fence.
@@ -1227,8 +1278,13 @@ cudaError_t backward(const Maps& m, const AttnArgs& a, int heads, int kv_heads, 
     cudaError_t e = allow_smem<Dq>(dq);
     if (e == cudaSuccess) e = allow_smem<Dkv>(dkv);
     if (e != cudaSuccess) return e;
-    const unsigned blocks = (unsigned)(((unsigned long long)a.n_tokens * heads * 8 + DELTA_THREADS - 1) / DELTA_THREADS);
-    attention_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
+    if (attention_near(a.window)) {
+        const unsigned blocks = (a.n_tokens + DELTA_THREADS / 32 - 1) / (DELTA_THREADS / 32);
+        attention_near_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
+    } else {
+        const unsigned blocks = (unsigned)(((unsigned long long)a.n_tokens * heads * 8 + DELTA_THREADS - 1) / DELTA_THREADS);
+        attention_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
+    }
     e = cudaGetLastError();
     // The one with the longer items goes first, so that the other's fill the
     // places that it leaves: a key head's item goes through the queries of its

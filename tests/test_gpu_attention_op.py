@@ -137,7 +137,7 @@ def test_lengths_and_windows(lens, window, dtype, max_len):
 
 
 @pytest.mark.parametrize("hq,hk", [(1, 1), (3, 1), (6, 2), (12, 12), (12, 4)])
-@pytest.mark.parametrize("window", [-1, 17])
+@pytest.mark.parametrize("window", [-1, 17, 3])
 @kernels
 def test_head_groups(hq, hk, window, max_len):
     p = Problem([70, 129], hq=hq, hk=hk, window=window, seed=hq, max_len=max_len)
@@ -265,13 +265,14 @@ def test_more_short_sequences_than_blocks(hq, hk, window, masked):
     p.check()
 
 
+@pytest.mark.parametrize("lens", [[1] * 50 + [9, 64, 30], [20, 3], [200, 70, 1], [500] * 4])
 @pytest.mark.parametrize("dtype", ["BF16", "F16"])
-def test_one_key_has_no_gradient_through_its_score(dtype):
+def test_one_key_has_no_gradient_through_its_score(dtype, lens):
     """A query that sees one key has P = 1 whatever the score: dQ and dK are 0
     but for what exp(S - lse) is off 1. delta = P dP, so dS = P dP (1 - P);
     |1 - P| <= 2^-18 (S and lse below 2^3 in f32, each off by a few 2^-21), and
     |dP| <= 64 |dO| |V| < 64 * 25: |dQ| <= 0.125 * 1600 * 2^-18 * 5 < 2^-8."""
-    p = Problem([1] * 50 + [9, 64, 30], hq=3, hk=3, window=0, dtype=dtype)
+    p = Problem(lens, hq=3, hk=3, window=0, dtype=dtype)
     p.run()
     assert (p.dqkv[POISON:p.T - POISON, :2 * 3 * 64].abs() < 2.0 ** -8).all()
     p.check()
