@@ -19,7 +19,7 @@
 //
 // The bytes are logits, reference and gradient once each. On the device, f32
 // with a reference: 64 decisions of 4 options 2.1 us, a launch; 65,536 of 4 to
-// 16 (10.5 MB) 5.9 us, 1.8 TB/s; bf16, 16,384 of 1 to 1,024 (51 MB) 49 us, 1.1
+// 16 (10.5 MB) 6.2 us, 1.7 TB/s; bf16, 16,384 of 1 to 1,024 (51 MB) 49 us, 1.1
 // TB/s, bound by instructions (630 a warp, 3.1 of 4 a cycle issued): some 50 an
 // option, and as many again a decision for its scalars and three reductions.
 #include "operators.cuh"
