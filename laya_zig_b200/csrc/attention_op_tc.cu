@@ -836,6 +836,7 @@ __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a,
 // few, it took a third of an item's time at 175-180 tokens (dQ 80 -> 47 us
 // there, delta 8.6).
 constexpr int DELTA_THREADS = 256;
+constexpr int DELTA_ROWS = 4;  // of a thread, all loads under way at once
 
 template <typename T>
 __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const AttnArgs a, int heads) {
@@ -843,22 +844,33 @@ __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const At
     if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the two kernels that follow
     const int n = a.n_seqs;
     const int first = max(a.cu[0], 0), last = min(a.cu[n], a.n_tokens);  // rows past either are not the call's
-    const unsigned at = blockIdx.x * (DELTA_THREADS / 8) + threadIdx.x / 8;  // tokens times heads: below 2^32
     const int c = threadIdx.x & 7;
-    const int t = (int)(at / (unsigned)heads), h = (int)(at - (unsigned)t * heads);
-    const bool ok = t >= first && t < last && (!a.mask || a.mask[t] != 0);
-    float sum = 0.f;
-    if (ok) {
-        const uint4 o = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.out.p) + t * a.io.out.ld + h * 64 + c * 8);
-        const uint4 d = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.dout.p) + t * a.io.dout.ld + h * 64 + c * 8);
-        const T* x = reinterpret_cast<const T*>(&o);
-        const T* y = reinterpret_cast<const T*>(&d);
+    uint4 o[DELTA_ROWS], d[DELTA_ROWS];
+    long long to[DELTA_ROWS];
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum = fmaf(to_float(x[k]), to_float(y[k]), sum);
+    for (int i = 0; i < DELTA_ROWS; i++) {
+        // tokens times heads: below 2^32 with the last block's surplus
+        const unsigned at = (blockIdx.x * DELTA_ROWS + i) * (DELTA_THREADS / 8) + threadIdx.x / 8;
+        const int t = (int)(at / (unsigned)heads), h = (int)(at - (unsigned)t * heads);
+        to[i] = -1;
+        o[i] = d[i] = make_uint4(0, 0, 0, 0);
+        if (t >= first && t < last && (!a.mask || a.mask[t] != 0)) {
+            to[i] = (long long)h * a.n_tokens + t;
+            o[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.out.p) + t * a.io.out.ld + h * 64 + c * 8);
+            d[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.dout.p) + t * a.io.dout.ld + h * 64 + c * 8);
+        }
     }
 #pragma unroll
-    for (int k = 1; k < 8; k *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-    if (ok && c == 0) a.io.delta[(long long)h * a.n_tokens + t] = sum;
+    for (int i = 0; i < DELTA_ROWS; i++) {
+        const T* x = reinterpret_cast<const T*>(&o[i]);
+        const T* y = reinterpret_cast<const T*>(&d[i]);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum = fmaf(to_float(x[k]), to_float(y[k]), sum);
+#pragma unroll
+        for (int k = 1; k < 8; k *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        if (to[i] >= 0 && c == 0) a.io.delta[to[i]] = sum;
+    }
 }
 
 // The same for narrow windows, as the sum over P dP of the few keys: O, rounded to
@@ -1282,7 +1294,8 @@ cudaError_t backward(const Maps& m, const AttnArgs& a, int heads, int kv_heads, 
         const unsigned blocks = (a.n_tokens + DELTA_THREADS / 32 - 1) / (DELTA_THREADS / 32);
         attention_near_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
     } else {
-        const unsigned blocks = (unsigned)(((unsigned long long)a.n_tokens * heads * 8 + DELTA_THREADS - 1) / DELTA_THREADS);
+        const unsigned per = DELTA_THREADS / 8 * DELTA_ROWS;
+        const unsigned blocks = (unsigned)(((unsigned long long)a.n_tokens * heads + per - 1) / per);
         attention_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
     }
     e = cudaGetLastError();
