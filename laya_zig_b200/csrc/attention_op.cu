@@ -19,7 +19,7 @@
 // counts is the chain of dependent steps in one block (find the sequence, load,
 // two to five products of 16 x 8 x 16 instructions, exponentials, store), not
 // a rate. One sequence of 64 tokens, 12 heads, bf16: forward 4.2 us, backward
-// 4.5 us (a short kernel on its own takes 2.1 there). Backward in one launch
+// 4.5 us (a short kernel on its own takes 1.8 there). Backward in one launch
 // instead of a dQ launch followed by a dK/dV launch that reads its delta: 9.3
 // -> 5.1 us there; delta is recomputed from O, which a row's tile costs little.
 //
@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(THREADS, 3) attention_fwd_kernel(const AttnArg
     T* sv = sk + 2 * TILE;
     __shared__ uint32_t bits[2][2];
     SeqTile t;
+    griddep_begin();
     if (!block_tile(a, &t)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int h = blockIdx.y, hk = h / a.group;
@@ -504,6 +505,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS, 2) attention_bwd_kernel(const AttnArgs a, int n_heads) {
     extern __shared__ __align__(128) uint8_t smem[];
     SeqTile t;
+    griddep_begin();
     if (!block_tile(a, &t)) return;
     const int y = blockIdx.y;
     if (y < n_heads)
@@ -554,6 +556,7 @@ __global__ void __launch_bounds__(THREADS, 6) attention_fwd_one_kernel(const Att
     __shared__ uint32_t bits[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, hk = h / a.group;
     const float sl2 = a.scale * LOG2E;
+    griddep_begin();
     for (long long seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
         SeqTile t;
         if (!one_sequence(a, seq, &t)) continue;
@@ -638,6 +641,7 @@ __global__ void __launch_bounds__(THREADS, SHARED ? 3 : 4) attention_bwd_one_ker
     __shared__ uint32_t bits[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y;
     const float sl2 = a.scale * LOG2E;
+    griddep_begin();
     for (long long seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
         SeqTile t;
         if (!one_sequence(a, seq, &t)) continue;
@@ -767,8 +771,7 @@ static cudaError_t launch_one(void (*kernel)(AttnArgs), int smem, unsigned heads
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const unsigned most = (148 * 16 + heads - 1) / heads;
-    kernel<<<dim3((unsigned)g.n_seqs < most ? g.n_seqs : most, heads), THREADS, smem, stream>>>(g);
-    return cudaGetLastError();
+    return launch_k(kernel, dim3((unsigned)g.n_seqs < most ? g.n_seqs : most, heads), dim3(THREADS), smem, stream, g);
 }
 
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
@@ -780,8 +783,7 @@ cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cuda
     if (!small_call(a)) return launch_attention_fwd_tc(bf16, (int)a.n_heads, g, stream);
     auto kernel = bf16 ? attention_fwd_kernel<__nv_bfloat16> : attention_fwd_kernel<__half>;
     const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), a.n_heads);
-    kernel<<<grid, THREADS, FWD_SMEM, stream>>>(g);
-    return cudaGetLastError();
+    return launch_k(kernel, grid, dim3(THREADS), FWD_SMEM, stream, g);
 }
 
 cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream) {
@@ -799,8 +801,7 @@ cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cuda
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), a.n_heads + a.n_kv_heads);
-    kernel<<<grid, THREADS, BWD_SMEM, stream>>>(g, (int)a.n_heads);
-    return cudaGetLastError();
+    return launch_k(kernel, grid, dim3(THREADS), BWD_SMEM, stream, g, (int)a.n_heads);
 }
 
 }  // namespace laya

@@ -6,6 +6,15 @@
 
 namespace laya {
 
+// The kernels that use no tensor memory are launched by launch_k and start with
+// this: they are set up while the kernel before them ends. The next kernel is let
+// in only when that one is complete: one that allocates tensor memory before it
+// waits would otherwise keep it from a kernel two places back that has yet to.
+__device__ __forceinline__ void griddep_begin() {
+    griddep_wait();
+    griddep_launch();
+}
+
 // ------------------------------------------------------------------ offset tables
 // The largest s of [0, n) with key(s) <= x, by the whole warp: 32 probes a
 // round, so 1,024 entries take two dependent loads (a bisection takes ten).

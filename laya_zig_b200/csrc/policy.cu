@@ -18,8 +18,8 @@
 // after the first time from cache.
 //
 // The bytes are logits, reference and gradient once each. On the device, f32
-// with a reference: 64 decisions of 4 options 2.1 us, a launch; 65,536 of 4 to
-// 16 (10.5 MB) 6.2 us, 1.7 TB/s; bf16, 16,384 of 1 to 1,024 (51 MB) 49 us, 1.1
+// with a reference: 64 decisions of 4 options 1.8 us, a launch; 65,536 of 4 to
+// 16 (10.5 MB) 5.7 us, 1.8 TB/s; bf16, 16,384 of 1 to 1,024 (51 MB) 48 us, 1.1
 // TB/s, bound by instructions (630 a warp, 3.1 of 4 a cycle issued): some 50 an
 // option, and as many again a decision for its scalars and three reductions.
 #include "operators.cuh"
@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
     const long long at = (long long)blockIdx.x * (THREADS / G) + group;
     const bool live = at < s.n;
     const int i = live ? (int)at : s.n - 1;  // whole warps take part in the shuffles
+    griddep_begin();
     Decision d = load_decision<T>(s, io, i);
     if (live && !d.ok && l == 0) atomicOr(s.status, ERR_BAD_INDEX);
     const T* x = static_cast<const T*>(io.logits) + d.start;
@@ -249,6 +250,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
 template <typename T>
 __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyIO io) {
     __shared__ float2 buf[3][THREADS / 32];
+    griddep_begin();
     for (long long at = blockIdx.x; at < s.n; at += gridDim.x) {
         const int i = (int)at;
         Decision d = load_decision<T>(s, io, i);
@@ -303,11 +305,8 @@ template <typename T, int G, int V>
 cudaError_t launch_g(const Scalars& s, const PolicyIO& io, cudaStream_t stream) {
     constexpr int per = THREADS / G;
     const unsigned grid = (unsigned)(((long long)s.n + per - 1) / per);
-    if (io.ref)
-        policy_kernel<T, G, V, true><<<grid, THREADS, 0, stream>>>(s, io);
-    else
-        policy_kernel<T, G, V, false><<<grid, THREADS, 0, stream>>>(s, io);
-    return cudaGetLastError();
+    return launch_k(io.ref ? policy_kernel<T, G, V, true> : policy_kernel<T, G, V, false>, dim3(grid), dim3(THREADS), 0,
+                    stream, s, io);
 }
 
 template <typename T>
@@ -324,8 +323,7 @@ cudaError_t launch_t(const Scalars& s, const PolicyIO& io, cudaStream_t stream) 
     if (s.max_k <= 256) return launch_g<T, 32, 8>(s, io, stream);
     if (s.max_k <= 512) return launch_g<T, 32, 16>(s, io, stream);
     if (s.max_k <= 1024) return launch_g<T, THREADS, 8>(s, io, stream);
-    policy_wide_kernel<T><<<(unsigned)(s.n < 148 * 8 ? s.n : 148 * 8), THREADS, 0, stream>>>(s, io);
-    return cudaGetLastError();
+    return launch_k(policy_wide_kernel<T>, dim3((unsigned)(s.n < 148 * 8 ? s.n : 148 * 8)), dim3(THREADS), 0, stream, s, io);
 }
 
 }  // namespace
