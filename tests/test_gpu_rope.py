@@ -135,3 +135,53 @@ def test_broken_offsets_are_recorded(table):
     with pytest.raises(gpu.LayaError) as e:
         gpu.op_status(st.data_ptr())
     assert e.value.code == gpu.ERR_ARG
+
+
+def test_captured_between_streams_that_join():
+    """Behind a join of two streams in a captured graph, ahead of one and behind
+    a copy: the kernel waits for all that comes before it, and what follows waits
+    for the kernel."""
+    import torch
+    from laya_zig_b200 import gpu
+    x = torch.randn((64, 2304), device="cuda").to(torch.bfloat16)
+    y, z = torch.zeros_like(x), torch.zeros_like(x)
+    cu = torch.tensor([0, 64], dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    slow = torch.zeros(1 << 24, device="cuda")
+    plan = gpu.RopePlan()
+    s, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def rope():
+        gpu.rope(plan, z.data_ptr(), 2304, y.data_ptr(), 2304, 64, 24, status.data_ptr(), cu_seqlens_ptr=cu.data_ptr(),
+                 n_seqs=1, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        z.copy_(x)
+        rope()
+    torch.cuda.synchronize()
+    want = y.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        other.wait_stream(s)
+        with torch.cuda.stream(other):
+            slow.add_(1)
+            z.copy_(x)
+        y.zero_()
+        s.wait_stream(other)
+        rope()
+        first = y.clone()
+        other.wait_stream(s)
+        with torch.cuda.stream(other):
+            slow.add_(1)
+            z.zero_()
+        s.wait_stream(other)
+        rope()
+        second = y.clone()
+        z.copy_(x)
+        rope()
+    for _ in range(3):
+        y.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and (second[:, :24 * 64] == 0).all() and torch.equal(y, want)
+    gpu.op_status(status.data_ptr())
