@@ -22,10 +22,11 @@ constexpr uint32_t COLS = 256;
 
 constexpr int STAGE_BYTES = 2048;  // staging for a softmax warp's stores
 
-// Of one kernel: 128-row tiles, floats besides.
-template <int BIGS_, int EXTRA_>
+// Of one kernel: 128-row tiles, floats besides, passes over the call's items (each
+// has barriers of its own).
+template <int BIGS_, int EXTRA_, int PASSES_ = 1>
 struct Shape {
-    static constexpr int BIGS = BIGS_, EXTRA = EXTRA_;
+    static constexpr int BIGS = BIGS_, EXTRA = EXTRA_, PASSES = PASSES_;
 };
 
 // What the loading warp found; n < 0: there is no further item.
@@ -85,12 +86,13 @@ __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, int* er
     }
 }
 
-// The same for a CTA that leaves: whatever the abort word says.
-__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err) {
+// The same at the end of a pass, whatever the abort word says.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err, int* abort) {
     const unsigned long long t0 = globaltimer();
     while (!mbar_try_wait(bar, parity))
         if (globaltimer() - t0 > WAIT_LIMIT_NS) {
             atomicOr(err, ERR_WAIT_TIMEOUT);
+            *(volatile int*)abort = 1;
             return;
         }
 }
@@ -120,7 +122,8 @@ struct Loader {
         if (patch < 0) return;
         Bars* bar = f.bar;
         const uint32_t parity = landed_parity >> patch & 1;
-        if (!wait_one(&bar->landed[patch], parity, a.status, &bar->abort)) drain(&bar->landed[patch], parity, a.status);
+        if (!wait_one(&bar->landed[patch], parity, a.status, &bar->abort))
+            drain(&bar->landed[patch], parity, a.status, &bar->abort);
         landed_parity ^= 1u << patch;
         uint8_t* s = f.ring + patch * 2 * SMALL;
         const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -188,8 +191,10 @@ struct Loader {
     // items the 128-row tiles were asked for.
     __device__ __forceinline__ void finish(int big) {
         fill();
-        for (int j = max(0, issued - STAGES); j < issued; j++) drain(&f.bar->full[j % STAGES], (j / STAGES) & 1, a.status);
-        if (big > 0) drain(&f.bar->big_full, (big - 1) & 1, a.status);
+        int* abort = &f.bar->abort;
+        for (int j = max(0, issued - STAGES); j < issued; j++)
+            drain(&f.bar->full[j % STAGES], (j / STAGES) & 1, a.status, abort);
+        if (big > 0) drain(&f.bar->big_full, (big - 1) & 1, a.status, abort);
     }
 };
 

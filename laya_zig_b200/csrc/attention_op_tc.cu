@@ -36,9 +36,9 @@
 // unit: on one sequence of 8,192 tokens, 12 heads, the SFU is busy 64 % of the
 // forward's time (512 cycles of ex2 for a 128 x 64 tile), 53 % of dQ's and 46 %
 // of dK/dV's, the tensor cores 32, 39 and 46 %, and issue slots 54 % at most.
-// There the forward takes 340 us (606 TFLOP/s) and the backward 760 (678 over
-// the five products needed, 949 over the seven that it does); 64 sequences of
-// 175-180 tokens 31 and 76 us, where an item has three tiles: of an item's 10,500
+// There the forward takes 340 us (606 TFLOP/s) and the backward 790 (652 over
+// the five products needed, 913 over the seven that it does); 64 sequences of
+// 175-180 tokens 31 and 72 us, where an item has three tiles: of an item's 10,500
 // cycles in dK/dV these take 6,000, waiting for the accumulators 800, storing them
 // 2,500 and the next item's beginning 600 (forward: 6,200, of them 3,500 in tiles);
 // 2 of 16,000 with a window of 64 (forward) 71 us. The mma.sync kernels took 3,619
@@ -65,7 +65,7 @@ namespace {
 
 template <typename C>
 constexpr int smem_bytes() {
-    return C::BIGS * BIG + STAGES * 2 * SMALL + 8 * STAGE_BYTES + C::EXTRA * 4 + (int)sizeof(Bars) +
+    return C::BIGS * BIG + STAGES * 2 * SMALL + 8 * STAGE_BYTES + C::EXTRA * 4 + C::PASSES * (int)sizeof(Bars) +
            (int)sizeof(Slots) + 1024;
 }
 
@@ -317,31 +317,32 @@ __device__ __forceinline__ Frame open_frame(uint8_t* raw, int warp) {
     f.stage = f.ring + STAGES * 2 * SMALL;
     f.extra = reinterpret_cast<float*>(f.stage + 8 * STAGE_BYTES);
     f.bar = reinterpret_cast<Bars*>(f.extra + C::EXTRA);
-    f.slots = reinterpret_cast<Slots*>(f.bar + 1);
+    f.slots = reinterpret_cast<Slots*>(f.bar + C::PASSES);
     f.stage += (warp & 7) * STAGE_BYTES;
     if (threadIdx.x == 0) {
-        Bars* b = f.bar;
-        for (int s = 0; s < STAGES; s++) {
-            mbar_init(&b->full[s], 33);
-            mbar_init(&b->empty[s], 1);
-            mbar_init(&b->landed[s], 1);
+        for (Bars* b = f.bar; b < f.bar + C::PASSES; b++) {
+            for (int s = 0; s < STAGES; s++) {
+                mbar_init(&b->full[s], 33);
+                mbar_init(&b->empty[s], 1);
+                mbar_init(&b->landed[s], 1);
+            }
+            mbar_init(&b->big_full, 1);
+            mbar_init(&b->big_empty, 1);
+            for (int s = 0; s < 2; s++) {
+                mbar_init(&b->item_full[s], 32);
+                mbar_init(&b->item_empty[s], SOFTMAX + 1);
+                mbar_init(&b->s_full[s], 2);  // the product, and the MMA lane on what the stage holds besides
+                mbar_init(&b->dp_full[s], 1);
+                mbar_init(&b->s_read[s], SOFTMAX);
+                mbar_init(&b->p_full[s], SOFTMAX);
+                mbar_init(&b->done[s], 1);
+                mbar_init(&b->acc_full[s], 1);
+                mbar_init(&b->acc_free[s], SOFTMAX);
+            }
+            mbar_init(&b->sync, SOFTMAX);
+            mbar_init(&b->drained, 1);
+            b->abort = 0;
         }
-        mbar_init(&b->big_full, 1);
-        mbar_init(&b->big_empty, 1);
-        for (int s = 0; s < 2; s++) {
-            mbar_init(&b->item_full[s], 32);
-            mbar_init(&b->item_empty[s], SOFTMAX + 1);
-            mbar_init(&b->s_full[s], 2);  // the product, and the MMA lane on what the stage holds besides
-            mbar_init(&b->dp_full[s], 1);
-            mbar_init(&b->s_read[s], SOFTMAX);
-            mbar_init(&b->p_full[s], SOFTMAX);
-            mbar_init(&b->done[s], 1);
-            mbar_init(&b->acc_full[s], 1);
-            mbar_init(&b->acc_free[s], SOFTMAX);
-        }
-        mbar_init(&b->sync, SOFTMAX);
-        mbar_init(&b->drained, 1);
-        b->abort = 0;
         fence_barrier_init();
         fence_proxy_async();
     }
@@ -362,6 +363,17 @@ __device__ __forceinline__ void close_frame(const Frame& f, int warp) {
     __syncthreads();
     tc_fence_after();
     if (warp == MMA) tmem_dealloc(f.tmem, COLS);
+}
+
+// From one pass to the next: its copies and MMAs are complete, and everyone is
+// done with shared memory and TMEM. False in a CTA that gave up.
+__device__ __forceinline__ bool next_pass(Frame& f) {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*(volatile int*)&f.bar->abort) return false;
+    f.bar++;
+    return true;
 }
 
 // The MMA lane's waits.
@@ -467,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 c += n;
             }
             tc_commit(&bar->drained);
-            drain(&bar->drained, 0, a.status);
+            drain(&bar->drained, 0, a.status, &bar->abort);
         }
         __syncwarp();
     } else {
@@ -632,7 +644,7 @@ __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a,
         c += n;
     }
     tc_commit(&bar->drained);
-    drain(&bar->drained, 0, a.status);
+    drain(&bar->drained, 0, a.status, &bar->abort);
 }
 
 // ------------------------------------------------------------------ delta
@@ -646,7 +658,7 @@ constexpr int DELTA_ROWS = 4;  // of a thread, all loads under way at once
 template <typename T>
 __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const AttnArgs a, int heads) {
     griddep_launch();
-    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the two kernels that follow
+    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the passes that follow
     const int n = a.n_seqs;
     const int first = max(a.cu[0], 0), last = min(a.cu[n], a.n_tokens);  // rows past either are not the call's
     const int c = threadIdx.x & 7;
@@ -687,7 +699,7 @@ __global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const At
 template <typename T>
 __global__ void __launch_bounds__(DELTA_THREADS) attention_near_delta_kernel(const AttnArgs a, int heads) {
     griddep_launch();
-    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the two kernels that follow
+    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the passes that follow
     const int lane = threadIdx.x & 31, c = (lane & 7) * 8;
     const long long t = (long long)blockIdx.x * (DELTA_THREADS / 32) + (threadIdx.x >> 5);
     if (t >= a.n_tokens) return;
@@ -727,42 +739,15 @@ __global__ void __launch_bounds__(DELTA_THREADS) attention_near_delta_kernel(con
     }
 }
 
-// dQ and dK/dV use nothing of one another. The first of them waits for delta
-// and the counters; then the second one's CTAs may take the places of its CTAs
-// as these come free, with what was complete there made visible by the fence.
-// The second waits for the first before it ends: what follows it in the stream
-// follows both.
-__device__ __forceinline__ void open_pass(bool first) {
-    if (!first) return;
-    griddep_wait();
-    __threadfence();
-    griddep_launch();
-}
-__device__ __forceinline__ void close_pass(bool first) {
-    if (!first) griddep_wait();
-}
-
 // ------------------------------------------------------------------ dQ
 // TMEM: S at columns 0, 64 (dP over it, dS over that, 8 columns of every 16);
 // dQ at 128, the next item's at 192. extra: -lse * log2 e and -delta of the rows
 // of two items in turn.
-using Dq = Shape<2, 4 * ROWS>;
-
 template <typename T, typename C>
-__global__ void __launch_bounds__(THREADS, CTAS)
-    attention_dq_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                           const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
-                           const AttnArgs a, int heads, bool first) {
-    extern __shared__ uint8_t raw[];
+__device__ __forceinline__ void dq_pass(const Frame& f, const CUtensorMap& mq, const CUtensorMap& mk,
+                                        const CUtensorMap& mv, const CUtensorMap& mdo, const AttnArgs& a, int heads) {
+    static_assert(C::EXTRA >= 4 * ROWS, "the rows' statistics");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == LOADER * 32) {
-        prefetch_tmap(&mq);
-        prefetch_tmap(&mk);
-        prefetch_tmap(&mv);
-        prefetch_tmap(&mdo);
-    }
-    const Frame f = open_frame<C>(raw, warp);
-    open_pass(first);
     Walk walk(a, heads, lane, warp == LOADER, a.io.tickets);
     Bars* bar = f.bar;
 
@@ -883,31 +868,17 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             mbar_arrive(&bar->item_empty[k & 1]);
         }
     }
-    close_frame<C>(f, warp);
-    close_pass(first);
 }
 
 // ------------------------------------------------------------------ dK, dV
 // TMEM: S^T at columns 0, 64 (dP^T over it, P^T and dS^T over
 // that, 8 columns of each in turn); dV at 128; dK at 192. extra: -lse * log2 e
 // and -delta of each stage's queries.
-using Dkv = Shape<2, 2 * STAGES * STEP>;
-
 template <typename T, typename C>
-__global__ void __launch_bounds__(THREADS, CTAS)
-    attention_dkv_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
-                            const AttnArgs a, int heads, bool first) {
-    extern __shared__ uint8_t raw[];
+__device__ __forceinline__ void dkv_pass(const Frame& f, const CUtensorMap& mq, const CUtensorMap& mk,
+                                         const CUtensorMap& mv, const CUtensorMap& mdo, const AttnArgs& a, int heads) {
+    static_assert(C::EXTRA >= 2 * STAGES * STEP, "the stages' statistics");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == LOADER * 32) {
-        prefetch_tmap(&mq);
-        prefetch_tmap(&mk);
-        prefetch_tmap(&mv);
-        prefetch_tmap(&mdo);
-    }
-    const Frame f = open_frame<C>(raw, warp);
-    open_pass(first);
     Walk walk(a, heads, lane, warp == LOADER, a.io.tickets + 1);
     Bars* bar = f.bar;
 
@@ -1047,8 +1018,37 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             mbar_arrive(&bar->item_empty[k & 1]);
         }
     }
+}
+
+// ------------------------------------------------------------------ backward
+// Both passes in one launch, whose CTAs go from dK/dV's items to dQ's as they come
+// free: the passes use nothing of one another, and all that they share (delta, the
+// counters) is complete when the CTA's wait returns. The longer items go first: a
+// key head's item goes through the queries of its whole group. (As two launches,
+// the second one's CTAs in the places of the first's, dQ first unless heads are
+// shared: 64 x 175-180 tokens, 12 heads 76 us instead of 72, 128 x 1-512, 12 heads
+// over 4 288 instead of 284, one sequence of 8,192 760 instead of 790; but there the
+// second launch has no wait of its own behind which delta is known to be complete.)
+using Bwd = Shape<2, 4 * ROWS, 2>;
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(THREADS, CTAS)
+    attention_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
+                            const AttnArgs a, int heads, int kv_heads) {
+    extern __shared__ uint8_t raw[];
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == LOADER * 32) {
+        prefetch_tmap(&mq);
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+        prefetch_tmap(&mdo);
+    }
+    Frame f = open_frame<C>(raw, warp);
+    griddep_wait();
+    dkv_pass<T, C>(f, mq, mk, mv, mdo, a, kv_heads);
+    if (next_pass(f)) dq_pass<T, C>(f, mq, mk, mv, mdo, a, heads);
     close_frame<C>(f, warp);
-    close_pass(first);
 }
 
 
@@ -1090,10 +1090,8 @@ cudaError_t forward(const Maps& m, const AttnArgs& a, int heads, cudaStream_t st
 
 template <typename T>
 cudaError_t backward(const Maps& m, const AttnArgs& a, int heads, int kv_heads, cudaStream_t stream) {
-    const auto dq = attention_dq_tc_kernel<T, Dq>;
-    const auto dkv = attention_dkv_tc_kernel<T, Dkv>;
-    cudaError_t e = allow_smem<Dq>(dq);
-    if (e == cudaSuccess) e = allow_smem<Dkv>(dkv);
+    const auto kernel = attention_bwd_tc_kernel<T, Bwd>;
+    cudaError_t e = allow_smem<Bwd>(kernel);
     if (e != cudaSuccess) return e;
     if (attention_near(a.window)) {
         const unsigned blocks = (a.n_tokens + DELTA_THREADS / 32 - 1) / (DELTA_THREADS / 32);
@@ -1104,19 +1102,9 @@ cudaError_t backward(const Maps& m, const AttnArgs& a, int heads, int kv_heads, 
         attention_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
     }
     e = cudaGetLastError();
-    // The one with the longer items goes first, so that the other's fill the
-    // places that it leaves: a key head's item goes through the queries of its
-    // whole group (128 x 1-512 tokens, 12 heads over 4: 288 us, 303 the other way
-    // round; one sequence of 8,192, 12 heads: 797 with dK and dV first, 765).
-    const bool dkv_first = a.group > 1;
-    for (int i = 0; i < 2 && e == cudaSuccess; i++) {
-        if ((i == 0) == dkv_first)
-            e = launch_k(dkv, dim3(ctas(a, kv_heads)), THREADS, smem_bytes<Dkv>(), stream, m.q, m.k, m.v, m.dout, a, kv_heads,
-                         i == 0);
-        else
-            e = launch_k(dq, dim3(ctas(a, heads)), THREADS, smem_bytes<Dq>(), stream, m.q, m.k, m.v, m.dout, a, heads, i == 0);
-    }
-    return e;
+    if (e != cudaSuccess) return e;
+    return launch_k(kernel, dim3(ctas(a, heads)), THREADS, smem_bytes<Bwd>(), stream, m.q, m.k, m.v, m.dout, a, heads,
+                    kv_heads);
 }
 
 }  // namespace
