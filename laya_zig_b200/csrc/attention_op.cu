@@ -5,7 +5,8 @@
 // pass over the keys), out = O / l and lse = m + log l.
 //
 // Backward, with the probabilities recomputed as P = exp(S - lse):
-//   delta_i = sum_d dO_id O_id            (= sum_j P_ij dP_ij)
+//   delta_i = sum_d dO_id O_id            (= sum_j P_ij dP_ij, which rows with few
+//                                          keys take: attention_op_delta.cu)
 //   dP = dO V^T,  dS = P (dP - delta)
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
 // One launch, without atomics: a block per query tile walks the keys for dQ, a
@@ -34,6 +35,8 @@
 // they hold enters a product: zero rows of Q and dO add nothing to dK and dV,
 // zero rows of K nothing to dQ, and the scores of such keys are masked where
 // the softmax sums them.
+#include <type_traits>
+
 #include "attention_op.cuh"
 
 namespace laya {
@@ -42,6 +45,7 @@ namespace {
 constexpr int TB = 64;  // rows per tile
 constexpr int THREADS = 128;
 constexpr int TILE = TB * 64;  // elements
+constexpr int SMALL_LEN = 512;  // tokens of the longest sequence of a small call
 
 // element offset of (row, col) in a 64 x 64 16-bit tile whose 16-byte chunks
 // are XORed by row: ldmatrix row fetches never share a bank
@@ -56,25 +60,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(smem_u32(p)));
-}
-
-template <typename T>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Rows row0 .. row0 + 63 of the sequence (the first n times 16 of them), 64
@@ -335,8 +320,73 @@ __device__ __forceinline__ void tile_delta(float* sdelta, const T* so, const T* 
     if ((threadIdx.x & 1) == 0) sdelta[r] = acc;
 }
 
+// Which rows of a small call's sequence are there and which of them see FEW keys at
+// most (absent tokens can leave them so few), a bit each.
+struct RowBits {
+    uint32_t there[SMALL_LEN / 32], few[SMALL_LEN / 32];
+};
+
+// few is to be read behind another barrier.
+__device__ __forceinline__ void find_few(RowBits* bits, const AttnArgs& a, const SeqTile& t) {
+    for (int i = threadIdx.x; i - (int)threadIdx.x < t.len; i += THREADS) {
+        const uint32_t b = __ballot_sync(0xffffffffu, present(a, t, i));
+        if ((threadIdx.x & 31) == 0) bits->there[i >> 5] = b;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i - (int)threadIdx.x < t.len; i += THREADS) {
+        bool f = bits->there[i >> 5] >> (i & 31) & 1;
+        if (f) {
+            int lo, hi, count = 0;
+            span(a, t, i, &lo, &hi);
+            for (int w = lo >> 5; w <= hi >> 5 && count <= FEW; w++) {
+                uint32_t keys = bits->there[w];
+                if (w == lo >> 5) keys &= ~0u << (lo & 31);
+                if (w == hi >> 5) keys &= ~0u >> (31 - (hi & 31));
+                count += __popc(keys);
+            }
+            f = count <= FEW;
+        }
+        const uint32_t b = __ballot_sync(0xffffffffu, f);
+        if ((threadIdx.x & 31) == 0) bits->few[i >> 5] = b;
+    }
+}
+__device__ __forceinline__ bool any_few(const RowBits* bits, int row0) {
+    return (bits->few[row0 >> 5] | bits->few[(row0 >> 5) + 1]) != 0;
+}
+
+// Their delta, of rows row0 .. row0 + 63 and one head, from P dP: eight lanes to a row.
 template <typename T>
-__device__ __forceinline__ void dq_block(const AttnArgs& a, const SeqTile& t, int h, uint8_t* smem) {
+__device__ __forceinline__ void few_delta(float* sdelta, const RowBits* bits, const AttnArgs& a, const SeqTile& t,
+                                          int h, int row0) {
+    const int lane = threadIdx.x & 31, l = lane & 7, c = l * 8, hk = h / a.group;
+    const uint32_t group = 0xffu << (lane & 24);
+    for (int r = threadIdx.x >> 3; r < TB; r += THREADS / 8) {
+        const int i = row0 + r;
+        if (!(bits->few[i >> 5] >> (i & 31) & 1)) continue;
+        const uint4 q = piece<T>(a.io.q, t.start + i, h, c), d = piece<T>(a.io.dout, t.start + i, h, c);
+        const float e = a.io.lse[(long long)h * a.n_tokens + t.start + i] * LOG2E;
+        float sum = 0.f;
+        int lo, hi;
+        span(a, t, i, &lo, &hi);
+        for (int j = lo; j <= hi; j += 8) {
+            uint32_t keys = __ballot_sync(group, j + l <= hi && present(a, t, j + l)) >> (lane & 24);
+            for (; keys; keys &= keys - 1) {
+                const long long at = t.start + j + __ffs(keys) - 1;
+                float s = dot8<T>(q, piece<T>(a.io.k, at, hk, c)), dp = dot8<T>(d, piece<T>(a.io.v, at, hk, c));
+#pragma unroll
+                for (int x = 1; x < 8; x *= 2) {
+                    s += __shfl_xor_sync(group, s, x);
+                    dp += __shfl_xor_sync(group, dp, x);
+                }
+                sum = fmaf(ex2_approx(fmaf(s, a.scale * LOG2E, -e)), dp, sum);
+            }
+        }
+        if (l == 0) sdelta[r] = sum;
+    }
+}
+
+template <typename T, bool MASKED>
+__device__ __forceinline__ void dq_block(const AttnArgs& a, const SeqTile& t, int h, uint8_t* smem, RowBits* rows) {
     T* sq = reinterpret_cast<T*>(smem);
     T* sdo = sq + TILE;
     T* sk = sdo + TILE;
@@ -355,10 +405,15 @@ __device__ __forceinline__ void dq_block(const AttnArgs& a, const SeqTile& t, in
     load_tile(sv, a.io.v, hk, a, t, kt0 * TB);
     key_bits(bits[0], a, t, kt0 * TB);
     copy_commit();
+    if (MASKED) find_few(rows, a, t);
     copy_wait<0>();
     __syncthreads();
     tile_delta(sdelta, so, sdo);
     __syncthreads();
+    if (MASKED && any_few(rows, t.row0)) {
+        few_delta<T>(sdelta, rows, a, t, h, t.row0);
+        __syncthreads();
+    }
     const float sl2 = a.scale * LOG2E;
     const int i0 = t.row0 + warp * 16 + (lane >> 2), i1 = i0 + 8;
     const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
@@ -411,8 +466,8 @@ __device__ __forceinline__ void dq_block(const AttnArgs& a, const SeqTile& t, in
     store_rows<T>(sq, a.io.dq, h, t, t.row0, warp, lane, dq, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
 }
 
-template <typename T>
-__device__ __forceinline__ void dkv_block(const AttnArgs& a, const SeqTile& t, int hk, uint8_t* smem) {
+template <typename T, bool MASKED>
+__device__ __forceinline__ void dkv_block(const AttnArgs& a, const SeqTile& t, int hk, uint8_t* smem, RowBits* rows) {
     T* sk = reinterpret_cast<T*>(smem);
     T* sv = sk + TILE;
     T* sq = sv + TILE;
@@ -440,6 +495,7 @@ __device__ __forceinline__ void dkv_block(const AttnArgs& a, const SeqTile& t, i
     load_tile(sv, a.io.v, hk, a, t, t.row0);
     load_q(0, 0);
     copy_commit();
+    if (MASKED) find_few(rows, a, t);  // read behind the loop's first barrier
     const float sl2 = a.scale * LOG2E;
     const int j0 = t.row0 + warp * 16 + (lane >> 2), j1 = j0 + 8;
     uint32_t ka[4][4], va[4][4];
@@ -458,6 +514,10 @@ __device__ __forceinline__ void dkv_block(const AttnArgs& a, const SeqTile& t, i
         }
         tile_delta(sdelta, so + b * TILE, sdo + b * TILE);  // read behind the barrier below
         const int row0 = (qt0 + it % nqt) * TB;
+        if (MASKED && any_few(rows, row0)) {
+            __syncthreads();
+            few_delta<T>(sdelta, rows, a, t, hk * a.group + it / nqt, row0);
+        }
         // transposed: rows are keys, columns queries
         float s[8][4], dp[8][4];
         mma_nt<T>(s, ka, sq + b * TILE, lane);
@@ -497,21 +557,6 @@ __device__ __forceinline__ void dkv_block(const AttnArgs& a, const SeqTile& t, i
     const bool p0 = present(a, t, j0), p1 = present(a, t, j1);
     store_rows<T>(sk, a.io.dk, hk, t, t.row0, warp, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
     store_rows<T>(sv, a.io.dv, hk, t, t.row0, warp, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
-}
-
-constexpr int BWD_SMEM = 8 * TILE * 2 + 3 * TB * 4;
-
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) attention_bwd_kernel(const AttnArgs a, int n_heads) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    SeqTile t;
-    griddep_begin();
-    if (!block_tile(a, &t)) return;
-    const int y = blockIdx.y;
-    if (y < n_heads)
-        dq_block<T>(a, t, y, smem);
-    else
-        dkv_block<T>(a, t, y - n_heads, smem);
 }
 
 // ------------------------------------------------------------------ short sequences
@@ -620,17 +665,15 @@ __global__ void __launch_bounds__(THREADS, 6) attention_fwd_one_kernel(const Att
 
 // The backward pass, all of a sequence and key head in one block.
 // S and dP are computed once, five products instead of seven; delta is the sum
-// over P dP, which is all there, in f32 (from O, rounded to 16 bits, it is off by
-// up to half a step of sum |dO O|, which dQ and dK of a few keys then show: 1.8
-// times the error of a 32-bit pass rounded once at 2 keys, 1.4 at 32 and more).
+// over P dP, which is all there, in f32 (attention_op_delta.cu says what that is
+// worth).
 template <bool SHARED>
 constexpr int ONE_SMEM = (SHARED ? 7 : 6) * TILE * 2;
 
 // SHARED: several query heads to a key head, whose dK and dV are then held
 // while the next one's scores are computed: fewer blocks to an SM.
 template <typename T, bool SHARED>
-__global__ void __launch_bounds__(THREADS, SHARED ? 3 : 4) attention_bwd_one_kernel(const AttnArgs a) {
-    extern __shared__ __align__(128) uint8_t smem[];
+__device__ __forceinline__ void one_block(const AttnArgs& a, const SeqTile& t, int hk, uint8_t* smem) {
     T* sk = reinterpret_cast<T*>(smem);
     T* sv = sk + TILE;
     T* sq = sv + TILE;
@@ -639,89 +682,123 @@ __global__ void __launch_bounds__(THREADS, SHARED ? 3 : 4) attention_bwd_one_ker
     T* sds = sp + TILE;
     T* sdq = SHARED ? sds + TILE : sv;  // V is not needed again when it has one query head
     __shared__ uint32_t bits[2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float sl2 = a.scale * LOG2E;
-    griddep_begin();
-    for (long long seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
-        SeqTile t;
-        if (!one_sequence(a, seq, &t)) continue;
-        const int n = (t.len + 15) >> 4;
-        const int i0 = warp * 16 + (lane >> 2), i1 = i0 + 8;  // this thread's queries, then keys
-        const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
-        load_tile(sk, a.io.k, hk, a, t, 0, n);
-        load_tile(sv, a.io.v, hk, a, t, 0, n);
-        key_bits(bits, a, t, 0);
-        float dk[8][4], dv[8][4];
-        if (SHARED) {
-            clear(dk);
-            clear(dv);
-        }
-        int h = hk * a.group;
-        do {
-            load_tile(sq, a.io.q, h, a, t, 0, n);
-            load_tile(sdo, a.io.dout, h, a, t, 0, n);
-            copy_commit();
-            const float* lse = a.io.lse + (long long)h * a.n_tokens + t.start;
-            const float e0 = p0 ? lse[i0] * LOG2E : 0.f, e1 = p1 ? lse[i1] * LOG2E : 0.f;
-            copy_wait<0>();
-            __syncthreads();
-            float dp[8][4];  // later dQ
-            if (warp < n) {
-                uint32_t f[4][4];
-                float s[8][4];
-                load_a(f, sq, warp, lane);
-                mma_nt<T>(s, f, sk, lane, n);
-                load_a(f, sdo, warp, lane);
-                mma_nt<T>(dp, f, sv, lane, n);
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        s[j][e] = ex2_approx(fmaf(s[j][e], sl2, -e0));
-                        s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -e1));
-                    }
-                hide(s, bits[0] | (uint64_t)bits[1] << 32, a.window, i0, i1, lane, 0.f);
-                float d0 = 0.f, d1 = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        d0 = fmaf(s[j][e], dp[j][e], d0);
-                        d1 = fmaf(s[j][2 + e], dp[j][2 + e], d1);
-                    }
-                put_rows<T>(sp, s, warp, lane);
-#pragma unroll
-                for (int x = 1; x < 4; x *= 2) {
-                    d0 += __shfl_xor_sync(0xffffffffu, d0, x);
-                    d1 += __shfl_xor_sync(0xffffffffu, d1, x);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        s[j][e] *= dp[j][e] - d0;
-                        s[j][2 + e] *= dp[j][2 + e] - d1;
-                    }
-                put_rows<T>(sds, s, warp, lane);
-                clear(dp);
-                mma_nn<T>(dp, s, sk, lane, n);
-            }
-            __syncthreads();
-            if (warp < n) store_rows<T>(sdq, a.io.dq, h, t, 0, warp, lane, dp, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
-            if (!SHARED) {
+            const int n = (t.len + 15) >> 4;
+            const int i0 = warp * 16 + (lane >> 2), i1 = i0 + 8;  // this thread's queries, then keys
+            const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
+            load_tile(sk, a.io.k, hk, a, t, 0, n);
+            load_tile(sv, a.io.v, hk, a, t, 0, n);
+            key_bits(bits, a, t, 0);
+            float dk[8][4], dv[8][4];
+            if (SHARED) {
                 clear(dk);
                 clear(dv);
             }
+            int h = hk * a.group;
+            do {
+                load_tile(sq, a.io.q, h, a, t, 0, n);
+                load_tile(sdo, a.io.dout, h, a, t, 0, n);
+                copy_commit();
+                const float* lse = a.io.lse + (long long)h * a.n_tokens + t.start;
+                const float e0 = p0 ? lse[i0] * LOG2E : 0.f, e1 = p1 ? lse[i1] * LOG2E : 0.f;
+                copy_wait<0>();
+                __syncthreads();
+                float dp[8][4];  // later dQ
+                if (warp < n) {
+                    uint32_t f[4][4];
+                    float s[8][4];
+                    load_a(f, sq, warp, lane);
+                    mma_nt<T>(s, f, sk, lane, n);
+                    load_a(f, sdo, warp, lane);
+                    mma_nt<T>(dp, f, sv, lane, n);
+    #pragma unroll
+                    for (int j = 0; j < 8; j++)
+    #pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            s[j][e] = ex2_approx(fmaf(s[j][e], sl2, -e0));
+                            s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -e1));
+                        }
+                    hide(s, bits[0] | (uint64_t)bits[1] << 32, a.window, i0, i1, lane, 0.f);
+                    float d0 = 0.f, d1 = 0.f;
+    #pragma unroll
+                    for (int j = 0; j < 8; j++)
+    #pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            d0 = fmaf(s[j][e], dp[j][e], d0);
+                            d1 = fmaf(s[j][2 + e], dp[j][2 + e], d1);
+                        }
+                    put_rows<T>(sp, s, warp, lane);
+    #pragma unroll
+                    for (int x = 1; x < 4; x *= 2) {
+                        d0 += __shfl_xor_sync(0xffffffffu, d0, x);
+                        d1 += __shfl_xor_sync(0xffffffffu, d1, x);
+                    }
+    #pragma unroll
+                    for (int j = 0; j < 8; j++)
+    #pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            s[j][e] *= dp[j][e] - d0;
+                            s[j][2 + e] *= dp[j][2 + e] - d1;
+                        }
+                    put_rows<T>(sds, s, warp, lane);
+                    clear(dp);
+                    mma_nn<T>(dp, s, sk, lane, n);
+                }
+                __syncthreads();
+                if (warp < n) store_rows<T>(sdq, a.io.dq, h, t, 0, warp, lane, dp, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+                if (!SHARED) {
+                    clear(dk);
+                    clear(dv);
+                }
+                if (warp < n) {
+                    mma_tn<T>(dv, sp, sdo, warp, lane, n);
+                    mma_tn<T>(dk, sds, sq, warp, lane, n);
+                }
+                __syncthreads();
+            } while (SHARED && ++h < (hk + 1) * a.group);
             if (warp < n) {
-                mma_tn<T>(dv, sp, sdo, warp, lane, n);
-                mma_tn<T>(dk, sds, sq, warp, lane, n);
+                store_rows<T>(sds, a.io.dk, hk, t, 0, warp, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+                store_rows<T>(sp, a.io.dv, hk, t, 0, warp, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
             }
-            __syncthreads();
-        } while (SHARED && ++h < (hk + 1) * a.group);
-        if (warp < n) {
-            store_rows<T>(sds, a.io.dk, hk, t, 0, warp, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
-            store_rows<T>(sp, a.io.dv, hk, t, 0, warp, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
-        }
+}
+
+template <typename T, bool SHARED>
+__global__ void __launch_bounds__(THREADS, SHARED ? 3 : 4) attention_bwd_one_kernel(const AttnArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    griddep_begin();
+    for (long long seq = blockIdx.x; seq < a.n_seqs; seq += gridDim.x) {
+        SeqTile t;
+        if (one_sequence(a, seq, &t)) one_block<T, SHARED>(a, t, blockIdx.y, smem);
+    }
+}
+
+// ------------------------------------------------------------------ backward of a little work
+constexpr int BWD_SMEM = 8 * TILE * 2 + 3 * TB * 4;
+static_assert(BWD_SMEM >= ONE_SMEM<true>, "a short sequence's block");
+
+// (inlined it would take registers from the longer ones' code)
+template <typename T>
+__device__ __noinline__ void short_sequence(const AttnArgs& a, const SeqTile& t, int hk, uint8_t* smem) {
+    one_block<T, true>(a, t, hk, smem);
+}
+
+template <typename T, bool MASKED>
+__global__ void __launch_bounds__(THREADS, 2)
+    attention_bwd_kernel(const __grid_constant__ AttnArgs a, int n_heads) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ typename std::conditional<MASKED, RowBits, int>::type bits;
+    RowBits* rows = reinterpret_cast<RowBits*>(&bits);
+    SeqTile t;
+    griddep_begin();
+    if (!block_tile(a, &t)) return;
+    const int y = blockIdx.y;
+    if (t.len <= SHORT) {  // delta from P dP, whatever the call holds besides
+        if (y >= n_heads) short_sequence<T>(a, t, y - n_heads, smem);
+    } else if (y < n_heads) {
+        dq_block<T, MASKED>(a, t, y, smem, rows);
+    } else {
+        dkv_block<T, MASKED>(a, t, y - n_heads, smem, rows);
     }
 }
 
@@ -737,6 +814,7 @@ AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
     g.window = a.window;
     g.scale = a.scale;
     g.io = io;
+    if (a.token_mask || narrow(a.window)) g.io.delta_short = io.delta;  // one kernel deals with all rows there
     return g;
 }
 
@@ -750,19 +828,18 @@ AttnArgs make_args(const laya_attention& a, const AttnIO& io) {
 // tcgen05: 1 x 256 tokens 17.1 / 27.0, 16 x 128 29.3 / 35.9; at the limit 1 x
 // 512 36.3 / 36.1; beyond it 8 x 256 47.1 / 34.2, 64 x 100 99.8 / 66.1.
 static bool small_call(const laya_attention& a) {
-    return a.max_len <= 512 && a.n_seqs <= 64 && a.n_heads <= 1024 &&
+    return a.max_len <= SMALL_LEN && a.n_seqs <= 64 && a.n_heads <= 1024 &&
            (uint64_t)a.n_tokens * a.n_heads * a.max_len <= 3u << 20;
 }
 
 // Does the backward pass of short sequences take a block to a sequence and key
-// head? Up to 32 tokens always: delta from P dP matters with few keys (see the
-// kernel), and costs nothing (1 x 16 tokens, 12 heads 5.3 us, 5.2 in blocks of
-// their own for dQ and for dK and dV). Up to 64 when there are more than 96 of
+// head? Up to 32 tokens always: they take delta from P dP, which is there (1 x 16
+// tokens, 12 heads 5.3 us, 5.2 in blocks of their own for dQ and for dK and dV). Up to 64 when there are more than 96 of
 // them: before that most SMs idle and the blocks of their own end sooner (1 x 64
 // 4.9 us instead of 6.8, 8 x 64 6.7 instead of 7.0, but 32 x 64 17.3 instead of
 // 9.2).
 static bool one_block_each(const laya_attention& a) {
-    return a.max_len <= 32 || (a.max_len <= TB && (uint64_t)a.n_seqs * a.n_kv_heads > 96);
+    return a.max_len <= SHORT || (a.max_len <= TB && (uint64_t)a.n_seqs * a.n_kv_heads > 96);
 }
 
 // A few times the blocks that the GPU holds at once: a block takes every
@@ -796,8 +873,10 @@ cudaError_t launch_attention_bwd(const laya_attention& a, const AttnIO& io, cuda
         return launch_one(bf16 ? attention_bwd_one_kernel<__nv_bfloat16, false> : attention_bwd_one_kernel<__half, false>,
                           ONE_SMEM<false>, a.n_kv_heads, g, stream);
     }
-    if (!small_call(a) || attention_near(a.window)) return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
-    auto kernel = bf16 ? attention_bwd_kernel<__nv_bfloat16> : attention_bwd_kernel<__half>;
+    if (!small_call(a) || narrow(a.window))
+        return launch_attention_bwd_tc(bf16, (int)a.n_heads, (int)a.n_kv_heads, g, stream);
+    auto kernel = a.token_mask ? (bf16 ? attention_bwd_kernel<__nv_bfloat16, true> : attention_bwd_kernel<__half, true>)
+                               : (bf16 ? attention_bwd_kernel<__nv_bfloat16, false> : attention_bwd_kernel<__half, false>);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)seq_tiles(g.n_tokens, g.n_seqs, TB), a.n_heads + a.n_kv_heads);

@@ -647,98 +647,6 @@ __device__ __forceinline__ void backward_mmas(const Frame& f, const AttnArgs& a,
     drain(&bar->drained, 0, a.status, &bar->abort);
 }
 
-// ------------------------------------------------------------------ delta
-// delta[h][t] = sum_d dO O, a thread to 8 elements, 8 lanes to a row of a head.
-// Bound by memory (both arrays once). Inside the dQ kernel, whose warps are
-// few, it took a third of an item's time at 175-180 tokens (dQ 80 -> 47 us
-// there, delta 8.6).
-constexpr int DELTA_THREADS = 256;
-constexpr int DELTA_ROWS = 4;  // of a thread, all loads under way at once
-
-template <typename T>
-__global__ void __launch_bounds__(DELTA_THREADS) attention_delta_kernel(const AttnArgs a, int heads) {
-    griddep_launch();
-    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the passes that follow
-    const int n = a.n_seqs;
-    const int first = max(a.cu[0], 0), last = min(a.cu[n], a.n_tokens);  // rows past either are not the call's
-    const int c = threadIdx.x & 7;
-    uint4 o[DELTA_ROWS], d[DELTA_ROWS];
-    long long to[DELTA_ROWS];
-#pragma unroll
-    for (int i = 0; i < DELTA_ROWS; i++) {
-        // tokens times heads: below 2^32 with the last block's surplus
-        const unsigned at = (blockIdx.x * DELTA_ROWS + i) * (DELTA_THREADS / 8) + threadIdx.x / 8;
-        const int t = (int)(at / (unsigned)heads), h = (int)(at - (unsigned)t * heads);
-        to[i] = -1;
-        o[i] = d[i] = make_uint4(0, 0, 0, 0);
-        if (t >= first && t < last && (!a.mask || a.mask[t] != 0)) {
-            to[i] = (long long)h * a.n_tokens + t;
-            o[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.out.p) + t * a.io.out.ld + h * 64 + c * 8);
-            d[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.io.dout.p) + t * a.io.dout.ld + h * 64 + c * 8);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < DELTA_ROWS; i++) {
-        const T* x = reinterpret_cast<const T*>(&o[i]);
-        const T* y = reinterpret_cast<const T*>(&d[i]);
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; k++) sum = fmaf(to_float(x[k]), to_float(y[k]), sum);
-#pragma unroll
-        for (int k = 1; k < 8; k *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-        if (to[i] >= 0 && c == 0) a.io.delta[to[i]] = sum;
-    }
-}
-
-// The same for narrow windows, as the sum over P dP of the few keys: O, rounded to
-// 16 bits, puts delta off by up to half a step of sum |dO O|, which gradients of
-// few keys show (1.7 times the error of a 32-bit pass rounded once at a window of
-// 1, 1.5 at 4; 1.4 this way, as at wider ones). A warp to a token, eight lanes to a
-// head. 64 x 180 tokens, 12 heads, window 4: forward and backward 144 us, 112 with
-// the kernel above; window 1: 125.
-template <typename T>
-__global__ void __launch_bounds__(DELTA_THREADS) attention_near_delta_kernel(const AttnArgs a, int heads) {
-    griddep_launch();
-    if (blockIdx.x == 0 && threadIdx.x < 2) a.io.tickets[threadIdx.x] = 0;  // for the passes that follow
-    const int lane = threadIdx.x & 31, c = (lane & 7) * 8;
-    const long long t = (long long)blockIdx.x * (DELTA_THREADS / 32) + (threadIdx.x >> 5);
-    if (t >= a.n_tokens) return;
-    const int seq = warp_search(a.n_seqs, lane, [&](int i) { return (long long)a.cu[i]; }, t);
-    if (seq < 0) return;
-    const int start = a.cu[seq], end = a.cu[seq + 1];
-    if (!run_ok(start, end, a.n_tokens, a.max_len) || t < start || t >= end || (a.mask && !a.mask[t])) return;
-    const long long lo = max((long long)start, t - a.window), hi = min((long long)end - 1, t + a.window);
-    const float sl2 = a.scale * LOG2E;
-    auto dot = [](const uint4& x, const uint4& y) {
-        const T* p = reinterpret_cast<const T*>(&x);
-        const T* q = reinterpret_cast<const T*>(&y);
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) sum = fmaf(to_float(p[e]), to_float(q[e]), sum);
-        return sum;
-    };
-    auto row = [&](const AttnRows& r, long long i, int head) {
-        return *reinterpret_cast<const uint4*>(static_cast<const T*>(r.p) + i * r.ld + head * 64 + c);
-    };
-    for (int h0 = 0; h0 < heads; h0 += 4) {
-        const int h = min(h0 + (lane >> 3), heads - 1), hk = h / a.group;  // a head too many: the last one again
-        const uint4 q = row(a.io.q, t, h), d = row(a.io.dout, t, h);
-        const float e = a.io.lse[(long long)h * a.n_tokens + t] * LOG2E;
-        float sum = 0.f;
-        for (long long j = lo; j <= hi; j++) {
-            if (a.mask && !a.mask[j]) continue;
-            float s = dot(q, row(a.io.k, j, hk)), dp = dot(d, row(a.io.v, j, hk));
-#pragma unroll
-            for (int x = 1; x < 8; x *= 2) {
-                s += __shfl_xor_sync(0xffffffffu, s, x);
-                dp += __shfl_xor_sync(0xffffffffu, dp, x);
-            }
-            sum = fmaf(ex2_approx(fmaf(s, sl2, -e)), dp, sum);
-        }
-        if (c == 0) a.io.delta[(long long)h * a.n_tokens + t] = sum;
-    }
-}
-
 // ------------------------------------------------------------------ dQ
 // TMEM: S at columns 0, 64 (dP over it, dS over that, 8 columns of every 16);
 // dQ at 128, the next item's at 192. extra: -lse * log2 e and -delta of the rows
@@ -764,13 +672,14 @@ __device__ __forceinline__ void dq_pass(const Frame& f, const CUtensorMap& mq, c
             // the rows' statistics (absent rows are not stored: 0 will do)
             float* stat = f.extra + (ld.items & 1) * 2 * ROWS + lane;
             float lse[4], delta[4];
+            const float* deltas = t.len <= SHORT ? a.io.delta_short : a.io.delta;
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const int i = t.row0 + x * 32 + lane;
                 const bool there = present(a, t, i);
                 const long long at = (long long)h * a.n_tokens + t.start + i;
                 lse[x] = there ? a.io.lse[at] : 0.f;
-                delta[x] = there ? a.io.delta[at] : 0.f;
+                delta[x] = there ? deltas[at] : 0.f;
             }
             ok = ld.slot();
             if (!ok) break;
@@ -895,6 +804,7 @@ __device__ __forceinline__ void dkv_pass(const Frame& f, const CUtensorMap& mq, 
             Presence rows;
             rows.read(a, t, qt0 * STEP, lane);
             ok = ld.item(Item{t.start, t.len, t.row0, hk, qt0, n}, &mk, &mv);
+            const float* deltas = t.len <= SHORT ? a.io.delta_short : a.io.delta;
             int h = hk * a.group, q = qt0;
             for (int j = 0; j < n && ok; j++) {
                 uint32_t bits[2];
@@ -904,7 +814,7 @@ __device__ __forceinline__ void dkv_pass(const Frame& f, const CUtensorMap& mq, 
                 const long long at = (long long)h * a.n_tokens + t.start + row0 + lane;
                 const bool b0 = bits[0] >> lane & 1, b1 = bits[1] >> lane & 1;
                 const float l0 = b0 ? a.io.lse[at] : 0.f, l1 = b1 ? a.io.lse[at + 32] : 0.f;
-                const float d0 = b0 ? a.io.delta[at] : 0.f, d1 = b1 ? a.io.delta[at + 32] : 0.f;
+                const float d0 = b0 ? deltas[at] : 0.f, d1 = b1 ? deltas[at + 32] : 0.f;
                 const int head = h;
                 if (++q == qt1) {
                     q = qt0;
@@ -1093,15 +1003,7 @@ cudaError_t backward(const Maps& m, const AttnArgs& a, int heads, int kv_heads, 
     const auto kernel = attention_bwd_tc_kernel<T, Bwd>;
     cudaError_t e = allow_smem<Bwd>(kernel);
     if (e != cudaSuccess) return e;
-    if (attention_near(a.window)) {
-        const unsigned blocks = (a.n_tokens + DELTA_THREADS / 32 - 1) / (DELTA_THREADS / 32);
-        attention_near_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
-    } else {
-        const unsigned per = DELTA_THREADS / 8 * DELTA_ROWS;
-        const unsigned blocks = (unsigned)(((unsigned long long)a.n_tokens * heads + per - 1) / per);
-        attention_delta_kernel<T><<<blocks, DELTA_THREADS, 0, stream>>>(a, heads);
-    }
-    e = cudaGetLastError();
+    e = launch_attention_delta(std::is_same<T, __nv_bfloat16>::value, heads, a, stream);
     if (e != cudaSuccess) return e;
     return launch_k(kernel, dim3(ctas(a, heads)), THREADS, smem_bytes<Bwd>(), stream, m.q, m.k, m.v, m.dout, a, heads,
                     kv_heads);

@@ -119,10 +119,10 @@ int check_attention(const char* op, const laya_attention* a) {
     return LAYA_OK;
 }
 
-// Two counters, then delta.
+// Two counters, then delta twice: of all rows, and of those of short sequences.
 constexpr uint64_t WORKSPACE_HEAD = 16;
 uint64_t workspace_bytes_of(const laya_attention* a) {
-    return WORKSPACE_HEAD + (uint64_t)a->n_heads * a->n_tokens * sizeof(float);
+    return WORKSPACE_HEAD + 2 * (uint64_t)a->n_heads * a->n_tokens * sizeof(float);
 }
 
 struct Rows {
@@ -312,6 +312,7 @@ int laya_gpu_attention_backward(const laya_attention* a, const void* q, int64_t 
     io.lse = const_cast<float*>(lse);
     io.tickets = static_cast<unsigned long long*>(workspace);
     io.delta = static_cast<float*>(workspace) + WORKSPACE_HEAD / sizeof(float);
+    io.delta_short = io.delta + (uint64_t)hq * T;
     const cudaError_t e = launch_attention_bwd(*a, io, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? LAYA_OK : cuda_fail(op, e);
 }

@@ -120,6 +120,7 @@ struct AttnIO {
     AttnRows q, k, v, out, dout, dq, dk, dv;
     float* lse;    // [n_heads][n_tokens]
     float* delta;  // [n_heads][n_tokens], of the backward pass's workspace
+    float* delta_short;  // the same for short sequences: delta, or an array of its own
     unsigned long long* tickets;  // two counters, of the workspace
 };
 cudaError_t launch_attention_fwd(const laya_attention& a, const AttnIO& io, cudaStream_t stream);
