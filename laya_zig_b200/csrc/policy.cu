@@ -1,8 +1,9 @@
 // policy.cu -- the clipped policy loss over each decision's options, with its
 // gradient, in one pass over the logits.
 //
-// Per decision, z = logits / t: lse = log sum e^z, lp_j = z_j - lse, p_j =
-// e^lp_j; H = -sum p_j lp_j; d_j = lp_j - log ref_j and
+// Per decision, z = (logits - their maximum) / t: the difference first, so that a
+// number added to all of a decision's logits costs no digits. lse = log sum e^z,
+// lp_j = z_j - lse, p_j = e^lp_j; H = -sum p_j lp_j; d_j = lp_j - log ref_j and
 //   KL(p||ref) = sum p_j d_j = sum (p_j d_j - p_j + ref_j),
 // whose terms p (d + e^-d - 1) are never negative and vanish quadratically in
 // d: a rounding error in either lse cancels to first order, so a policy that
@@ -35,7 +36,7 @@ struct Scalars {
     const uint32_t* qtypes;
     int n, G;
     int max_k;
-    float scale[3];   // log2(e) / temperature: logits -> z in units of log 2
+    float scale[3];   // log2(e) / temperature: differences of logits -> z in units of log 2
     float inv_t[3];
     float lo, hi, kl_coef, ent_coef;
     int* status;
@@ -69,7 +70,7 @@ __device__ __forceinline__ void group_reduce(float& a, float& b, float2* buf) {
 struct Decision {
     int start, k, action;
     float adv, old_logp, grad, inv_t, scale;
-    float taken;  // z of the action
+    float taken;  // the action's logit
     bool ok;
 };
 
@@ -89,7 +90,7 @@ __device__ __forceinline__ Decision load_decision(const Scalars& s, const Policy
     d.inv_t = q == 1u ? s.inv_t[1] : q == 2u ? s.inv_t[2] : s.inv_t[0];
     d.scale = q == 1u ? s.scale[1] : q == 2u ? s.scale[2] : s.scale[0];
     if (!run) d.k = 0;  // nothing of it can be addressed
-    d.taken = d.ok && d.k > 0 ? to_float(static_cast<const T*>(io.logits)[start + d.action]) * d.scale : 0.f;
+    d.taken = d.ok && d.k > 0 ? to_float(static_cast<const T*>(io.logits)[start + d.action]) : 0.f;
     return d;
 }
 
@@ -188,8 +189,8 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
         }
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            z[v] = l + v * G < k ? to_float(raw[v]) * d.scale : -INFINITY;
-            zr[v] = REF && l + v * G < k ? to_float(rawr[v]) * d.scale : -INFINITY;
+            z[v] = l + v * G < k ? to_float(raw[v]) : -INFINITY;
+            zr[v] = REF && l + v * G < k ? to_float(rawr[v]) : -INFINITY;
         }
     }
     float m = -INFINITY, mr = -INFINITY;
@@ -206,12 +207,16 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
 #pragma unroll
     for (int v = 0; v < V; v++) {
         if (v * G >= k) break;  // of the whole group
-        sum += ex2_approx(z[v] - mz);
-        if (REF) sumr += ex2_approx(zr[v] - mrz);
+        z[v] = (z[v] - mz) * d.scale;
+        sum += ex2_approx(z[v]);
+        if (REF) {
+            zr[v] = (zr[v] - mrz) * d.scale;
+            sumr += ex2_approx(zr[v]);
+        }
     }
     group_reduce<G, false>(sum, sumr, buf[1]);
     const bool some = d.ok && !(sum == 0.f);  // an option that is not ruled out
-    const float lse = mz + lg2_approx(sum), lser = mrz + lg2_approx(sumr);
+    const float lse = lg2_approx(sum), lser = lg2_approx(sumr);
     float ent = 0.f, kl = 0.f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
         }
     }
     group_reduce<G, false>(ent, kl, buf[2]);
-    Result r = some ? finish(s, d, (d.taken - lse) * LN2, kl * LN2, ent * LN2) : Result{};
+    Result r = some ? finish(s, d, ((d.taken - mz) * d.scale - lse) * LN2, kl * LN2, ent * LN2) : Result{};
     if (!live) return;
     if (l == 0) store_scalars(io, i, r);
     if (io.dlogits) {
@@ -260,39 +265,39 @@ __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyI
         const int k = d.k;
         float m = -INFINITY, mr = -INFINITY;
         for (int j = threadIdx.x; j < k; j += THREADS) {
-            m = fmaxf(m, to_float(x[j]) * d.scale);
-            if (io.ref) mr = fmaxf(mr, to_float(xr[j]) * d.scale);
+            m = fmaxf(m, to_float(x[j]));
+            if (io.ref) mr = fmaxf(mr, to_float(xr[j]));
         }
         group_reduce<THREADS, true>(m, mr, buf[0]);
         const float mz = m == -INFINITY ? 0.f : m, mrz = mr == -INFINITY ? 0.f : mr;
         float sum = 0.f, sumr = 0.f;
         for (int j = threadIdx.x; j < k; j += THREADS) {
-            sum += ex2_approx(to_float(x[j]) * d.scale - mz);
-            if (io.ref) sumr += ex2_approx(to_float(xr[j]) * d.scale - mrz);
+            sum += ex2_approx((to_float(x[j]) - mz) * d.scale);
+            if (io.ref) sumr += ex2_approx((to_float(xr[j]) - mrz) * d.scale);
         }
         group_reduce<THREADS, false>(sum, sumr, buf[1]);
         const bool some = d.ok && !(sum == 0.f);
-        const float lse = mz + lg2_approx(sum), lser = mrz + lg2_approx(sumr);
+        const float lse = lg2_approx(sum), lser = lg2_approx(sumr);
         float ent = 0.f, kl = 0.f;
         for (int j = threadIdx.x; j < k; j += THREADS) {
-            const float lp = to_float(x[j]) * d.scale - lse, p = ex2_approx(lp);
+            const float lp = (to_float(x[j]) - mz) * d.scale - lse, p = ex2_approx(lp);
             if (!(p == 0.f)) ent = fmaf(-p, lp, ent);
             if (io.ref) {
-                const float lr = to_float(xr[j]) * d.scale - lser;
+                const float lr = (to_float(xr[j]) - mrz) * d.scale - lser;
                 kl += kl_term(lp - lr, p, lr);
             }
         }
         group_reduce<THREADS, false>(ent, kl, buf[2]);
-        const Result r = some ? finish(s, d, (d.taken - lse) * LN2, kl * LN2, ent * LN2) : Result{};
+        const Result r = some ? finish(s, d, ((d.taken - mz) * d.scale - lse) * LN2, kl * LN2, ent * LN2) : Result{};
         __syncthreads();  // buf is free for the next decision
         if (threadIdx.x == 0) store_scalars(io, i, r);
         if (io.dlogits) {
             T* dx = static_cast<T*>(io.dlogits) + d.start;
             const Slope c = slope(s, d, r);
             for (int j = threadIdx.x; j < k; j += THREADS) {
-                const float lp = to_float(x[j]) * d.scale - lse, p = ex2_approx(lp);
+                const float lp = (to_float(x[j]) - mz) * d.scale - lse, p = ex2_approx(lp);
                 float g = fmaf(c.c2, lp, c.c0);
-                if (io.ref) g = fmaf(c.c1, lp - (to_float(xr[j]) * d.scale - lser), g);
+                if (io.ref) g = fmaf(c.c1, lp - ((to_float(xr[j]) - mrz) * d.scale - lser), g);
                 g = p == 0.f ? 0.f : p * g;
                 if (j == d.action) g += c.own;
                 dx[j] = from_float<T>(some ? g : 0.f);
