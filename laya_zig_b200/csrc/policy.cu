@@ -90,7 +90,7 @@ __device__ __forceinline__ Decision load_decision(const Scalars& s, const Policy
     d.inv_t = q == 1u ? s.inv_t[1] : q == 2u ? s.inv_t[2] : s.inv_t[0];
     d.scale = q == 1u ? s.scale[1] : q == 2u ? s.scale[2] : s.scale[0];
     if (!run) d.k = 0;  // nothing of it can be addressed
-    d.taken = d.ok && d.k > 0 ? to_float(static_cast<const T*>(io.logits)[start + d.action]) : 0.f;
+    d.taken = d.ok && d.k > 0 ? to_float(static_cast<const T*>(io.logits)[start + d.action]) : -INFINITY;
     return d;
 }
 
@@ -99,6 +99,34 @@ __device__ __forceinline__ float lg2_approx(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// What is made of the sum of e^z over the options that were not taken.
+struct Sum {
+    float taken;   // z of the option that was taken
+    float others;  // 1 - p of it
+    float lse;     // log2
+    bool some;     // an option is not ruled out
+};
+// In a decision that is nearly certain the others are all that log p is made of:
+// lg2.approx of 1 + rest would be off by 2^-22, not by that much of log p. With q = 1 -
+// p <= 1/9, -log(1 - q) = q + q^2 / 2 + ... up to q^7 / 7; the next term is below 2^-25
+// of the sum.
+__device__ __forceinline__ Sum make_sum(const Decision& d, float mz, float rest) {
+    Sum s;
+    s.taken = (d.taken - mz) * d.scale;
+    const float total = ex2_approx(s.taken) + rest;
+    const float q = __fdividef(rest, total);
+    s.some = d.ok && !(total == 0.f);
+    s.others = q;
+    float y = fmaf(q, LOG2E / 7.f, LOG2E / 6.f);
+    y = fmaf(q, y, LOG2E / 5.f);
+    y = fmaf(q, y, LOG2E / 4.f);
+    y = fmaf(q, y, LOG2E / 3.f);
+    y = fmaf(q, y, LOG2E / 2.f);
+    y = fmaf(q, y, LOG2E);
+    s.lse = s.taken == 0.f && rest < 0.125f ? q * y : lg2_approx(total);
+    return s;
 }
 
 struct Result {
@@ -144,16 +172,19 @@ __device__ __forceinline__ float kl_term(float d, float p, float lr) {
     return !(p == 0.f) && fabsf(d) < 0.25f / L ? near : p == 0.f ? ex2_approx(lr) * (1.f / L) : far;
 }
 
-// dloss/dz of one option, times the weights: p (c0 + c1 d + c2 lp), plus
-// own for the option that was taken.
+// dloss/dz of one option, times the weights: p (c0 + c1 d + c2 lp); of the option
+// that was taken p (c + c1 d + c2 lp) plus own, which is g (1 - p) from the other
+// options' sum: 1 - p as a difference would leave a certain decision's gradients no
+// digits.
 struct Slope {
-    float own, c0, c1, c2;
+    float own, c, c0, c1, c2;
 };
-__device__ __forceinline__ Slope slope(const Scalars& s, const Decision& d, const Result& r) {
+__device__ __forceinline__ Slope slope(const Scalars& s, const Decision& d, const Result& r, float others) {
     const float w = d.grad * d.inv_t;
     Slope c;
-    c.own = r.g * w;
-    c.c0 = w * (-r.g - s.kl_coef * r.kl + s.ent_coef * r.ent);
+    c.own = r.g * w * others;
+    c.c = w * (s.ent_coef * r.ent - s.kl_coef * r.kl);
+    c.c0 = c.c - w * r.g;
     c.c1 = w * s.kl_coef * LN2;
     c.c2 = w * s.ent_coef * LN2;
     return c;
@@ -173,7 +204,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
     if (live && !d.ok && l == 0) atomicOr(s.status, ERR_BAD_INDEX);
     const T* x = static_cast<const T*>(io.logits) + d.start;
     const T* xr = REF ? static_cast<const T*>(io.ref) + d.start : x;
-    const int k = d.k;
+    const int k = d.k, mine = d.action - l;  // v * G if option v of this thread was taken
     // thread l holds options l, l + G, ..; all loads are under way before the
     // first is used
     float z[V], zr[V], p[V];
@@ -208,15 +239,15 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
     for (int v = 0; v < V; v++) {
         if (v * G >= k) break;  // of the whole group
         z[v] = (z[v] - mz) * d.scale;
-        sum += ex2_approx(z[v]);
+        if (v * G != mine) sum += ex2_approx(z[v]);
         if (REF) {
             zr[v] = (zr[v] - mrz) * d.scale;
             sumr += ex2_approx(zr[v]);
         }
     }
     group_reduce<G, false>(sum, sumr, buf[1]);
-    const bool some = d.ok && !(sum == 0.f);  // an option that is not ruled out
-    const float lse = lg2_approx(sum), lser = lg2_approx(sumr);
+    const Sum t = make_sum(d, mz, sum);
+    const float lse = t.lse, lser = lg2_approx(sumr);
     float ent = 0.f, kl = 0.f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -232,21 +263,21 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
         }
     }
     group_reduce<G, false>(ent, kl, buf[2]);
-    Result r = some ? finish(s, d, ((d.taken - mz) * d.scale - lse) * LN2, kl * LN2, ent * LN2) : Result{};
+    Result r = t.some ? finish(s, d, (t.taken - lse) * LN2, kl * LN2, ent * LN2) : Result{};
     if (!live) return;
     if (l == 0) store_scalars(io, i, r);
     if (io.dlogits) {
         T* dx = static_cast<T*>(io.dlogits) + d.start;
-        const Slope c = slope(s, d, r);
+        const Slope c = slope(s, d, r, t.others);
 #pragma unroll
         for (int v = 0; v < V; v++) {
             if (v * G >= k) break;
             const int j = l + v * G;
-            float g = fmaf(c.c2, z[v], c.c0);
+            float g = fmaf(c.c2, z[v], v * G == mine ? c.c : c.c0);
             if (REF) g = fmaf(c.c1, zr[v], g);
             g = p[v] == 0.f ? 0.f : p[v] * g;  // an option that is ruled out has log p = -inf
-            if (j == d.action) g += c.own;
-            if (j < k) dx[j] = from_float<T>(some ? g : 0.f);
+            if (v * G == mine) g += c.own;
+            if (j < k) dx[j] = from_float<T>(t.some ? g : 0.f);
         }
     }
 }
@@ -272,12 +303,12 @@ __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyI
         const float mz = m == -INFINITY ? 0.f : m, mrz = mr == -INFINITY ? 0.f : mr;
         float sum = 0.f, sumr = 0.f;
         for (int j = threadIdx.x; j < k; j += THREADS) {
-            sum += ex2_approx((to_float(x[j]) - mz) * d.scale);
+            if (j != d.action) sum += ex2_approx((to_float(x[j]) - mz) * d.scale);
             if (io.ref) sumr += ex2_approx((to_float(xr[j]) - mrz) * d.scale);
         }
         group_reduce<THREADS, false>(sum, sumr, buf[1]);
-        const bool some = d.ok && !(sum == 0.f);
-        const float lse = lg2_approx(sum), lser = lg2_approx(sumr);
+        const Sum t = make_sum(d, mz, sum);
+        const float lse = t.lse, lser = lg2_approx(sumr);
         float ent = 0.f, kl = 0.f;
         for (int j = threadIdx.x; j < k; j += THREADS) {
             const float lp = (to_float(x[j]) - mz) * d.scale - lse, p = ex2_approx(lp);
@@ -288,19 +319,19 @@ __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyI
             }
         }
         group_reduce<THREADS, false>(ent, kl, buf[2]);
-        const Result r = some ? finish(s, d, ((d.taken - mz) * d.scale - lse) * LN2, kl * LN2, ent * LN2) : Result{};
+        const Result r = t.some ? finish(s, d, (t.taken - lse) * LN2, kl * LN2, ent * LN2) : Result{};
         __syncthreads();  // buf is free for the next decision
         if (threadIdx.x == 0) store_scalars(io, i, r);
         if (io.dlogits) {
             T* dx = static_cast<T*>(io.dlogits) + d.start;
-            const Slope c = slope(s, d, r);
+            const Slope c = slope(s, d, r, t.others);
             for (int j = threadIdx.x; j < k; j += THREADS) {
                 const float lp = (to_float(x[j]) - mz) * d.scale - lse, p = ex2_approx(lp);
-                float g = fmaf(c.c2, lp, c.c0);
+                float g = fmaf(c.c2, lp, j == d.action ? c.c : c.c0);
                 if (io.ref) g = fmaf(c.c1, lp - ((to_float(xr[j]) - mrz) * d.scale - lser), g);
                 g = p == 0.f ? 0.f : p * g;
                 if (j == d.action) g += c.own;
-                dx[j] = from_float<T>(some ? g : 0.f);
+                dx[j] = from_float<T>(t.some ? g : 0.f);
             }
         }
     }

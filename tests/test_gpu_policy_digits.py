@@ -53,3 +53,96 @@ def test_a_shift_of_all_logits_changes_nothing(lens, dtype, which):
         want = lp[int(act[i])].item()
         bound = 2.0 ** -21 * (2 + far[int(act[i])].item() + (lp.exp() * far).sum().item())
         assert abs(b["logp"][i].item() - want) <= bound and math.isfinite(want)
+
+
+def _certain(lens, seed):
+    """Logits 8 to 12 below the decision's best option, which was taken; old log
+    probabilities near the present ones."""
+    import torch
+    g = torch.Generator()
+    g.manual_seed(seed)
+    z, act, old = [], [], []
+    for k in lens:
+        x = -8 - 4 * torch.rand(k, generator=g)
+        a = int(torch.randint(0, k, (1,), generator=g))
+        x[a] = 0.0
+        z.append(x + 3.0)
+        act.append(a)
+        old.append(0.1 * (torch.rand((), generator=g).item() - 0.5))
+    n = len(lens)
+    q = torch.randint(0, 3, (n,), generator=g).to(torch.int32)
+    return (torch.cat(z), torch.tensor(act, dtype=torch.int32), q, torch.rand(n, generator=g) + 0.5,
+            torch.tensor(old), torch.ones(n))
+
+
+@pytest.mark.parametrize("lens", ["to16", "to32", "to64", "to128", "to256", "to512", "to1024", "wider"])
+def test_certain_decisions_keep_their_digits(lens):
+    """1 - p near 1e-4 a rival: log p, the entropy and the gradients, relative to
+    themselves. In units of 2^-23: a rival's e^z is off by |z| (z's rounding) and 2
+    (ex2.approx), their sum by 20 (39 roundings at most), the logarithm by 12 (of
+    1/8 and more, where lg2.approx's 2^-22 is that part of it; less below), its
+    products by 4: R = |z| + 38 for log p and 1 - p. The ratio: exp of log p - old,
+    both at most 1 in size and off by R |log p| + 2^-24: 2^-20. The entropy's terms
+    are p times log p, products of values off by R and 2^-23 (1 + |z|)."""
+    import torch
+    from laya_zig_b200 import gpu
+    shape = SHAPES[lens]
+    z, act, q, adv, old, grad = _certain(shape, 7)
+    out, status = _call(shape, z, None, act, q, adv, old, grad, klc=0.0, entc=0.0, lead=2)
+    gpu.op_status(status.data_ptr())
+    at = 0
+    for i, k in enumerate(shape):
+        t = float(np.float32(TEMP[int(q[i])]))
+        zi = (z[at:at + k].double()).requires_grad_(True)
+        got = out["dlogits"][2 + at:2 + at + k].cpu().double()
+        at += k
+        loss, logp, _, ent = ref.policy(zi, None, int(act[i]), float(adv[i]), float(old[i]), t, float(np.float32(0.2)),
+                                        float(np.float32(0.3)), 0.0, 0.0)
+        want = torch.autograd.grad(loss, zi)[0]
+        if k == 1:
+            assert out["logp"][i] == 0 and out["entropy"][i] == 0 and got[0] == 0
+            continue
+        R = 2.0 ** -23 * (12 / t + 38)
+        assert abs(out["logp"][i].item() / logp.item() - 1) <= R
+        assert abs(out["entropy"][i].item() / ent.item() - 1) <= 2 * R
+        assert ((got - want).abs() <= (2 * R + 2.0 ** -20) * want.abs()).all()
+        assert abs(got.sum().item()) <= (2 * R + 2.0 ** -20) * got.abs().sum().item()
+
+
+@pytest.mark.parametrize("lens", ["to16", "to32", "to64", "to128", "to256", "to512", "to1024", "wider"])
+@pytest.mark.parametrize("every", [1, 2, 3])
+def test_ties_at_the_maximum(lens, every):
+    """All options, or every second or third, at the maximum, the others ruled out:
+    the sum is the whole number n, log p its logarithm within 2^-21 (of two or
+    more: lg2.approx 2^-22 of 1 at least, two products), 1 / n and 1 - 1 / n right
+    to 2^-20, and the gradients, -1/n of the difference, to 2^-19."""
+    import torch
+    from laya_zig_b200 import gpu
+    shape = [k for k in SHAPES[lens] if k >= 3]
+    z = torch.full((sum(shape),), -math.inf)
+    at, act = 0, []
+    for k in shape:
+        z[at:at + k:every] = 1.5
+        act.append((k - 1) // every * every)
+        at += k
+    n = len(shape)
+    act = torch.tensor(act, dtype=torch.int32)
+    adv, old = torch.ones(n), torch.zeros(n)
+    out, status = _call(shape, z, z, act, None, adv, old, torch.ones(n), klc=0.0, entc=0.0)
+    gpu.op_status(status.data_ptr())
+    at = 0
+    for i, k in enumerate(shape):
+        m = len(range(0, k, every))
+        d = out["dlogits"][2 + at:2 + at + k].cpu().double()
+        at += k
+        assert abs(out["logp"][i].item() + math.log(m)) <= 2.0 ** -21 * math.log(m)
+        assert abs(out["entropy"][i].item() - math.log(m)) <= 2.0 ** -20 * math.log(m)
+        assert out["kl"][i].item() == 0
+        if m == 1:
+            assert (d == 0).all()
+            continue
+        want = torch.zeros(k, dtype=torch.float64)
+        want[::every] = 1.0 / m
+        want[int(act[i])] -= 1.0
+        want /= m  # the ratio: old is 0; below the clip's range min keeps r A
+        assert ((d - want).abs() <= 2.0 ** -19 * want.abs()).all()
