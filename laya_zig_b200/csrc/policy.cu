@@ -158,8 +158,9 @@ __device__ __forceinline__ void store_scalars(const PolicyIO& io, int i, const R
 // One option's share of the KL in units of log 2, from its log2
 // probabilities: p d - p + ref. For |d| < 1/4 that is p times the series of
 // d + e^-d - 1 = d^2 (1/2 - d/6 + d^2/24 - ...), six terms of it (the next is
-// below 2^-23 of the sum); from there on the plain differences, whose
-// rounding is below 2^-20 of it. In units of log 2: a = log 2 times d.
+// below 2^-23 of the sum); from there on the plain differences, off by 2^-22 of p
+// and ref each: 2^-16 of the term at 1/4, 2^-20 from 1 on. In units of log 2: a = log
+// 2 times d.
 __device__ __forceinline__ float kl_term(float d, float p, float lr) {
     constexpr float L = LN2;
     float g = fmaf(d, -L * L * L * L * L * L / 5040.f, L * L * L * L * L / 720.f);
