@@ -394,7 +394,9 @@ LAYA_API int laya_gpu_attention_backward(const laya_attention* a, const void* q,
  *          + kl_coef * sum_j p_j (log p_j - log ref_j) - entropy_coef * H(p),
  * dlogits = grad * dloss/dlogits. An option whose logit is -inf is ruled out:
  * p = 0, it adds nothing and its gradient is 0 (in ref_logits it should be
- * -inf too: it then carries no reference probability either). A decision
+ * -inf too: it then carries no reference probability either; where only the
+ * reference rules it out the divergence is infinite, and with kl_coef 0
+ * reported alone). A decision
  * without options, or with every option ruled out, has loss 0 and gradient
  * 0. The temperature is held to 1e-3 at least, as in the tempered softmax of
  * src/main.zig:3799-3813. */

@@ -134,6 +134,10 @@ struct Result {
     float g;  // d loss / d logp through the clipped ratio
 };
 
+// kl_coef times x, and 0 where the divergence is only reported: it may be infinite
+// (a reference that rules out what the policy does not).
+__device__ __forceinline__ float kl_times(const Scalars& s, float x) { return s.kl_coef == 0.f ? 0.f : s.kl_coef * x; }
+
 __device__ __forceinline__ Result finish(const Scalars& s, const Decision& d, float logp, float kl, float ent) {
     Result r;
     r.logp = logp;
@@ -143,7 +147,7 @@ __device__ __forceinline__ Result finish(const Scalars& s, const Decision& d, fl
     const float free_ = ratio * d.adv;
     const float held = fminf(fmaxf(ratio, s.lo), s.hi) * d.adv;
     const bool active = !(free_ > held);  // NaN stays NaN
-    r.loss = -(active ? free_ : held) + s.kl_coef * kl - s.ent_coef * ent;
+    r.loss = -(active ? free_ : held) + kl_times(s, kl) - s.ent_coef * ent;
     r.g = active ? -free_ : 0.f;
     return r;
 }
@@ -184,7 +188,7 @@ __device__ __forceinline__ Slope slope(const Scalars& s, const Decision& d, cons
     const float w = d.grad * d.inv_t;
     Slope c;
     c.own = r.g * w * others;
-    c.c = w * (s.ent_coef * r.ent - s.kl_coef * r.kl);
+    c.c = w * (s.ent_coef * r.ent - kl_times(s, r.kl));
     c.c0 = c.c - w * r.g;
     c.c1 = w * s.kl_coef * LN2;
     c.c2 = w * s.ent_coef * LN2;
@@ -275,7 +279,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(Scalars s, PolicyIO io)
             if (v * G >= k) break;
             const int j = l + v * G;
             float g = fmaf(c.c2, z[v], v * G == mine ? c.c : c.c0);
-            if (REF) g = fmaf(c.c1, zr[v], g);
+            if (REF && s.kl_coef != 0.f) g = fmaf(c.c1, zr[v], g);
             g = p[v] == 0.f ? 0.f : p[v] * g;  // an option that is ruled out has log p = -inf
             if (v * G == mine) g += c.own;
             if (j < k) dx[j] = from_float<T>(t.some ? g : 0.f);
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(THREADS) policy_wide_kernel(Scalars s, PolicyI
             for (int j = threadIdx.x; j < k; j += THREADS) {
                 const float lp = (to_float(x[j]) - mz) * d.scale - lse, p = ex2_approx(lp);
                 float g = fmaf(c.c2, lp, j == d.action ? c.c : c.c0);
-                if (io.ref) g = fmaf(c.c1, lp - ((to_float(xr[j]) - mrz) * d.scale - lser), g);
+                if (io.ref && s.kl_coef != 0.f) g = fmaf(c.c1, lp - ((to_float(xr[j]) - mrz) * d.scale - lser), g);
                 g = p == 0.f ? 0.f : p * g;
                 if (j == d.action) g += c.own;
                 dx[j] = from_float<T>(t.some ? g : 0.f);

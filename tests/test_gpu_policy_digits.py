@@ -146,3 +146,28 @@ def test_ties_at_the_maximum(lens, every):
         want[int(act[i])] -= 1.0
         want /= m  # the ratio: old is 0; below the clip's range min keeps r A
         assert ((d - want).abs() <= 2.0 ** -19 * want.abs()).all()
+
+
+@pytest.mark.parametrize("lens", ["to16", "to64", "to512", "to1024", "wider"])
+def test_a_reference_that_rules_options_out(lens):
+    """An option that only the reference rules out makes the divergence infinite.
+    With kl_coef 0 it is reported and nothing else: loss and gradients are those
+    without a reference."""
+    import torch
+    from laya_zig_b200 import gpu
+    shape = SHAPES[lens]
+    z, zr, act, q, adv, old, grad = _make(shape, seed=3)
+    zr = zr.clone()
+    at = 0
+    for k in shape:
+        if k > 1:
+            zr[at + k // 2] = -math.inf
+        at += k
+    a, sa = _call(shape, z, zr, act, q, adv, old, grad, klc=0.0)
+    b, sb = _call(shape, z, None, act, q, adv, old, grad, klc=0.0)
+    for s in (sa, sb):
+        gpu.op_status(s.data_ptr())
+    for i, k in enumerate(shape):
+        assert a["kl"][i].item() == (math.inf if k > 1 else 0.0)
+    for name in ("loss", "logp", "entropy", "dlogits"):
+        assert torch.isfinite(b[name]).all() and torch.equal(a[name], b[name]), name
