@@ -19,16 +19,16 @@
 // These kernels serve calls that a few waves of blocks finish, where what
 // counts is the chain of dependent steps in one block (find the sequence, load,
 // two to five products of 16 x 8 x 16 instructions, exponentials, store), not
-// a rate. One sequence of 64 tokens, 12 heads, bf16: forward 4.2 us, backward
-// 4.5 us (a short kernel on its own takes 1.8 there). Backward in one launch
-// instead of a dQ launch followed by a dK/dV launch that reads its delta: 9.3
-// -> 5.1 us there; delta is recomputed from O, which a row's tile costs little.
+// a rate. One sequence of 64 tokens, 12 heads, bf16: forward 3.7 us, backward
+// 4.3 us (a short kernel on its own takes 1.8 there). Backward in one launch
+// instead of a dQ launch followed by a dK/dV launch that reads its delta: half the
+// time there; delta is recomputed from O, which a row's tile costs little.
 //
-// Sequences of 64 tokens at most have kernels of their own below, whatever
-// their number, because a 128-row tcgen05 item or a search for each of them
-// costs more than its work: forward and backward of 512 sequences of 16 / 32 /
-// 64 tokens, 12 heads, 265 / 230 / 235 us on tcgen05, 72 / 102 / 154 here (139 /
-// 277 / 553 MB: 3.6 TB/s for the last).
+// Sequences of 64 tokens at most have kernels of their own below (the backward
+// pass of a few of more than 32 tokens does without, see one_block_each), because a
+// 128-row tcgen05 item or a search for each of them costs more than its work: forward
+// and backward of 512 sequences of 16 / 32 / 64 tokens, 12 heads, 265 / 230 / 235 us
+// on tcgen05, 72 / 102 / 153 here (139 / 277 / 553 MB: 3.6 TB/s for the last).
 //
 // Rows outside their sequence and absent tokens are filled with zeros on
 // their way into shared memory (cp.async with a source size of 0), so nothing
@@ -834,12 +834,17 @@ static bool small_call(const laya_attention& a) {
 
 // Does the backward pass of short sequences take a block to a sequence and key
 // head? Up to 32 tokens always: they take delta from P dP, which is there (1 x 16
-// tokens, 12 heads 5.3 us, 5.2 in blocks of their own for dQ and for dK and dV). Up to 64 when there are more than 96 of
-// them: before that most SMs idle and the blocks of their own end sooner (1 x 64
-// 4.9 us instead of 6.8, 8 x 64 6.7 instead of 7.0, but 32 x 64 17.3 instead of
-// 9.2).
+// tokens, 12 heads 5.3 us, 5.2 in blocks of their own for dQ and for dK and dV); up to
+// 64 in a narrow window for the same reason (1 x 64, window 2, 6.3 us, 19.8 with
+// delta's own launch). Otherwise up to 64 when there are more than 96 of them: before
+// that most SMs idle and the blocks of their own end sooner (12 heads over 12, blocks of
+// their own / a block each: 1 x 64 4.3 / 5.9, 8 x 64 8.0 / 7.1, 32 x 64 17.3 / 11.4).
+// Heads that share a key head lengthen a block: 12 over 4, 1 x 64 7.6 / 14.1, 24 x 64
+// 16.5 / 20.1; 12 over 1, 64 x 64 42 / 69, and from 65 sequences to 96, where it is no
+// longer a small call, 31-36 on tcgen05.
 static bool one_block_each(const laya_attention& a) {
-    return a.max_len <= SHORT || (a.max_len <= TB && (uint64_t)a.n_seqs * a.n_kv_heads > 96);
+    return a.max_len <= SHORT ||
+           (a.max_len <= TB && (narrow(a.window) || (uint64_t)a.n_seqs * a.n_kv_heads > 96));
 }
 
 // A few times the blocks that the GPU holds at once: a block takes every

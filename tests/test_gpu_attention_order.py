@@ -67,3 +67,20 @@ def test_workspace_of_the_call_before(hq, hk):
         torch.cuda.synchronize()
         for k, w in zip(kept, want):
             assert torch.equal(k, w)
+
+
+@pytest.mark.parametrize("lens,window", [([64], 2), ([33, 40, 64], 0), ([50] * 5, 4)])
+def test_short_sequences_in_a_narrow_window_are_one_launch(lens, window):
+    """Their blocks have all of delta at hand."""
+    import torch
+    p = Problem(lens, window=window)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        p.run(s.cuda_stream)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g, stream=s):
+        p.backward(s.cuda_stream)
+    assert _nodes(g.raw_cuda_graph()) == [0]
+    torch.cuda.synchronize()
+    p.check()
