@@ -443,6 +443,12 @@ def _op_check(rc: int) -> None:
         raise _error(rc, lib.laya_gpu_last_error(None).decode())
 
 
+def _fits(op: str, signed: int = 0, *counts: int) -> None:
+    """Refuse whole numbers that would wrap into another one on their way to C."""
+    if any(c >> 32 for c in counts) or not -1 << 31 <= signed < 1 << 31:
+        raise LayaError(ERR_ARG, "%s: a count is negative or does not fit 32 bits" % op)
+
+
 def op_status(status_ptr: int, stream: int = 0) -> None:
     """Wait for `stream`; raise if an operator that was given this status
     word recorded a failed check or a wait that ran out; clear the word."""
@@ -459,6 +465,7 @@ class RopePlan:
                  beta_slow: float = 1.0, magnitude: float = 1.0):
         if layout not in ROPE_LAYOUTS:
             raise LayaError(ERR_ARG, "rope_plan: layout %s" % layout)
+        _fits("rope_plan", 0, head_dim, rot_dim or 0, original_len)
         self.c = _RopePlan()
         _op_check(lib.laya_gpu_rope_plan(head_dim, head_dim if rot_dim is None else rot_dim, theta,
                                          ROPE_LAYOUTS[layout], factor, original_len, beta_fast, beta_slow, magnitude,
@@ -470,6 +477,7 @@ def rope(plan: RopePlan, x_ptr: int, x_stride: int, y_ptr: int, y_stride: int, n
          dtype: str = "BF16", stream: int = 0) -> None:
     """Rotate `heads` adjacent heads of every row (queries and keys side by
     side in a packed projection, say); inverse=True is the gradient."""
+    _fits("rope", 0, n_tokens, heads, n_seqs)
     _op_check(lib.laya_gpu_rope(ctypes.byref(plan.c), x_ptr or None, x_stride, y_ptr or None, y_stride, n_tokens,
                                 heads, cu_seqlens_ptr or None, n_seqs, positions_ptr or None, int(inverse), DT[dtype],
                                 status_ptr or None, stream or None))
@@ -481,6 +489,7 @@ class AttentionShape:
     def __init__(self, cu_seqlens_ptr: int, n_seqs: int, n_tokens: int, max_len: int, n_heads: int, n_kv_heads: int,
                  status_ptr: int, window: int = -1, scale: float = 0.125, dtype: str = "BF16",
                  token_mask_ptr: int = 0):
+        _fits("attention", window, n_seqs, n_tokens, max_len, n_heads, n_kv_heads)
         self.c = _Attention(cu_seqlens_ptr or None, token_mask_ptr or None, status_ptr or None, n_seqs, n_tokens,
                             max_len, n_heads, n_kv_heads, window, scale, DT[dtype])
 
@@ -522,6 +531,7 @@ class PolicyBatch:
     def __init__(self, cu_options_ptr: int, n_decisions: int, n_options: int, max_options: int, status_ptr: int,
                  qtypes_ptr: int = 0, temperature: Sequence[float] = (1.0, 1.0, 1.0), clip_low: float = 0.2,
                  clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0, dtype: str = "F32"):
+        _fits("policy_loss", 0, n_decisions, n_options, max_options)
         self.c = _Policy(cu_options_ptr or None, qtypes_ptr or None, status_ptr or None, n_decisions, n_options,
                          max_options, (ctypes.c_float * 3)(*temperature), clip_low, clip_high, kl_coef, entropy_coef,
                          DT[dtype])
