@@ -270,8 +270,9 @@ LAYA_API int laya_gpu_linear(const void* x, const void* w, const float* bias, fl
  * keeps nothing that a gradient needs. The calls below are the same
  * operators by themselves, with their gradients, over rows that the caller
  * holds: rotary positions, packed attention with its statistics and its
- * backward pass, and the policy loss over a decision's options. They need no
- * context. Each runs on `stream` (NULL = the legacy default stream) of the
+ * backward pass, and the policy loss over a decision's options. The rest of
+ * such a step (the gradients of projections, norms, MLP, embedding and heads,
+ * the optimizer) is the caller's. They need no context. Each runs on `stream` (NULL = the legacy default stream) of the
  * current device, allocates nothing, never synchronises, keeps no state
  * between calls, and may be captured into a CUDA graph; calls on different
  * streams share nothing unless the caller hands them the same buffers. Every
@@ -302,7 +303,8 @@ LAYA_API int laya_gpu_op_status(int32_t* status, void* stream);
  * divided by `factor` (>= 1) to reach longer contexts; with original_len >
  * 0 only as far as the pair turns seldom within it: with r = original_len *
  * f_i / (2 pi) turns and g = clamp((r - beta_slow) / (beta_fast -
- * beta_slow), 0, 1), f_i becomes f_i (g + (1 - g) / factor). */
+ * beta_slow), 0, 1), f_i becomes f_i (g + (1 - g) / factor): a ramp over the
+ * number of turns, not over the pair's index. */
 typedef enum {
     LAYA_ROPE_HALF = 0,        /* pair i = elements i and i + rot_dim / 2 */
     LAYA_ROPE_INTERLEAVED = 1, /* pair i = elements 2i and 2i + 1 */
@@ -348,7 +350,12 @@ LAYA_API int laya_gpu_rope(const laya_rope_plan* plan, const void* x, int64_t x_
  * absent (a padded batch's filler): no query sees it, its own out row is 0,
  * its lse -inf, its gradients 0, and whatever its rows hold, NaN included,
  * is not used. So are rows outside their sequence. The values of present
- * tokens should be finite: a NaN reaches every row whose tile holds it. */
+ * tokens should be finite: a NaN reaches every row whose tile holds it.
+ * Scores, statistics and sums are f32; the probabilities and, in the backward
+ * pass, dS are rounded to elem_dtype as operands of the products that follow
+ * (out and gradients are about 1.4 times as far off as f32 arithmetic rounded
+ * once). In F16 that asks for a loss scale: dS below 2^-24 is 0 there, above
+ * 65,504 infinite. */
 #define LAYA_HEAD_DIM 64
 
 typedef struct {

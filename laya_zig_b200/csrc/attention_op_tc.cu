@@ -34,11 +34,11 @@
 // sub-partition, and what bounds the kernels is the latency of these warps'
 // dependent steps (TMEM load, ex2, pack, TMEM store, barrier) more than any
 // unit: on one sequence of 8,192 tokens, 12 heads, the SFU is busy 64 % of the
-// forward's time (512 cycles of ex2 for a 128 x 64 tile), 53 % of dQ's and 46 %
-// of dK/dV's, the tensor cores 32, 39 and 46 %, and issue slots 54 % at most.
-// There the forward takes 340 us (606 TFLOP/s) and the backward 790 (652 over
-// the five products needed, 913 over the seven that it does); 64 sequences of
-// 175-180 tokens 31 and 72 us, where an item has three tiles: of an item's 10,500
+// forward's time (512 cycles of ex2 for a 128 x 64 tile) and 51 % of the backward's,
+// the tensor cores 32 and 45 %, and issue slots 54 % at most.
+// There the forward takes 345 us (597 TFLOP/s) and the backward 800 (644 over
+// the five products needed, 901 over the seven that it does); 64 sequences of
+// 175-180 tokens 31 and 73 us, where an item has three tiles: of an item's 10,500
 // cycles in dK/dV these take 6,000, waiting for the accumulators 800, storing them
 // 2,500 and the next item's beginning 600 (forward: 6,200, of them 3,500 in tiles);
 // 2 of 16,000 with a window of 64 (forward) 71 us. The mma.sync kernels took 3,619
@@ -937,7 +937,7 @@ __device__ __forceinline__ void dkv_pass(const Frame& f, const CUtensorMap& mq, 
 // key head's item goes through the queries of its whole group. (As two launches,
 // the second one's CTAs in the places of the first's, dQ first unless heads are
 // shared: 64 x 175-180 tokens, 12 heads 76 us instead of 72, 128 x 1-512, 12 heads
-// over 4 288 instead of 284, one sequence of 8,192 760 instead of 790; but there the
+// over 4 288 instead of 284, one sequence of 8,192 760 instead of 800; but there the
 // second launch has no wait of its own behind which delta is known to be complete.)
 using Bwd = Shape<2, 4 * ROWS, 2>;
 

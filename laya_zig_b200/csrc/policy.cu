@@ -19,10 +19,11 @@
 // after the first time from cache.
 //
 // The bytes are logits, reference and gradient once each. On the device, f32
-// with a reference: 64 decisions of 4 options 1.8 us, a launch; 65,536 of 4 to
-// 16 (10.5 MB) 5.7 us, 1.8 TB/s; bf16, 16,384 of 1 to 1,024 (51 MB) 48 us, 1.1
-// TB/s, bound by instructions (630 a warp, 3.1 of 4 a cycle issued): some 50 an
-// option, and as many again a decision for its scalars and three reductions.
+// with a reference: 64 decisions of 4 options 2.0 us, a launch; 65,536 of 4 to
+// 16 (10.5 MB) 8.4 us, 1.3 TB/s (6.0 from L2); bf16, 16,384 of 1 to 1,024 (51 MB) 50
+// us, 1.0 TB/s (42 from L2), bound by instructions (649 a warp, 3.1 of 4 a cycle issued): about half for
+// the decision's scalars and three reductions over a block, however few its options,
+// and some 70 for each of the four that a thread has on average.
 #include "operators.cuh"
 
 namespace laya {
