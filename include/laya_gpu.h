@@ -354,8 +354,8 @@ LAYA_API int laya_gpu_rope(const laya_rope_plan* plan, const void* x, int64_t x_
  * Scores, statistics and sums are f32; the probabilities and, in the backward
  * pass, dS are rounded to elem_dtype as operands of the products that follow
  * (out and gradients are about 1.4 times as far off as f32 arithmetic rounded
- * once). In F16 that asks for a loss scale: dS below 2^-24 is 0 there, above
- * 65,504 infinite. */
+ * once). In F16 that asks for a loss scale: dS loses digits below 2^-14 there,
+ * is 0 from 2^-25 down and infinite above 65,504. */
 #define LAYA_HEAD_DIM 64
 
 typedef struct {

@@ -684,83 +684,83 @@ __device__ __forceinline__ void one_block(const AttnArgs& a, const SeqTile& t, i
     __shared__ uint32_t bits[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float sl2 = a.scale * LOG2E;
-            const int n = (t.len + 15) >> 4;
-            const int i0 = warp * 16 + (lane >> 2), i1 = i0 + 8;  // this thread's queries, then keys
-            const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
-            load_tile(sk, a.io.k, hk, a, t, 0, n);
-            load_tile(sv, a.io.v, hk, a, t, 0, n);
-            key_bits(bits, a, t, 0);
-            float dk[8][4], dv[8][4];
-            if (SHARED) {
-                clear(dk);
-                clear(dv);
+    const int n = (t.len + 15) >> 4;
+    const int i0 = warp * 16 + (lane >> 2), i1 = i0 + 8;  // this thread's queries, then keys
+    const bool p0 = present(a, t, i0), p1 = present(a, t, i1);
+    load_tile(sk, a.io.k, hk, a, t, 0, n);
+    load_tile(sv, a.io.v, hk, a, t, 0, n);
+    key_bits(bits, a, t, 0);
+    float dk[8][4], dv[8][4];
+    if (SHARED) {
+        clear(dk);
+        clear(dv);
+    }
+    int h = hk * a.group;
+    do {
+        load_tile(sq, a.io.q, h, a, t, 0, n);
+        load_tile(sdo, a.io.dout, h, a, t, 0, n);
+        copy_commit();
+        const float* lse = a.io.lse + (long long)h * a.n_tokens + t.start;
+        const float e0 = p0 ? lse[i0] * LOG2E : 0.f, e1 = p1 ? lse[i1] * LOG2E : 0.f;
+        copy_wait<0>();
+        __syncthreads();
+        float dp[8][4];  // later dQ
+        if (warp < n) {
+            uint32_t f[4][4];
+            float s[8][4];
+            load_a(f, sq, warp, lane);
+            mma_nt<T>(s, f, sk, lane, n);
+            load_a(f, sdo, warp, lane);
+            mma_nt<T>(dp, f, sv, lane, n);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    s[j][e] = ex2_approx(fmaf(s[j][e], sl2, -e0));
+                    s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -e1));
+                }
+            hide(s, bits[0] | (uint64_t)bits[1] << 32, a.window, i0, i1, lane, 0.f);
+            float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    d0 = fmaf(s[j][e], dp[j][e], d0);
+                    d1 = fmaf(s[j][2 + e], dp[j][2 + e], d1);
+                }
+            put_rows<T>(sp, s, warp, lane);
+#pragma unroll
+            for (int x = 1; x < 4; x *= 2) {
+                d0 += __shfl_xor_sync(0xffffffffu, d0, x);
+                d1 += __shfl_xor_sync(0xffffffffu, d1, x);
             }
-            int h = hk * a.group;
-            do {
-                load_tile(sq, a.io.q, h, a, t, 0, n);
-                load_tile(sdo, a.io.dout, h, a, t, 0, n);
-                copy_commit();
-                const float* lse = a.io.lse + (long long)h * a.n_tokens + t.start;
-                const float e0 = p0 ? lse[i0] * LOG2E : 0.f, e1 = p1 ? lse[i1] * LOG2E : 0.f;
-                copy_wait<0>();
-                __syncthreads();
-                float dp[8][4];  // later dQ
-                if (warp < n) {
-                    uint32_t f[4][4];
-                    float s[8][4];
-                    load_a(f, sq, warp, lane);
-                    mma_nt<T>(s, f, sk, lane, n);
-                    load_a(f, sdo, warp, lane);
-                    mma_nt<T>(dp, f, sv, lane, n);
-    #pragma unroll
-                    for (int j = 0; j < 8; j++)
-    #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            s[j][e] = ex2_approx(fmaf(s[j][e], sl2, -e0));
-                            s[j][2 + e] = ex2_approx(fmaf(s[j][2 + e], sl2, -e1));
-                        }
-                    hide(s, bits[0] | (uint64_t)bits[1] << 32, a.window, i0, i1, lane, 0.f);
-                    float d0 = 0.f, d1 = 0.f;
-    #pragma unroll
-                    for (int j = 0; j < 8; j++)
-    #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            d0 = fmaf(s[j][e], dp[j][e], d0);
-                            d1 = fmaf(s[j][2 + e], dp[j][2 + e], d1);
-                        }
-                    put_rows<T>(sp, s, warp, lane);
-    #pragma unroll
-                    for (int x = 1; x < 4; x *= 2) {
-                        d0 += __shfl_xor_sync(0xffffffffu, d0, x);
-                        d1 += __shfl_xor_sync(0xffffffffu, d1, x);
-                    }
-    #pragma unroll
-                    for (int j = 0; j < 8; j++)
-    #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            s[j][e] *= dp[j][e] - d0;
-                            s[j][2 + e] *= dp[j][2 + e] - d1;
-                        }
-                    put_rows<T>(sds, s, warp, lane);
-                    clear(dp);
-                    mma_nn<T>(dp, s, sk, lane, n);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    s[j][e] *= dp[j][e] - d0;
+                    s[j][2 + e] *= dp[j][2 + e] - d1;
                 }
-                __syncthreads();
-                if (warp < n) store_rows<T>(sdq, a.io.dq, h, t, 0, warp, lane, dp, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
-                if (!SHARED) {
-                    clear(dk);
-                    clear(dv);
-                }
-                if (warp < n) {
-                    mma_tn<T>(dv, sp, sdo, warp, lane, n);
-                    mma_tn<T>(dk, sds, sq, warp, lane, n);
-                }
-                __syncthreads();
-            } while (SHARED && ++h < (hk + 1) * a.group);
-            if (warp < n) {
-                store_rows<T>(sds, a.io.dk, hk, t, 0, warp, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
-                store_rows<T>(sp, a.io.dv, hk, t, 0, warp, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
-            }
+            put_rows<T>(sds, s, warp, lane);
+            clear(dp);
+            mma_nn<T>(dp, s, sk, lane, n);
+        }
+        __syncthreads();
+        if (warp < n) store_rows<T>(sdq, a.io.dq, h, t, 0, warp, lane, dp, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+        if (!SHARED) {
+            clear(dk);
+            clear(dv);
+        }
+        if (warp < n) {
+            mma_tn<T>(dv, sp, sdo, warp, lane, n);
+            mma_tn<T>(dk, sds, sq, warp, lane, n);
+        }
+        __syncthreads();
+    } while (SHARED && ++h < (hk + 1) * a.group);
+    if (warp < n) {
+        store_rows<T>(sds, a.io.dk, hk, t, 0, warp, lane, dk, p0 ? a.scale : 0.f, p1 ? a.scale : 0.f);
+        store_rows<T>(sp, a.io.dv, hk, t, 0, warp, lane, dv, p0 ? 1.f : 0.f, p1 ? 1.f : 0.f);
+    }
 }
 
 template <typename T, bool SHARED>

@@ -12,7 +12,9 @@
 // its lanes take a pair each for the table (in shared memory) and then 16
 // bytes each of the row. Bound by memory: 64 sequences of 175-180 tokens, 24
 // heads of 64, bf16 (70 MB) 14.9 us, 4.7 TB/s; 32,768 tokens with 32 of 64
-// elements rotated, f16 (201 MB) 33.7 us, 6.0 TB/s; one sequence of 64 tokens
+// elements rotated, f16 (201 MB) 33.7 us, 6.0 TB/s; the former in f32 (139 MB) 23.2
+// us, 6.0 TB/s, in place 15.1 us, with a position a row 14.0; rows that are not 16-byte
+// aligned, an element at a time, 41 us; one sequence of 64 tokens
 // 2.5 us. The first pieces are loaded before the search of the position and
 // the table, which leave the memory idle at a call's beginning and end; set up
 // while the kernel before ends, calls in a row take 14.8 instead of 16.4 us and 34.9
